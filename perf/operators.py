@@ -160,7 +160,7 @@ class _Handle:
         c = self.lib.tg_kv_create_ex(capacity, kv_heads, head_dim, 1 if dtype == torch.bfloat16 else 0)
         assert c, self.lib.tg_kv_last_error()
         self.caches.append(c)
-        view = _tensor(self.lib.tg_kv_device_handle(c), (2, capacity, kv_heads * head_dim), dtype)
+        view = _tensor(self, self.lib.tg_kv_device_handle(c), (2, capacity, kv_heads * head_dim), dtype)
         if rows is not None:
             view[:, :rows.shape[1]] = rows
             self.lib.tg_kv_advance(c, rows.shape[1])
@@ -175,15 +175,18 @@ class _Handle:
 
 
 class _Memory:
-    def __init__(self, address, shape, kind):
+    """Part of a cache as torch sees it; keeps the owner, so that a tensor outlives its state."""
+
+    def __init__(self, owner, address, shape, kind):
+        self.owner = owner
         self.__cuda_array_interface__ = {"data": (address, False), "shape": shape, "typestr": kind, "version": 3}
 
 
-def _tensor(address, shape, dtype):
-    """Device memory as a tensor, without a copy."""
+def _tensor(owner, address, shape, dtype):
+    """Device memory of `owner` as a tensor, without a copy."""
     if dtype == torch.bfloat16:
-        return torch.as_tensor(_Memory(address, shape, "<i2"), device=DEV).view(torch.bfloat16)
-    return torch.as_tensor(_Memory(address, shape, "<f4"), device=DEV)
+        return torch.as_tensor(_Memory(owner, address, shape, "<i2"), device=DEV).view(torch.bfloat16)
+    return torch.as_tensor(_Memory(owner, address, shape, "<f4"), device=DEV)
 
 
 def _library():
