@@ -184,6 +184,53 @@ int tg_cuda_kv_rope_append(int dtype, const float* qkv, const float* cs, const f
                            uint32_t n_kv_heads, uint32_t head_dim, uint32_t start_pos,
                            uint32_t max_seq, void* stream);
 
+/* ---- row moves and groups of caches (include/tgai_kv_group.h) ------------ */
+
+/* A cache buffer [2][max_seq][row]. */
+typedef struct {
+    uint64_t base;
+    uint64_t max_seq;
+} TGCudaRowCache;
+
+/* The current device (-1 if the runtime cannot tell). */
+int tg_cuda_kv_device(void);
+
+/* Rows [0, n_rows) of src[i] into dst[i * fan + j], j < fan.  row_bytes: one K
+ * row, a multiple of 16; buffers 16-byte aligned and disjoint.
+ * n_src * fan <= 1024. */
+int tg_cuda_kv_fork_rows(const TGCudaRowCache* src, uint32_t n_src, const TGCudaRowCache* dst,
+                         uint32_t fan, uint64_t row_bytes, uint32_t n_rows, void* stream);
+
+/* In-place compaction of n <= 1024 caches to n_ranges <= 1024 ascending,
+ * disjoint, non-empty ranges of rows. */
+int tg_cuda_kv_compact_rows(const TGCudaRowCache* caches, uint32_t n, uint64_t row_bytes,
+                            const uint32_t* start, const uint32_t* count, uint32_t n_ranges,
+                            void* stream);
+
+/* Device table of a group: its n sequences' caches, then the prefix cache
+ * (base 0: none).  bf16, head_dim 64 or 128.  Blocks; free with
+ * tg_cuda_kv_free. */
+void* tg_cuda_kv_group_table(const TGCudaRowCache* caches, uint32_t n, uint32_t n_kv_heads,
+                             uint32_t head_dim);
+
+/* One group call: n_new[i] queries of sequence i, after n_new[i] rows of
+ * k_new / v_new (or NULL: they are there) went to rows old_len[i] .. of its
+ * cache. */
+typedef struct {
+    int      act;                   /* 0 fp32, 1 bf16: q, k_new, v_new, out */
+    uint32_t n_seq, n_heads, n_kv_heads, head_dim;
+    uint32_t prefix_len;
+    const void*     table_dev;      /* tg_cuda_kv_group_table */
+    const uint32_t* old_len;        /* host [n_seq] */
+    const uint32_t* n_new;          /* host [n_seq] */
+    const void* q;
+    const void* k_new;
+    const void* v_new;
+    void*       out;
+    float       scale;              /* softmax scale */
+} TGCudaGroupCall;
+int tg_cuda_kv_group_attention(const TGCudaGroupCall* c, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,316 @@
+"""Groups of caches on the GPU: decode over a shared prefix, packed prompts,
+fork and compaction, against plain 64-bit forms.
+
+Rows behind a cache's length hold NaN, Inf or huge values (what a truncated
+turn may leave), so every result also shows that they take no part.  The
+tolerances are the roundings the kernels make (group_model.py), element by
+element.
+"""
+import numpy as np
+import pytest
+
+import tgkv
+from conftest import rel_head_err
+from group_model import bf16, group_reference
+
+pytestmark = pytest.mark.gpu
+
+F32, BF16 = tgkv.TG_KV_F32, tgkv.TG_KV_BF16
+C = tgkv.C
+
+
+def put(lib, c, dtype, cap, kvd, rows, junk):
+    """The whole buffer of cache c: `rows` [2][n][kvd], then junk rows."""
+    n = rows.shape[1]
+    full = np.empty((2, cap, kvd), np.float32)
+    full[:, :n] = rows
+    full[:, n:] = np.resize(np.array(junk, np.float32), (2, cap - n, kvd))
+    raw = bf16(full)[0] if dtype == BF16 else full
+    assert lib.tg_cuda_kv_h2d(lib.tg_kv_device_handle(c), raw.ctypes.data, raw.nbytes, None)
+    lib.tg_kv_reset(c)
+    lib.tg_kv_advance(c, n)
+    return raw
+
+
+def get(lib, c, dtype, cap, kvd):
+    raw = np.empty(lib.tg_kv_bytes(c), np.uint8)
+    tgkv.check(lib.tg_kv_download(c, raw.ctypes.data), lib)
+    return raw.view(np.uint16 if dtype == BF16 else np.float32).reshape(2, cap, kvd)
+
+
+JUNK = [np.nan, np.inf, -np.inf, 3e38, -1.0]
+
+
+class Setup:
+    """n caches with old[i] rows each (and a prefix of P), a group over them."""
+
+    def __init__(self, lib, old, room, P, nh, nkv, hd, act, seed=0, mscale=None):
+        self.lib, self.nh, self.nkv, self.hd, self.act, self.P = lib, nh, nkv, hd, act, P
+        self.rng = np.random.default_rng(seed)
+        self.kvd, self.q_scale = nkv * hd, 1
+        self.old, self.cap = list(old), [o + r for o, r in zip(old, room)]
+        self.rows, self.caches = [], []
+        for o, cap in zip(self.old, self.cap):
+            self._cache(cap, o)
+        self.prefix = None
+        if P is not None:
+            self._cache(P + 5, P)
+            self.prefix, self.prefix_rows = self.caches.pop(), self.rows.pop()
+        scale = hd ** -0.5
+        if mscale is not None:
+            scale *= mscale
+            for c in self.caches + [self.prefix] * (P is not None):
+                lib.tg_kv_set_attn_mscale(c, mscale)
+        self.scale = float(np.float32(scale))
+        self.arr = (C.c_void_p * len(old))(*self.caches)
+        self.g = lib.tg_kv_group_create(self.prefix, self.arr, len(old), nh, act)
+        tgkv.check(self.g, lib, "group")
+
+    def _cache(self, cap, n):
+        c = self.lib.tg_kv_create_ex(cap, self.nkv, self.hd, BF16)
+        tgkv.check(c, self.lib)
+        x = self.rng.standard_normal((2, n, self.kvd))
+        put(self.lib, c, BF16, cap, self.kvd, x, JUNK)
+        self.caches.append(c)
+        self.rows.append(bf16(x)[1])
+
+    def new(self, total):
+        """q, k, v of `total` tokens: (device-ready array, float64 value) each."""
+        got = []
+        for cols, mul in ((self.nh * self.hd, self.q_scale), (self.kvd, 1), (self.kvd, 1)):
+            x = (mul * self.rng.standard_normal((total, cols))).astype(np.float32)
+            b, v = bf16(x)
+            got.append((b, v) if self.act == BF16 else (x, x.astype(np.float64)))
+        return got
+
+    def expect(self, q, n_new):
+        """The reference for the rows as they are in self.rows now."""
+        def heads(r):
+            return r[0].reshape(-1, self.nkv, self.hd), r[1].reshape(-1, self.nkv, self.hd)
+        pre = heads(self.prefix_rows) if self.P else None
+        return group_reference(q.reshape(-1, self.nh, self.hd), pre, [heads(r) for r in self.rows], n_new, self.nkv,
+                               self.scale, self.act == BF16)
+
+    def grow(self, n_new, k, v):
+        at = 0
+        for i, t in enumerate(n_new):
+            add = np.stack([bf16(k[at:at + t])[1], bf16(v[at:at + t])[1]])
+            self.rows[i] = np.concatenate([self.rows[i], add], 1)
+            at += t
+
+    def read(self, buf, total):
+        if self.act == BF16:
+            import oracle as O
+            return O.bf16_to_f32(buf.get(np.uint16, (total, self.nh, self.hd))).astype(np.float64)
+        return buf.get(np.float32, (total, self.nh, self.hd)).astype(np.float64)
+
+    def check_caches(self):
+        """Every cache holds its rows, and what lay behind them as it was."""
+        for c, cap, r in zip(self.caches, self.cap, self.rows):
+            n = r.shape[1]
+            assert self.lib.tg_kv_len(c) == n
+            raw = get(self.lib, c, BF16, cap, self.kvd)
+            assert np.array_equal(raw[:, :n], bf16(r)[0])
+
+    def close(self):
+        self.lib.tg_kv_group_destroy(self.g)
+        for c in self.caches + [self.prefix] * (self.prefix is not None):
+            self.lib.tg_kv_destroy(c)
+
+
+def call(s, devbuf, n_new, append=True, decode=False, stream=None):
+    """One call on fresh tokens; checks outputs, caches and what lies behind out."""
+    lib, total = s.lib, sum(n_new)
+    (qb, q), (kb, k), (vb, v) = s.new(total)
+    if append:
+        s.grow(n_new, k, v)
+    qd, kd, vd = devbuf(qb), devbuf(kb), devbuf(vb)
+    guard = np.full(qb.size + 4096, 0x55, qb.dtype)
+    od = devbuf(guard)
+    ptrs = (qd.ptr, kd.ptr if append else None, vd.ptr if append else None, od.ptr, stream)
+    if decode:
+        tgkv.check(lib.tg_kv_group_decode(s.g, *ptrs), lib, "decode")
+    else:
+        tgkv.check(lib.tg_kv_group_prompt(s.g, (C.c_uint32 * len(n_new))(*n_new), *ptrs), lib, "prompt")
+    assert lib.tg_cuda_kv_sync(stream)
+    got = s.read(od, total)
+    assert np.all(od.get(qb.dtype, guard.shape)[qb.size:] == 0x55)
+    want, tol = s.expect(q, n_new)
+    bad = ~(np.abs(got - want) <= tol)
+    assert not bad.any(), (np.argwhere(bad)[:5], got[bad][:5], want[bad][:5], tol[bad][:5])
+    s.check_caches()
+    assert lib.tg_cuda_kv_device_error() == 0
+    return got
+
+
+DECODE = [  # old lengths, prefix (None: no cache), heads, kv heads, head_dim
+    ([0], None, 1, 1, 64),
+    ([0], 0, 4, 2, 128),
+    ([0, 1, 5], 1, 8, 8, 64),
+    ([127, 128, 129, 0, 63], 127, 16, 4, 128),
+    ([300, 31, 2], 128, 12, 4, 128),
+    ([500] * 9, 129, 32, 8, 128),
+    ([1, 700, 40], 1000, 7, 1, 64),
+    (list(range(0, 140, 2)), 640, 16, 2, 128),
+    ([2000], 3001, 128, 1, 64),
+    ([17] * 40, 4000, 6, 3, 64),
+]
+
+
+@pytest.mark.parametrize("act", [F32, BF16])
+@pytest.mark.parametrize("case", range(len(DECODE)))
+def test_decode(cuda, devbuf, case, act):
+    old, P, nh, nkv, hd = DECODE[case]
+    s = Setup(cuda, old, [4] * len(old), P, nh, nkv, hd, act, seed=case)
+    ones = [1] * len(old)
+    call(s, devbuf, ones, decode=True)
+    call(s, devbuf, ones, decode=True)                       # the second step reads the first one's row
+    call(s, devbuf, ones, decode=True, append=False)         # other queries of the same last rows
+    tgkv.check(cuda.tg_kv_group_truncate(s.g, (C.c_uint32 * len(old))(*old)), cuda)
+    s.rows = [r[:, :o] for r, o in zip(s.rows, old)]
+    s.check_caches()
+    call(s, devbuf, ones, decode=True)
+    s.close()
+
+
+PROMPT = [  # old lengths, new tokens, prefix, heads, kv heads, head_dim
+    ([0], [1], None, 1, 1, 64),
+    ([0], [130], None, 2, 2, 128),
+    ([0, 0, 0], [1, 5, 17], 0, 8, 8, 64),
+    ([40, 129, 0, 7], [0, 3, 64, 0], 100, 16, 4, 128),
+    ([300, 0, 77], [200, 129, 1], None, 12, 4, 128),
+    ([0, 500], [257, 128], 383, 32, 8, 128),
+    ([10] * 12, [2, 9, 1, 4, 31, 8, 1, 1, 3, 5, 6, 7], 700, 16, 2, 128),
+    ([0, 20], [70, 33], 65, 7, 1, 64),
+    ([1500], [600], 900, 4, 1, 64),
+    ([0, 0], [3, 2], 50, 128, 1, 128),
+]
+
+
+@pytest.mark.parametrize("act", [F32, BF16])
+@pytest.mark.parametrize("case", range(len(PROMPT)))
+def test_prompt(cuda, devbuf, case, act):
+    old, new, P, nh, nkv, hd = PROMPT[case]
+    s = Setup(cuda, old, [n + 3 for n in new], P, nh, nkv, hd, act, seed=50 + case)
+    call(s, devbuf, new)
+    call(s, devbuf, new, append=False)                       # other queries of the rows just appended
+    call(s, devbuf, [1] * len(old), decode=True)
+    s.close()
+
+
+def test_scale_with_mscale(cuda, devbuf):
+    s = Setup(cuda, [200, 3], [8, 8], 150, 8, 2, 128, F32, seed=7, mscale=1.37)
+    call(s, devbuf, [5, 2])
+    call(s, devbuf, [1, 1], decode=True)
+    s.close()
+
+
+@pytest.mark.parametrize("act", [F32, BF16])
+def test_large_scores(cuda, devbuf, act):
+    """Scores in the hundreds: one key takes nearly all the weight."""
+    s = Setup(cuda, [260, 140], [8, 8], 300, 8, 2, 128, act, seed=9)
+    s.q_scale = 40
+    call(s, devbuf, [2, 1])
+    s.close()
+
+
+def test_matches_the_single_cache_operators(cuda, devbuf):
+    """The same history in one plain cache: tg_kv_append_attention and tg_kv_attention agree."""
+    lib, nh, nkv, hd, P = cuda, 16, 4, 128, 200
+    s = Setup(lib, [90, 0], [300, 300], P, nh, nkv, hd, F32, seed=21)
+    for n_new in ([150, 70], [1, 1]):
+        (qb, q), (kb, k), (vb, v) = s.new(sum(n_new))
+        before = [r.copy() for r in s.rows]
+        s.grow(n_new, k, v)
+        qd, kd, vd, od = devbuf(qb), devbuf(kb), devbuf(vb), devbuf(nbytes=qb.nbytes)
+        tgkv.check(lib.tg_kv_group_prompt(s.g, (C.c_uint32 * 2)(*n_new), qd.ptr, kd.ptr, vd.ptr, od.ptr, None), lib)
+        got, at = s.read(od, sum(n_new)), 0
+        for i, t in enumerate(n_new):
+            one = lib.tg_kv_create_ex(1000, nkv, hd, BF16)
+            put(lib, one, BF16, 1000, s.kvd, np.concatenate([s.prefix_rows, before[i]], 1), JUNK)
+            part = [devbuf(np.ascontiguousarray(x[at:at + t])) for x in (kb, vb, qb)]
+            o1 = devbuf(nbytes=t * nh * hd * 4)
+            tgkv.check(lib.tg_kv_append_attention(one, part[0].ptr, part[1].ptr, part[2].ptr, o1.ptr, nh, t, None), lib)
+            assert lib.tg_cuda_kv_sync(None)
+            # both sit within 5e-5 of the head's output scale of the 64-bit value
+            assert rel_head_err(got[at:at + t], o1.get(np.float32, (t, nh, hd))) < 1e-4
+            lib.tg_kv_destroy(one)
+            at += t
+    s.close()
+
+
+# ------------------------------------------------------------- row moves
+FORK = [(1, 1, 1, 1, 64, F32), (1, 3, 37, 2, 64, F32), (3, 2, 1000, 4, 128, BF16), (2, 5, 513, 1, 128, F32),
+        (24, 8, 65, 3, 32, BF16), (2, 1, 0, 4, 64, BF16), (600, 1, 4, 1, 32, BF16)]
+
+
+@pytest.mark.parametrize("n_src,fan,rows,nkv,hd,dtype", FORK)
+def test_fork(cuda, n_src, fan, rows, nkv, hd, dtype):
+    lib, kvd = cuda, nkv * hd
+    rng = np.random.default_rng(rows)
+    src, dst, want, before = [], [], [], []
+    for i in range(n_src):
+        cap = rows + 1 + i % 3
+        src.append(lib.tg_kv_create_ex(cap, nkv, hd, dtype))
+        want.append(put(lib, src[-1], dtype, cap, kvd, rng.standard_normal((2, rows + 1, kvd)), JUNK))
+    for j in range(n_src * fan):
+        cap = rows + 1 + j % 2
+        dst.append(lib.tg_kv_create_ex(cap, nkv, hd, dtype))
+        before.append(put(lib, dst[-1], dtype, cap, kvd, rng.standard_normal((2, min(j % 3, cap), kvd)), JUNK))
+    tgkv.check(lib.tg_kv_fork((C.c_void_p * n_src)(*src), n_src, (C.c_void_p * len(dst))(*dst), fan, rows, None), lib)
+    assert lib.tg_cuda_kv_sync(None)
+    bits = np.uint16 if dtype == BF16 else np.uint32
+    for j, c in enumerate(dst):
+        assert lib.tg_kv_len(c) == rows
+        raw = get(lib, c, dtype, lib.tg_kv_capacity(c), kvd).view(bits)
+        assert np.array_equal(raw[:, :rows], want[j // fan].view(bits)[:, :rows])
+        assert np.array_equal(raw[:, rows:], before[j].view(bits)[:, rows:])
+    for i, c in enumerate(src):
+        assert lib.tg_kv_len(c) == rows + 1
+        assert np.array_equal(get(lib, c, dtype, lib.tg_kv_capacity(c), kvd).view(bits), want[i].view(bits))
+    for c in src + dst:
+        lib.tg_kv_destroy(c)
+
+
+COMPACT = [  # caches, rows, kv heads, head_dim, dtype, ranges
+    (1, 1, 1, 64, F32, "all"), (1, 50, 1, 64, BF16, "none"), (1, 50, 2, 64, F32, "last"),
+    (3, 700, 4, 128, BF16, "window"), (1, 20000, 8, 128, BF16, "window"), (2, 5000, 8, 64, F32, 300),
+    (24, 900, 4, 128, BF16, 40), (1, 9001, 1, 128, BF16, 1024), (1, 30000, 3, 32, F32, 7),
+    (2, 333, 5, 64, BF16, "shift"), (1, 4096, 4, 128, BF16, "halves"), (1, 300, 1, 8, BF16, 9),
+]
+
+
+@pytest.mark.parametrize("n,rows,nkv,hd,dtype,kind", COMPACT)
+def test_compact(cuda, n, rows, nkv, hd, dtype, kind):
+    lib, kvd, cap = cuda, nkv * hd, rows + 3
+    rng = np.random.default_rng(rows + n)
+    if kind == "all":
+        start, count = [0], [rows]
+    elif kind == "none":
+        start, count = [], []
+    elif kind == "last":
+        start, count = [rows - 1], [1]
+    elif kind == "window":                                   # 4 sinks and the last third
+        start, count = [0, rows - rows // 3], [4, rows // 3]
+    elif kind == "shift":                                    # everything moves by one row
+        start, count = [1], [rows - 1]
+    elif kind == "halves":                                   # adjoining ranges, nothing dropped between
+        start, count = [1, 101, 2000], [100, 1899, rows - 2000]
+    else:
+        cuts = np.sort(rng.choice(rows + 1, 2 * kind, replace=False))
+        start, count = list(cuts[0::2]), list(cuts[1::2] - cuts[0::2])
+    index = np.concatenate([np.arange(a, a + c) for a, c in zip(start, count)] + [np.arange(0)]).astype(int)
+    caches, before = [], []
+    for i in range(n):
+        caches.append(lib.tg_kv_create_ex(cap, nkv, hd, dtype))
+        before.append(put(lib, caches[-1], dtype, cap, kvd, rng.standard_normal((2, rows, kvd)), JUNK))
+    tgkv.check(lib.tg_kv_compact((C.c_void_p * n)(*caches), n, (C.c_uint32 * len(start))(*start),
+                                 (C.c_uint32 * len(start))(*count), len(start), None), lib)
+    assert lib.tg_cuda_kv_sync(None)
+    bits = np.uint16 if dtype == BF16 else np.uint32
+    for c, b in zip(caches, before):
+        assert lib.tg_kv_len(c) == len(index)
+        raw = get(lib, c, dtype, cap, kvd).view(bits)
+        assert np.array_equal(raw[:, :len(index)], b.view(bits)[:, index])
+        assert np.array_equal(raw[:, len(index):], b.view(bits)[:, len(index):])   # the rest as it was
+        lib.tg_kv_destroy(c)

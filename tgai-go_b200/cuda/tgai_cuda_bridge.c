@@ -1,6 +1,6 @@
 /* tgai_cuda_bridge.c -- thin C layer from TGAI GO host code to CUDA for the
  * KV-cache path.  Plain C (C11); talks to the CUDA runtime and to the kernel
- * launchers of tgkv_kernels.cu, nothing else.
+ * launchers of the .cu files, nothing else.
  *
  * Host-side planning of split-sequence attention lives here: the per-item
  * position counts, the chunk length and the chunk prefix table are computed
@@ -918,4 +918,167 @@ int tg_cuda_kv_rope_append(int dtype, const float* qkv, const float* cs, const f
     p.max_seq = max_seq;
     p.dtype = dtype;
     return launch_rc(tgkv_launch_rope_append(&p, stream), "rope kernel");
+}
+
+/* ---- row moves and groups of caches -------------------------------------- */
+int tg_cuda_kv_device(void) {
+    int dev = -1;
+    return cuda_ok(cudaGetDevice(&dev), "cudaGetDevice") ? dev : -1;
+}
+
+int tg_cuda_kv_fork_rows(const TGCudaRowCache* src, uint32_t n_src, const TGCudaRowCache* dst,
+                         uint32_t fan, uint64_t row_bytes, uint32_t n_rows, void* stream) {
+    if (!src || !dst) { set_err("fork: NULL pointer"); return 0; }
+    if (row_bytes == 0 || row_bytes % 16) { set_err("fork: rows of %llu bytes", (unsigned long long)row_bytes); return 0; }
+    if (n_src == 0 || fan == 0 || (uint64_t)n_src * fan > TGKV_FORK_MAX) {
+        set_err("fork: %u sources x %u copies (1..%u in all)", n_src, fan, TGKV_FORK_MAX);
+        return 0;
+    }
+    for (uint32_t i = 0; i < n_src + n_src * fan; i++) {
+        const TGCudaRowCache* c = i < n_src ? src + i : dst + (i - n_src);
+        if (!c->base || (c->base & 15u) || n_rows > c->max_seq) {
+            set_err("fork: %s %u is not 16-byte aligned or holds fewer than %u rows",
+                    i < n_src ? "source" : "copy", i < n_src ? i : i - n_src, n_rows);
+            return 0;
+        }
+    }
+    if (!g_ready && !tg_cuda_kv_init()) return 0;
+    if (n_rows == 0) return 1;
+    static _Thread_local TGKvForkParams p;     /* 24 KB: keep off the stack */
+    const uint32_t most = TGKV_FORK_MAX / 2;
+    for (uint32_t i0 = 0; i0 < n_src; i0 += most) {
+        const uint32_t n = n_src - i0 < most ? n_src - i0 : most;
+        p.row_bytes = row_bytes;
+        p.n_vec = (uint64_t)n_rows * (row_bytes / 16);
+        p.n_src = n;
+        p.fan = fan;
+        memcpy(p.src, src + i0, n * sizeof(TGKvRowCache));
+        memcpy(p.dst, dst + (size_t)i0 * fan, (size_t)n * fan * sizeof(TGKvRowCache));
+        if (!launch_rc(tgkv_launch_fork(&p, stream), "fork kernel")) return 0;
+    }
+    return 1;
+}
+
+/* Column slices and CTAs per cluster of a compaction: a cluster serialises its
+ * slice's waves, so the slices are what runs in parallel.  Rows are cut (down
+ * to 256 bytes, two DRAM bursts of a row) until there are two CTAs of a
+ * cluster of 8 per SM; clusters shrink when a slice's rows fit fewer CTAs. */
+static void compact_shape(uint32_t n, uint64_t row_bytes, uint32_t n_move, uint32_t sms,
+                          uint32_t* n_slices, uint32_t* cluster) {
+    uint32_t s = 1;
+    while ((uint64_t)n * 2 * s * 8 < 2ull * sms && row_bytes % (2 * s * 256) == 0) s *= 2;
+    const uint64_t bytes = (uint64_t)n_move * (row_bytes / s);
+    uint32_t c = 8;
+    while (c > 1 && bytes <= (uint64_t)(c / 2) * 256 * 8 * 16) c /= 2;
+    *n_slices = s;
+    *cluster = c;
+}
+
+int tg_cuda_kv_compact_rows(const TGCudaRowCache* caches, uint32_t n, uint64_t row_bytes,
+                            const uint32_t* start, const uint32_t* count, uint32_t n_ranges,
+                            void* stream) {
+    if (!caches || (n_ranges && (!start || !count))) { set_err("compact: NULL pointer"); return 0; }
+    if (row_bytes == 0 || row_bytes % 16) { set_err("compact: rows of %llu bytes", (unsigned long long)row_bytes); return 0; }
+    if (n == 0 || n > TGKV_MAX_ITEMS || n_ranges > TGKV_MAX_ITEMS) {
+        set_err("compact: %u caches, %u ranges (at most %u of each)", n, n_ranges, TGKV_MAX_ITEMS);
+        return 0;
+    }
+    static _Thread_local TGKvCompactParams p;  /* 24 KB: keep off the stack */
+    uint64_t keep = 0, end = 0;
+    p.n_ranges = 0;
+    for (uint32_t r = 0; r < n_ranges; r++) {
+        if (count[r] == 0 || start[r] < end) {
+            set_err("compact: range %u (%u rows from %u) is empty or out of order", r,
+                    count[r], start[r]);
+            return 0;
+        }
+        if (p.n_ranges == 0 || start[r] != end) {   /* a range that continues the last one joins it */
+            p.start[p.n_ranges] = start[r];
+            p.first[p.n_ranges] = (uint32_t)keep;
+            p.n_ranges++;
+        }
+        keep += count[r];
+        end = (uint64_t)start[r] + count[r];
+    }
+    for (uint32_t i = 0; i < n; i++)
+        if (!caches[i].base || (caches[i].base & 15u) || end > caches[i].max_seq) {
+            set_err("compact: cache %u is not 16-byte aligned or holds fewer than %llu rows", i,
+                    (unsigned long long)end);
+            return 0;
+        }
+    if (!g_ready && !tg_cuda_kv_init()) return 0;
+    p.n_keep = (uint32_t)keep;
+    p.skip = 0;
+    if (p.n_ranges && p.start[0] == 0) p.skip = p.n_ranges > 1 ? p.first[1] : p.n_keep;
+    if (p.skip == p.n_keep) return 1;              /* nothing moves */
+    p.row_bytes = row_bytes;
+    p.n_caches = n;
+    memcpy(p.caches, caches, n * sizeof(TGKvRowCache));
+    uint32_t cluster;
+    compact_shape(n, row_bytes, p.n_keep - p.skip, (uint32_t)g_sm_count, &p.n_slices, &cluster);
+    return launch_rc(tgkv_launch_compact(&p, cluster, stream), "compact kernel");
+}
+
+void* tg_cuda_kv_group_table(const TGCudaRowCache* caches, uint32_t n, uint32_t n_kv_heads,
+                             uint32_t head_dim) {
+    if (!caches || n == 0 || n > TGKV_MAX_ITEMS || n_kv_heads == 0 ||
+        (head_dim != 64 && head_dim != 128)) {
+        set_err("group table: bad argument");
+        return NULL;
+    }
+    if (!g_ready && !tg_cuda_kv_init()) return NULL;
+    const size_t bytes = (size_t)(n + 1) * sizeof(TGKvRowCache);
+    void* d = tg_cuda_kv_malloc(bytes);
+    if (!d) return NULL;
+    if (!cuda_ok(cudaMemcpy(d, caches, bytes, cudaMemcpyHostToDevice), "group table h2d") ||
+        !cuda_ok(cudaStreamSynchronize(0), "group table h2d")) {
+        tg_cuda_kv_free(d);
+        return NULL;
+    }
+    return d;
+}
+
+int tg_cuda_kv_group_attention(const TGCudaGroupCall* c, void* stream) {
+    if (!c || !c->table_dev || !c->old_len || !c->n_new || !c->q || !c->out) {
+        set_err("group: NULL pointer");
+        return 0;
+    }
+    if (!c->k_new != !c->v_new) { set_err("group: k_new and v_new go together"); return 0; }
+    if (((uintptr_t)c->q | (uintptr_t)c->out | (uintptr_t)c->k_new | (uintptr_t)c->v_new) & 15u) {
+        set_err("group: q, k_new, v_new and out must be 16-byte aligned");
+        return 0;
+    }
+    if (c->n_seq == 0 || c->n_seq > TGKV_MAX_ITEMS || c->n_kv_heads == 0 || c->n_heads == 0 ||
+        c->n_heads % c->n_kv_heads || c->n_heads / c->n_kv_heads > 128 ||
+        (c->head_dim != 64 && c->head_dim != 128) || (c->act != 0 && c->act != 1)) {
+        set_err("group: no kernel for %u/%u heads of %u, %u sequences, activations of type %d",
+                c->n_heads, c->n_kv_heads, c->head_dim, c->n_seq, c->act);
+        return 0;
+    }
+    static _Thread_local TGKvGroupParams p;    /* 8 KB: keep off the stack */
+    uint64_t total = 0;
+    for (uint32_t i = 0; i < c->n_seq; i++) {
+        p.tok0[i] = (uint32_t)total;
+        p.old_len[i] = c->old_len[i];
+        total += c->n_new[i];
+        if (total * c->n_heads > 0x7fffffffull) {
+            set_err("group: too many query rows (tokens x heads above 2^31 - 1)");
+            return 0;
+        }
+    }
+    if (!g_ready && !tg_cuda_kv_init()) return 0;
+    if (total == 0) return 1;
+    p.tok0[c->n_seq] = (uint32_t)total;
+    p.table = (const TGKvRowCache*)c->table_dev;
+    p.q = c->q;
+    p.k_new = c->k_new;
+    p.v_new = c->v_new;
+    p.out = c->out;
+    p.n_seq = c->n_seq;
+    p.n_heads = c->n_heads;
+    p.n_kv_heads = c->n_kv_heads;
+    p.head_dim = c->head_dim;
+    p.prefix_len = c->prefix_len;
+    p.qscale = c->scale * 1.4426950408889634f;
+    return launch_rc(tgkv_launch_group(&p, c->act, stream), "group attention");
 }

@@ -170,6 +170,51 @@ void tgkv_prefill_f32_plan(uint32_t n_q, uint32_t pos0, uint32_t group, uint32_t
                            uint32_t sm_count, uint32_t* n_blocks, uint32_t* tps,
                            uint32_t* n_split);
 
+/* ---- row moves (tgkv_rows.cu) ---- */
+typedef struct {
+    uint64_t base;               /* device address of [2][max_seq][row] */
+    uint64_t max_seq;
+} TGKvRowCache;
+
+/* The first n_vec 16-byte vectors of K and of V of src[i] into
+ * dst[i * fan + j], j < fan. */
+#define TGKV_FORK_MAX 1024
+typedef struct {
+    uint64_t row_bytes, n_vec;
+    uint32_t n_src, fan;
+    TGKvRowCache src[TGKV_FORK_MAX / 2];
+    TGKvRowCache dst[TGKV_FORK_MAX];
+} TGKvForkParams;
+
+/* In-place compaction of n_caches caches: destination row first[r] + j takes
+ * row start[r] + j; the first `skip` rows stay where they are.  A cluster per
+ * (cache, half, column slice); row_bytes / 16 is a multiple of n_slices. */
+typedef struct {
+    uint64_t row_bytes;
+    uint32_t n_caches, n_slices, n_ranges, n_keep, skip, pad;
+    TGKvRowCache caches[TGKV_MAX_ITEMS];
+    uint32_t start[TGKV_MAX_ITEMS];
+    uint32_t first[TGKV_MAX_ITEMS];
+} TGKvCompactParams;
+
+/* ---- groups of caches with a shared prefix (tgkv_group.cu) ---- */
+typedef struct {
+    const TGKvRowCache* table;   /* device: the n_seq caches, then the prefix cache */
+    const void* q;               /* [tokens][n_heads][head_dim] */
+    const void* k_new;           /* NULL, or [tokens][kv_dim]: rows old_len[i] .. of cache i */
+    const void* v_new;
+    void*       out;             /* as q */
+    uint32_t n_seq, n_heads, n_kv_heads, head_dim;
+    uint32_t prefix_len;
+    float    qscale;             /* softmax scale * log2(e) */
+    uint32_t old_len[TGKV_MAX_ITEMS];       /* own rows before the call's tokens */
+    uint32_t tok0[TGKV_MAX_ITEMS + 1];      /* first packed token of each sequence; the total */
+} TGKvGroupParams;
+int tgkv_launch_fork(const TGKvForkParams* p, void* stream);
+int tgkv_launch_compact(const TGKvCompactParams* p, uint32_t cluster, void* stream);
+/* act: 0 fp32, 1 bf16 activations */
+int tgkv_launch_group(const TGKvGroupParams* p, int act, void* stream);
+
 /* Launchers (tgkv_kernels.cu, tgkv_prefill.cu, tgkv_prefill_f32.cu).  Return 0
  * on success, else a cudaError_t. */
 int tgkv_launch_prefill_f32(const TGKvPrefillF32Params* p, void* stream);

@@ -7,7 +7,7 @@
  * goes through tgai_gpu_dispatch.c / tgai_cuda_bridge.c; nothing here falls
  * back to the CPU.
  */
-#include "tgai_kv_cache.h"
+#include "tgai_kv_internal.h"
 #include "tgai_backend.h"
 #include "tgai_cuda_bridge.h"
 #include "tgai_gpu_dispatch.h"
@@ -18,34 +18,21 @@
 #include <stdlib.h>
 #include <string.h>
 
-struct TGKvCache {
-    uint32_t max_seq, n_kv_heads, head_dim, kv_dim;
-    int      dtype;
-    uint32_t esize;
-    size_t   bytes;               /* 2 * max_seq * kv_dim * esize */
-    void*    dev;                 /* device address of the buffer */
-    float*   host;                /* always NULL (not mappable) */
-    uint32_t len;
-    TGBackend* be;                /* backend that owns dev */
-    void*    scratch;             /* split-sequence partials */
-    uint64_t scratch_bytes;
-    uint32_t* counters;
-    uint64_t counter_slots;
-    float*   staging;             /* device staging of host rows (bf16 append) */
-    size_t   staging_bytes;
-    void*    tmap;                /* TMA tensor map of dev (NULL: no attention kernel) */
-    void*    tmap_sw;             /* swizzled map for the tensor-core suffix kernel, or NULL */
-    uint32_t* npos;               /* host item table for attention */
-    uint32_t npos_cap;
-    float    mscale;              /* YaRN temperature on the 1/sqrt(head_dim) scale */
-};
-
 static _Thread_local char t_err[256] = "kv: no error";
+
+static void set_err_v(const char* fmt, va_list ap) { vsnprintf(t_err, sizeof(t_err), fmt, ap); }
 
 static void set_err(const char* fmt, ...) {
     va_list ap;
     va_start(ap, fmt);
-    vsnprintf(t_err, sizeof(t_err), fmt, ap);
+    set_err_v(fmt, ap);
+    va_end(ap);
+}
+
+void tgkv_kv_set_err(const char* fmt, ...) {
+    va_list ap;
+    va_start(ap, fmt);
+    set_err_v(fmt, ap);
     va_end(ap);
 }
 

@@ -3,7 +3,7 @@
 This mirrors how the reference's Python layer binds its engine
 (python/tgai_go/_engine.py:344-347 declares tg_kvcache_new/free/reset and
 tg_forward with ctypes): every entry point of include/tgai_kv_cache.h,
-include/tgai_backend.h, include/tgai_gpu_dispatch.h, include/tgai_cuda_bridge.h
+include/tgai_kv_group.h, include/tgai_backend.h, include/tgai_gpu_dispatch.h, include/tgai_cuda_bridge.h
 and include/tgai_engine_bridge.h gets argtypes/restype here.  Loading fails loudly if
 the library is missing -- there is no Python or CPU fallback.
 """
@@ -109,6 +109,14 @@ PROTOS = {
     "tg_kv_gather_buffer": (vp, [vp]),
     "tg_kv_batch_decode_gather": (i32, [vp, vp, vp, vp, vp, vp, vp]),
     "tg_kv_batch_decode_gather_host": (i32, [vp, vp, vp, vp, vp, vp, vp]),
+    # tgai_kv_group.h
+    "tg_kv_group_create": (vp, [vp, C.POINTER(vp), u32, u32, i32]),
+    "tg_kv_group_destroy": (None, [vp]),
+    "tg_kv_group_decode": (i32, [vp, vp, vp, vp, vp, vp]),
+    "tg_kv_group_prompt": (i32, [vp, PU32, vp, vp, vp, vp, vp]),
+    "tg_kv_group_truncate": (i32, [vp, PU32]),
+    "tg_kv_fork": (i32, [C.POINTER(vp), u32, C.POINTER(vp), u32, u32, vp]),
+    "tg_kv_compact": (i32, [C.POINTER(vp), u32, PU32, PU32, u32, vp]),
     # tgai_backend.h
     "tg_be_probe": (i32, []),
     "tg_be_select": (i32, [cp]),
@@ -178,6 +186,11 @@ PROTOS = {
     "tg_cuda_kv_attention": (i32, [vp, vp]),
     "tg_cuda_kv_rope_append": (i32, [i32, vp, vp, vp, vp, vp, u32, u32, u32, u32, u32, u32,
                                      vp]),
+    "tg_cuda_kv_device": (i32, []),
+    "tg_cuda_kv_fork_rows": (i32, [vp, u32, vp, u32, u64, u32, vp]),
+    "tg_cuda_kv_compact_rows": (i32, [vp, u32, u64, PU32, PU32, u32, vp]),
+    "tg_cuda_kv_group_table": (vp, [vp, u32, u32, u32]),
+    "tg_cuda_kv_group_attention": (i32, [vp, vp]),
     # tgai_engine_bridge.h -- the engine's CUDA seam (cuda/tgai_cuda_bridge.h:31-60)
     "tg_engine_cuda_init": (i32, [vp]),
     "tg_engine_cuda_forward": (i32, [vp, C.POINTER(C.c_int32), i32, vp, i32,
