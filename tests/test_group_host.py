@@ -13,7 +13,7 @@ class Call(C.Structure):
                 ("head_dim", u32), ("prefix_len", u32), ("table_dev", C.c_void_p),
                 ("old_len", C.POINTER(u32)), ("n_new", C.POINTER(u32)), ("q", C.c_void_p),
                 ("k_new", C.c_void_p), ("v_new", C.c_void_p), ("out", C.c_void_p),
-                ("scale", C.c_float)]
+                ("scale", C.c_float), ("scratch", C.c_void_p)]
 
 
 def caches(*rows):
@@ -80,19 +80,20 @@ def test_compact_rows_refuses(lib, cache, start, count, row, why):
 
 @pytest.mark.parametrize("change,why", [
     ({"q": None}, b"NULL pointer"), ({"out": None}, b"NULL pointer"), ({"table_dev": None}, b"NULL pointer"),
+    ({"scratch": None}, b"NULL pointer"), ({"old_len": None}, b"NULL pointer"), ({"n_new": None}, b"NULL pointer"),
     ({"k_new": None}, b"go together"), ({"v_new": None}, b"go together"),
     ({"q": 0x1008}, b"16-byte aligned"), ({"out": 0x1004}, b"16-byte aligned"),
     ({"k_new": 0x1002}, b"16-byte aligned"), ({"v_new": 0x1008}, b"16-byte aligned"),
     ({"n_seq": 0}, b"no kernel"), ({"n_seq": 1025}, b"no kernel"), ({"head_dim": 96}, b"no kernel"),
     ({"n_heads": 6}, b"no kernel"), ({"n_kv_heads": 0}, b"no kernel"),
     ({"n_heads": 516, "n_kv_heads": 4}, b"no kernel"), ({"act": 2}, b"no kernel"),
-    ({"new": 0x7fffffff}, b"too many query rows"),
+    ({"new": 0x7fffffff}, b"too many query rows"), ({"prefix_len": 0x80000000}, b"too long"),
 ])
 def test_group_attention_refuses(lib, change, why):
     change = dict(change)
     old, new = (u32 * 1)(0), (u32 * 1)(change.pop("new", 1))
     a = dict(act=0, n_seq=1, n_heads=8, n_kv_heads=4, head_dim=64, prefix_len=0, table_dev=0x1000, old_len=old,
-             n_new=new, q=0x1000, k_new=0x2000, v_new=0x3000, out=0x4000, scale=1.0)
+             n_new=new, q=0x1000, k_new=0x2000, v_new=0x3000, out=0x4000, scale=1.0, scratch=0x5000)
     a.update(change)
     c = Call(**a)
     assert lib.tg_cuda_kv_group_attention(C.byref(c), None) == 0
@@ -103,3 +104,55 @@ def test_group_table_refuses(lib):
     for n, nkv, hd in ((0, 4, 64), (1025, 4, 64), (1, 0, 64), (1, 4, 96)):
         assert not lib.tg_cuda_kv_group_table(caches((16, 8), (0, 0)), n, nkv, hd)
         assert b"bad argument" in lib.tg_cuda_kv_last_error()
+
+
+def plan(lib, old, new, prefix, nh, nkv, sms=148):
+    """(share, CTA starts) of a call; the last start is the end of the line."""
+    n = len(old)
+    c = Call(act=0, n_seq=n, n_heads=nh, n_kv_heads=nkv, head_dim=64, prefix_len=prefix, old_len=(u32 * n)(*old),
+             n_new=(u32 * n)(*new))
+    share, n_cta, starts = u32(), u32(), (u32 * (161 * 4))()
+    assert lib.tg_cuda_kv_group_plan(C.byref(c), sms, C.byref(share), C.byref(n_cta), starts), \
+        lib.tg_cuda_kv_last_error()
+    return share.value, [tuple(starts[4 * b:4 * b + 4]) for b in range(n_cta.value + 1)]
+
+
+def line(old, new, prefix, nh, nkv, share):
+    """Every (item, tile) of the line in order, from the description of the cut alone."""
+    tpt = 128 // (nh // nkv)
+
+    def row_tiles(seq, tokens, tiles_of):
+        return [(seq, h, r, j) for h in range(nkv) for r in range(-(-tokens // tpt)) for j in range(tiles_of(r))]
+    pre = -(-prefix // 128)
+    got = row_tiles(0, sum(new), lambda r: pre) if share else []
+    for i, (o, t) in enumerate(zip(old, new)):
+        got += row_tiles(i + 1, t, lambda r: (0 if share else pre) + -(-(o + min((r + 1) * tpt, t)) // 128))
+    return got
+
+
+@pytest.mark.parametrize("old,new,prefix,nh,nkv,share", [
+    ([0], [1], 0, 1, 1, 0), ([0], [1], 1, 1, 1, 0), ([5] * 64, [1] * 64, 32768, 32, 8, 1),
+    ([100] * 1024, [1] * 1024, 300, 8, 8, 1), ([0, 3, 900], [0, 7, 0], 500, 12, 4, 0),
+    ([0] * 5, [0] * 5, 100, 4, 4, 0), ([0, 0], [5000, 1], 0, 16, 4, 0), ([10] * 12, [2, 9, 0, 4, 0, 8, 1, 1, 3, 5, 6, 7],
+                                                                       700, 16, 2, 1),
+    ([77] * 9, [40] * 9, 4000, 16, 4, 1), ([1], [3], 129, 128, 1, 0), ([200000], [1], 0, 7, 1, 0),
+    ([0] * 30, [600] * 30, 100, 32, 8, 0),
+])
+@pytest.mark.parametrize("sms", [148, 1, 7, 0])
+def test_plan_covers_the_line(lib, old, new, prefix, nh, nkv, share, sms):
+    """The CTAs' stretches are the line of tiles, cut in order into parts of about one size."""
+    got_share, starts = plan(lib, old, new, prefix, nh, nkv, sms)
+    assert got_share == share
+    tiles = line(old, new, prefix, nh, nkv, share)
+    if not tiles:
+        assert len(starts) == 1
+        return
+    index = {t: k for k, t in enumerate(tiles)}
+    cuts = [index[s] for s in starts[:-1]] + [len(tiles)]
+    assert starts[-1] == (len(old) + 1, 0, 0, 0)
+    assert cuts[0] == 0 and all(a <= b for a, b in zip(cuts, cuts[1:]))
+    n_cta = len(starts) - 1
+    assert n_cta == min(len(tiles), sms or 160)
+    items = len({t[:3] for t in tiles})
+    most = max(b - a + len({t[:3] for t in tiles[a:b]}) for a, b in zip(cuts, cuts[1:]))
+    assert most <= (len(tiles) + items) / n_cta + 3

@@ -8,6 +8,7 @@
  * needs no copy of its own.
  */
 #include "tgai_cuda_bridge.h"
+#include "tgkv_group_plan.h"
 #include "tgkv_launch.h"
 
 #include <cuda.h>                 /* CUtensorMap types; the encoder comes from the runtime */
@@ -1019,6 +1020,12 @@ int tg_cuda_kv_compact_rows(const TGCudaRowCache* caches, uint32_t n, uint64_t r
     return launch_rc(tgkv_launch_compact(&p, cluster, stream), "compact kernel");
 }
 
+/* A group's device table: n + 1 buffer records, then (128-byte aligned) their
+ * tensor maps. */
+static size_t group_maps_offset(uint32_t n) {
+    return ((size_t)(n + 1) * sizeof(TGKvRowCache) + 127) / 128 * 128;
+}
+
 void* tg_cuda_kv_group_table(const TGCudaRowCache* caches, uint32_t n, uint32_t n_kv_heads,
                              uint32_t head_dim) {
     if (!caches || n == 0 || n > TGKV_MAX_ITEMS || n_kv_heads == 0 ||
@@ -1027,19 +1034,140 @@ void* tg_cuda_kv_group_table(const TGCudaRowCache* caches, uint32_t n, uint32_t 
         return NULL;
     }
     if (!g_ready && !tg_cuda_kv_init()) return NULL;
-    const size_t bytes = (size_t)(n + 1) * sizeof(TGKvRowCache);
+    const size_t at = group_maps_offset(n), bytes = at + (size_t)(n + 1) * sizeof(CUtensorMap);
+    unsigned char* h = (unsigned char*)aligned_alloc(128, (bytes + 127) / 128 * 128);
+    if (!h) { set_err("group table: out of host memory"); return NULL; }
+    memset(h, 0, bytes);
+    memcpy(h, caches, (n + 1) * sizeof(TGKvRowCache));
+    for (uint32_t i = 0; i <= n; i++)
+        if (caches[i].base &&
+            !encode_tmap_box(1, caches[i].base, (uint32_t)caches[i].max_seq, n_kv_heads, head_dim, 64,
+                             TGKV_GROUP_TILE, 1, (CUtensorMap*)(h + at) + i)) {
+            free(h);
+            return NULL;
+        }
     void* d = tg_cuda_kv_malloc(bytes);
-    if (!d) return NULL;
-    if (!cuda_ok(cudaMemcpy(d, caches, bytes, cudaMemcpyHostToDevice), "group table h2d") ||
-        !cuda_ok(cudaStreamSynchronize(0), "group table h2d")) {
+    if (d && (!cuda_ok(cudaMemcpy(d, h, bytes, cudaMemcpyHostToDevice), "group table h2d") ||
+              !cuda_ok(cudaStreamSynchronize(0), "group table h2d"))) {
         tg_cuda_kv_free(d);
-        return NULL;
+        d = NULL;
     }
+    free(h);
     return d;
 }
 
+/* Partial rows of a group's scratch below the CTAs' slots: two parts of every
+ * row of a decode step, and of up to 16384 rows of prompts (longer ones run
+ * joined, where only the CTAs' slots are needed). */
+static uint64_t group_share_rows(uint32_t n_seq, uint32_t n_heads) {
+    const uint64_t rows = (uint64_t)n_seq * n_heads;
+    return 2 * (rows > 16384 ? rows : 16384);
+}
+static uint64_t group_rows(uint32_t n_seq, uint32_t n_heads) {
+    return group_share_rows(n_seq, n_heads) + 256ull * TGKV_GROUP_MAX_CTAS;
+}
+uint64_t tg_cuda_kv_group_scratch_bytes(uint32_t n_seq, uint32_t n_heads, uint32_t head_dim) {
+    return group_rows(n_seq, n_heads) * (head_dim + 2) * 4;
+}
+
+/* Checks a call and fills p's lengths, geometry and plan. */
+static int plan_group(const TGCudaGroupCall* c, uint32_t sms, TGKvGroupParams* p) {
+    if (!c || !c->old_len || !c->n_new) { set_err("group: NULL pointer"); return 0; }
+    if (c->n_seq == 0 || c->n_seq > TGKV_MAX_ITEMS || c->n_kv_heads == 0 || c->n_heads == 0 ||
+        c->n_heads % c->n_kv_heads || c->n_heads / c->n_kv_heads > TGKV_GROUP_ROWS ||
+        (c->head_dim != 64 && c->head_dim != 128) || (c->act != 0 && c->act != 1)) {
+        set_err("group: no kernel for %u/%u heads of %u, %u sequences, activations of type %d",
+                c->n_heads, c->n_kv_heads, c->head_dim, c->n_seq, c->act);
+        return 0;
+    }
+    uint64_t total = 0;
+    for (uint32_t i = 0; i < c->n_seq; i++) {
+        p->tok0[i] = (uint32_t)total;
+        p->old_len[i] = c->old_len[i];
+        total += c->n_new[i];
+        if (total * c->n_heads > 0x7fffffffull) {
+            set_err("group: too many query rows (tokens x heads above 2^31 - 1)");
+            return 0;
+        }
+        if ((uint64_t)c->old_len[i] + c->n_new[i] > 0x7fffffffull || c->prefix_len > 0x7fffffffu) {
+            set_err("group: sequence %u is too long", i);
+            return 0;
+        }
+    }
+    p->tok0[c->n_seq] = (uint32_t)total;
+    p->n_seq = c->n_seq;
+    p->n_heads = c->n_heads;
+    p->n_kv_heads = c->n_kv_heads;
+    p->head_dim = c->head_dim;
+    p->prefix_len = c->prefix_len;
+    p->n_cta = p->n_split = p->share = 0;
+    p->cta_rows = 0;
+    if (total == 0) return 1;
+    /* Split when row tiles over all sequences' tokens need at most 3/4 of the
+     * prefix passes that the sequences' own row tiles make. */
+    uint64_t own_tiles = 0;
+    for (uint32_t i = 1; i <= c->n_seq; i++) own_tiles += tgkv_group_row_tiles(p, i);
+    const uint32_t tpt = tgkv_group_tpt(p);
+    if (c->prefix_len && 4 * ((total + tpt - 1) / tpt) <= 3 * own_tiles &&
+        2 * total * c->n_heads <= group_share_rows(c->n_seq, c->n_heads)) {
+        p->share = 1;
+        p->cta_rows = (uint32_t)(2 * total * c->n_heads);
+    }
+    /* the line's cost: tiles, and TGKV_GROUP_ITEM_COST per item */
+    uint64_t cost = 0, units = 0;
+    for (uint32_t s = tgkv_group_skip(p, 0); s <= c->n_seq; s = tgkv_group_skip(p, s + 1)) {
+        const uint32_t nrt = tgkv_group_row_tiles(p, s);
+        uint64_t tiles = 0;
+        for (uint32_t rt = 0; rt < nrt; rt++) tiles += tgkv_group_item_tiles(p, s, rt);
+        units += tiles * c->n_kv_heads;
+        cost += (tiles + (uint64_t)nrt * TGKV_GROUP_ITEM_COST) * c->n_kv_heads;
+    }
+    uint32_t n_cta = sms && sms < TGKV_GROUP_MAX_CTAS ? sms : TGKV_GROUP_MAX_CTAS;
+    if (units < n_cta) n_cta = (uint32_t)units;
+    p->n_cta = n_cta;
+    TGKvGroupPos* start = (TGKvGroupPos*)p->start;
+    uint32_t b = 0;
+    uint64_t at = 0;                                /* cost before the current item */
+    for (uint32_t s = tgkv_group_skip(p, 0); s <= c->n_seq; s = tgkv_group_skip(p, s + 1)) {
+        const uint32_t nrt = tgkv_group_row_tiles(p, s);
+        uint64_t head = 0;                          /* cost of one KV head's items of s */
+        for (uint32_t rt = 0; rt < nrt; rt++)
+            head += tgkv_group_item_tiles(p, s, rt) + TGKV_GROUP_ITEM_COST;
+        for (uint32_t kvh = 0; kvh < c->n_kv_heads; kvh++) {
+            if (b >= n_cta || (uint64_t)b * cost / n_cta >= at + head) { at += head; continue; }
+            for (uint32_t rt = 0; rt < nrt; rt++) {
+                const uint64_t end = at + tgkv_group_item_tiles(p, s, rt) + TGKV_GROUP_ITEM_COST;
+                for (; b < n_cta && (uint64_t)b * cost / n_cta < end; b++) {
+                    const uint64_t off = (uint64_t)b * cost / n_cta - at;
+                    start[b].seq = s;
+                    start[b].kvh = kvh;
+                    start[b].rt = rt;
+                    start[b].tile = off > TGKV_GROUP_ITEM_COST ? (uint32_t)(off - TGKV_GROUP_ITEM_COST) : 0;
+                    if (start[b].tile) p->n_split++;
+                }
+                at = end;
+            }
+        }
+    }
+    start[n_cta].seq = c->n_seq + 1;
+    start[n_cta].kvh = start[n_cta].rt = start[n_cta].tile = 0;
+    return 1;
+}
+
+int tg_cuda_kv_group_plan(const TGCudaGroupCall* c, uint32_t sms, uint32_t* share, uint32_t* n_cta,
+                          uint32_t* starts) {
+    static _Thread_local TGKvGroupParams p;    /* 11 KB: keep off the stack */
+    if (!share || !n_cta || !starts) { set_err("group: NULL pointer"); return 0; }
+    if (!plan_group(c, sms, &p)) return 0;
+    *share = p.share;
+    *n_cta = p.n_cta;
+    memcpy(starts, p.start, (p.n_cta + 1) * sizeof(TGKvGroupPos));
+    return 1;
+}
+
 int tg_cuda_kv_group_attention(const TGCudaGroupCall* c, void* stream) {
-    if (!c || !c->table_dev || !c->old_len || !c->n_new || !c->q || !c->out) {
+    static _Thread_local TGKvGroupParams p;    /* 11 KB: keep off the stack */
+    if (!c || !c->table_dev || !c->scratch || !c->q || !c->out) {
         set_err("group: NULL pointer");
         return 0;
     }
@@ -1048,37 +1176,18 @@ int tg_cuda_kv_group_attention(const TGCudaGroupCall* c, void* stream) {
         set_err("group: q, k_new, v_new and out must be 16-byte aligned");
         return 0;
     }
-    if (c->n_seq == 0 || c->n_seq > TGKV_MAX_ITEMS || c->n_kv_heads == 0 || c->n_heads == 0 ||
-        c->n_heads % c->n_kv_heads || c->n_heads / c->n_kv_heads > 128 ||
-        (c->head_dim != 64 && c->head_dim != 128) || (c->act != 0 && c->act != 1)) {
-        set_err("group: no kernel for %u/%u heads of %u, %u sequences, activations of type %d",
-                c->n_heads, c->n_kv_heads, c->head_dim, c->n_seq, c->act);
-        return 0;
-    }
-    static _Thread_local TGKvGroupParams p;    /* 8 KB: keep off the stack */
-    uint64_t total = 0;
-    for (uint32_t i = 0; i < c->n_seq; i++) {
-        p.tok0[i] = (uint32_t)total;
-        p.old_len[i] = c->old_len[i];
-        total += c->n_new[i];
-        if (total * c->n_heads > 0x7fffffffull) {
-            set_err("group: too many query rows (tokens x heads above 2^31 - 1)");
-            return 0;
-        }
-    }
+    if (!plan_group(c, (uint32_t)g_sm_count, &p)) return 0;
     if (!g_ready && !tg_cuda_kv_init()) return 0;
-    if (total == 0) return 1;
-    p.tok0[c->n_seq] = (uint32_t)total;
+    if (p.n_cta == 0) return 1;
     p.table = (const TGKvRowCache*)c->table_dev;
+    p.tmaps = (uint64_t)(uintptr_t)c->table_dev + group_maps_offset(c->n_seq);
     p.q = c->q;
     p.k_new = c->k_new;
     p.v_new = c->v_new;
     p.out = c->out;
-    p.n_seq = c->n_seq;
-    p.n_heads = c->n_heads;
-    p.n_kv_heads = c->n_kv_heads;
-    p.head_dim = c->head_dim;
-    p.prefix_len = c->prefix_len;
+    p.part_o = (float*)c->scratch;
+    p.part_ml = p.part_o + group_rows(c->n_seq, c->n_heads) * c->head_dim;
+    p.err = g_err_word;
     p.qscale = c->scale * 1.4426950408889634f;
     return launch_rc(tgkv_launch_group(&p, c->act, stream), "group attention");
 }

@@ -18,6 +18,7 @@ extern "C" {
 #define TGKV_MAX_ITEMS 1024      /* items (query rows / caches) per launch */
 #define TGKV_MAX_RANKS 8         /* GPUs of one node in an output gather */
 #define TGKV_TILE      32        /* positions per pipeline stage */
+#define TGKV_GROUP_MAX_CTAS 160  /* CTAs of a group launch */
 
 /* One cache buffer [2][max_seq][kv_dim] in device memory, with the device
  * address of its TMA tensor map: a 3-D map over (kv_dim, max_seq, 2) whose box
@@ -197,18 +198,33 @@ typedef struct {
     uint32_t first[TGKV_MAX_ITEMS];
 } TGKvCompactParams;
 
-/* ---- groups of caches with a shared prefix (tgkv_group.cu) ---- */
+/* ---- groups of caches with a shared prefix (tgkv_group.cu); the plan is in
+ * tgkv_group_plan.h ---- */
 typedef struct {
     const TGKvRowCache* table;   /* device: the n_seq caches, then the prefix cache */
+    uint64_t    tmaps;           /* device: their tensor maps (128 bytes each; box 64 dims x
+                                  * 128 positions, 128-byte swizzle) */
     const void* q;               /* [tokens][n_heads][head_dim] */
     const void* k_new;           /* NULL, or [tokens][kv_dim]: rows old_len[i] .. of cache i */
     const void* v_new;
     void*       out;             /* as q */
+    /* partial rows: [..][head_dim] unnormalised outputs and [..][2] (maximum,
+     * in the log2 domain, and sum of weights) */
+    float*      part_o;
+    float*      part_ml;
+    int32_t*    err;             /* device error word */
     uint32_t n_seq, n_heads, n_kv_heads, head_dim;
     uint32_t prefix_len;
     float    qscale;             /* softmax scale * log2(e) */
+    uint32_t share, n_cta;
+    uint32_t cta_rows;           /* first partial row of the CTAs' slots: CTA b's rows are
+                                  * cta_rows + 256 b + (0: the item it continues, 128: the one
+                                  * it leaves unfinished) + r; below it, with share, query row x's
+                                  * prefix part at x and own part at total rows + x */
+    uint32_t n_split;            /* CTAs that continue an item */
     uint32_t old_len[TGKV_MAX_ITEMS];       /* own rows before the call's tokens */
     uint32_t tok0[TGKV_MAX_ITEMS + 1];      /* first packed token of each sequence; the total */
+    uint32_t start[(TGKV_GROUP_MAX_CTAS + 1) * 4];  /* TGKvGroupPos of each CTA, and the end */
 } TGKvGroupParams;
 int tgkv_launch_fork(const TGKvForkParams* p, void* stream);
 int tgkv_launch_compact(const TGKvCompactParams* p, uint32_t cluster, void* stream);

@@ -64,6 +64,7 @@ struct TGKvGroup {
     uint32_t* old_len;                /* host [n]: own rows before the call's tokens */
     uint32_t* ones;                   /* host [n]: the n_new of a decode step */
     void* table_dev;
+    void* scratch;                    /* partial rows, sized for every call of the group */
 };
 
 TGKvGroup* tg_kv_group_create(TGKvCache* prefix, TGKvCache* const* caches, uint32_t n,
@@ -127,9 +128,11 @@ TGKvGroup* tg_kv_group_create(TGKvCache* prefix, TGKvCache* const* caches, uint3
     g->device = tg_cuda_kv_device();
     g->table_dev = tg_cuda_kv_group_table(table, n, c0->n_kv_heads, c0->head_dim);
     free(table);
-    if (!g->table_dev) {
-        tg_kv_group_destroy(g);
+    if (g->table_dev)
+        g->scratch = tg_cuda_kv_malloc(tg_cuda_kv_group_scratch_bytes(n, n_heads, c0->head_dim));
+    if (!g->table_dev || !g->scratch) {
         set_err("group: %s", tg_cuda_kv_last_error());
+        tg_kv_group_destroy(g);
         return NULL;
     }
     return g;
@@ -138,6 +141,7 @@ TGKvGroup* tg_kv_group_create(TGKvCache* prefix, TGKvCache* const* caches, uint3
 void tg_kv_group_destroy(TGKvGroup* g) {
     if (!g) return;
     tg_cuda_kv_free(g->table_dev);
+    tg_cuda_kv_free(g->scratch);
     free(g->caches);
     free(g->old_len);
     free(g->ones);
@@ -195,6 +199,7 @@ static int group_call(TGKvGroup* g, const uint32_t* n_new, const void* q, const 
     call.k_new = k_new;
     call.v_new = v_new;
     call.out = out;
+    call.scratch = g->scratch;
     call.scale = (1.0f / sqrtf((float)c0->head_dim)) * mscale;
     if (!tg_cuda_kv_group_attention(&call, stream)) {
         set_err("%s", tg_cuda_kv_last_error());

@@ -190,6 +190,8 @@ PROTOS = {
     "tg_cuda_kv_fork_rows": (i32, [vp, u32, vp, u32, u64, u32, vp]),
     "tg_cuda_kv_compact_rows": (i32, [vp, u32, u64, PU32, PU32, u32, vp]),
     "tg_cuda_kv_group_table": (vp, [vp, u32, u32, u32]),
+    "tg_cuda_kv_group_scratch_bytes": (u64, [u32, u32, u32]),
+    "tg_cuda_kv_group_plan": (i32, [vp, u32, PU32, PU32, PU32]),
     "tg_cuda_kv_group_attention": (i32, [vp, vp]),
     # tgai_engine_bridge.h -- the engine's CUDA seam (cuda/tgai_cuda_bridge.h:31-60)
     "tg_engine_cuda_init": (i32, [vp]),
