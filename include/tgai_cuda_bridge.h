@@ -234,8 +234,9 @@ uint64_t tg_cuda_kv_group_scratch_bytes(uint32_t n_seq, uint32_t n_heads, uint32
 /* How a call's work is dealt to CTAs on a device of `sms` SMs (no launch, no
  * device needed): share 1 if the prefix is attended for all sequences' tokens
  * together, the CTAs, and where on the line of tiles each starts: n_cta + 1
- * records (sequence: 0 the shared prefix, i + 1 sequence i; KV head; row tile;
- * K/V tile), at most 161. */
+ * records (sequence: 0 the shared prefix, i + 1 sequence i; KV head; item, of
+ * 256 / G tokens with bf16 activations and 128 / G with fp32 ones, G = n_heads /
+ * n_kv_heads; K/V tile of 128 positions), at most 161. */
 int tg_cuda_kv_group_plan(const TGCudaGroupCall* c, uint32_t sms, uint32_t* share, uint32_t* n_cta,
                           uint32_t* starts);
 int tg_cuda_kv_group_attention(const TGCudaGroupCall* c, void* stream);

@@ -214,6 +214,26 @@ def test_large_scores(cuda, devbuf, act):
     s.close()
 
 
+@pytest.mark.parametrize("act", [F32, BF16])
+@pytest.mark.parametrize("new", [None, 40])                 # a decode step, or packed prompts of 40 tokens
+def test_repeats_are_identical(cuda, devbuf, act, new):
+    """Long stretches per CTA: the same call gives the same bits every time."""
+    n = 24
+    s = Setup(cuda, [1000 + 37 * i for i in range(n)], [41] * n, 6000, 32, 8, 128, act, seed=3)
+    n_new = [new or 1] * n
+    (qb, q), (kb, k), (vb, v) = s.new(sum(n_new))
+    qd, kd, vd, od = devbuf(qb), devbuf(kb), devbuf(vb), devbuf(nbytes=qb.nbytes)
+    arr, first = (C.c_uint32 * n)(*n_new), None
+    tgkv.check(cuda.tg_kv_group_prompt(s.g, arr, qd.ptr, kd.ptr, vd.ptr, od.ptr, None), cuda)
+    for _ in range(8):
+        tgkv.check(cuda.tg_kv_group_prompt(s.g, arr, qd.ptr, None, None, od.ptr, None), cuda)
+        assert cuda.tg_cuda_kv_sync(None)
+        got = od.get(qb.dtype, qb.shape)
+        first = got if first is None else first
+        assert np.array_equal(got.view(np.uint8), first.view(np.uint8))
+    s.close()
+
+
 def test_matches_the_single_cache_operators(cuda, devbuf):
     """The same history in one plain cache: tg_kv_append_attention and tg_kv_attention agree."""
     lib, nh, nkv, hd, P = cuda, 16, 4, 128, 200

@@ -106,10 +106,10 @@ def test_group_table_refuses(lib):
         assert b"bad argument" in lib.tg_cuda_kv_last_error()
 
 
-def plan(lib, old, new, prefix, nh, nkv, sms=148):
+def plan(lib, old, new, prefix, nh, nkv, act, sms):
     """(share, CTA starts) of a call; the last start is the end of the line."""
     n = len(old)
-    c = Call(act=0, n_seq=n, n_heads=nh, n_kv_heads=nkv, head_dim=64, prefix_len=prefix, old_len=(u32 * n)(*old),
+    c = Call(act=act, n_seq=n, n_heads=nh, n_kv_heads=nkv, head_dim=64, prefix_len=prefix, old_len=(u32 * n)(*old),
              n_new=(u32 * n)(*new))
     share, n_cta, starts = u32(), u32(), (u32 * (161 * 4))()
     assert lib.tg_cuda_kv_group_plan(C.byref(c), sms, C.byref(share), C.byref(n_cta), starts), \
@@ -117,9 +117,9 @@ def plan(lib, old, new, prefix, nh, nkv, sms=148):
     return share.value, [tuple(starts[4 * b:4 * b + 4]) for b in range(n_cta.value + 1)]
 
 
-def line(old, new, prefix, nh, nkv, share):
+def line(old, new, prefix, nh, nkv, share, act):
     """Every (item, tile) of the line in order, from the description of the cut alone."""
-    tpt = 128 // (nh // nkv)
+    tpt = 128 // (nh // nkv) * (1 + act)
 
     def row_tiles(seq, tokens, tiles_of):
         return [(seq, h, r, j) for h in range(nkv) for r in range(-(-tokens // tpt)) for j in range(tiles_of(r))]
@@ -135,15 +135,16 @@ def line(old, new, prefix, nh, nkv, share):
     ([100] * 1024, [1] * 1024, 300, 8, 8, 1), ([0, 3, 900], [0, 7, 0], 500, 12, 4, 0),
     ([0] * 5, [0] * 5, 100, 4, 4, 0), ([0, 0], [5000, 1], 0, 16, 4, 0), ([10] * 12, [2, 9, 0, 4, 0, 8, 1, 1, 3, 5, 6, 7],
                                                                        700, 16, 2, 1),
-    ([77] * 9, [40] * 9, 4000, 16, 4, 1), ([1], [3], 129, 128, 1, 0), ([200000], [1], 0, 7, 1, 0),
+    ([77] * 9, [40] * 9, 4000, 16, 4, 1), ([77] * 9, [60] * 9, 4000, 16, 4, 0), ([1], [3], 129, 128, 1, 0), ([200000], [1], 0, 7, 1, 0),
     ([0] * 30, [600] * 30, 100, 32, 8, 0),
 ])
+@pytest.mark.parametrize("act", [0, 1])
 @pytest.mark.parametrize("sms", [148, 1, 7, 0])
-def test_plan_covers_the_line(lib, old, new, prefix, nh, nkv, share, sms):
+def test_plan_covers_the_line(lib, old, new, prefix, nh, nkv, share, sms, act):
     """The CTAs' stretches are the line of tiles, cut in order into parts of about one size."""
-    got_share, starts = plan(lib, old, new, prefix, nh, nkv, sms)
+    got_share, starts = plan(lib, old, new, prefix, nh, nkv, act, sms)
     assert got_share == share
-    tiles = line(old, new, prefix, nh, nkv, share)
+    tiles = line(old, new, prefix, nh, nkv, share, act)
     if not tiles:
         assert len(starts) == 1
         return

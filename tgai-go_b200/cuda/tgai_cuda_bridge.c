@@ -1064,10 +1064,17 @@ static uint64_t group_share_rows(uint32_t n_seq, uint32_t n_heads) {
     return 2 * (rows > 16384 ? rows : 16384);
 }
 static uint64_t group_rows(uint32_t n_seq, uint32_t n_heads) {
-    return group_share_rows(n_seq, n_heads) + 256ull * TGKV_GROUP_MAX_CTAS;
+    return group_share_rows(n_seq, n_heads) + 512ull * TGKV_GROUP_MAX_CTAS;
 }
 uint64_t tg_cuda_kv_group_scratch_bytes(uint32_t n_seq, uint32_t n_heads, uint32_t head_dim) {
     return group_rows(n_seq, n_heads) * (head_dim + 2) * 4;
+}
+
+static TGKvGroupShape group_shape(const TGKvGroupParams* p) {
+    TGKvGroupShape s = {p->n_seq, p->n_kv_heads, p->prefix_len, p->share, 0, 0, p->old_len, p->tok0};
+    s.tpt = TGKV_GROUP_ROWS / (p->n_heads / p->n_kv_heads);
+    s.item_tokens = s.tpt * p->pair;
+    return s;
 }
 
 /* Checks a call and fills p's lengths, geometry and plan. */
@@ -1101,56 +1108,75 @@ static int plan_group(const TGCudaGroupCall* c, uint32_t sms, TGKvGroupParams* p
     p->head_dim = c->head_dim;
     p->prefix_len = c->prefix_len;
     p->n_cta = p->n_split = p->share = 0;
+    p->pair = c->act == 1 ? 2 : 1;
     p->cta_rows = 0;
     if (total == 0) return 1;
-    /* Split when row tiles over all sequences' tokens need at most 3/4 of the
-     * prefix passes that the sequences' own row tiles make. */
-    uint64_t own_tiles = 0;
-    for (uint32_t i = 1; i <= c->n_seq; i++) own_tiles += tgkv_group_row_tiles(p, i);
-    const uint32_t tpt = tgkv_group_tpt(p);
-    if (c->prefix_len && 4 * ((total + tpt - 1) / tpt) <= 3 * own_tiles &&
+    TGKvGroupShape sh = group_shape(p);
+    /* Split when items over all sequences' tokens need at most 3/4 of the
+     * prefix passes that the sequences' own items make. */
+    uint64_t own_items = 0;
+    for (uint32_t i = 1; i <= c->n_seq; i++) own_items += tgkv_group_items(&sh, i);
+    if (c->prefix_len && 4 * ((total + sh.item_tokens - 1) / sh.item_tokens) <= 3 * own_items &&
         2 * total * c->n_heads <= group_share_rows(c->n_seq, c->n_heads)) {
-        p->share = 1;
+        p->share = sh.share = 1;
         p->cta_rows = (uint32_t)(2 * total * c->n_heads);
     }
     /* the line's cost: tiles, and TGKV_GROUP_ITEM_COST per item */
     uint64_t cost = 0, units = 0;
-    for (uint32_t s = tgkv_group_skip(p, 0); s <= c->n_seq; s = tgkv_group_skip(p, s + 1)) {
-        const uint32_t nrt = tgkv_group_row_tiles(p, s);
+    for (uint32_t s = tgkv_group_skip(&sh, 0); s <= c->n_seq; s = tgkv_group_skip(&sh, s + 1)) {
+        const uint32_t n = tgkv_group_items(&sh, s);
         uint64_t tiles = 0;
-        for (uint32_t rt = 0; rt < nrt; rt++) tiles += tgkv_group_item_tiles(p, s, rt);
+        for (uint32_t at = 0; at < n; at++) tiles += tgkv_group_item_tiles(&sh, s, at);
         units += tiles * c->n_kv_heads;
-        cost += (tiles + (uint64_t)nrt * TGKV_GROUP_ITEM_COST) * c->n_kv_heads;
+        cost += (tiles + (uint64_t)n * TGKV_GROUP_ITEM_COST) * c->n_kv_heads;
     }
     uint32_t n_cta = sms && sms < TGKV_GROUP_MAX_CTAS ? sms : TGKV_GROUP_MAX_CTAS;
     if (units < n_cta) n_cta = (uint32_t)units;
     p->n_cta = n_cta;
     TGKvGroupPos* start = (TGKvGroupPos*)p->start;
     uint32_t b = 0;
-    uint64_t at = 0;                                /* cost before the current item */
-    for (uint32_t s = tgkv_group_skip(p, 0); s <= c->n_seq; s = tgkv_group_skip(p, s + 1)) {
-        const uint32_t nrt = tgkv_group_row_tiles(p, s);
+    uint64_t done = 0;                              /* cost before the current item */
+    for (uint32_t s = tgkv_group_skip(&sh, 0); s <= c->n_seq; s = tgkv_group_skip(&sh, s + 1)) {
+        const uint32_t n = tgkv_group_items(&sh, s);
         uint64_t head = 0;                          /* cost of one KV head's items of s */
-        for (uint32_t rt = 0; rt < nrt; rt++)
-            head += tgkv_group_item_tiles(p, s, rt) + TGKV_GROUP_ITEM_COST;
+        for (uint32_t at = 0; at < n; at++)
+            head += tgkv_group_item_tiles(&sh, s, at) + TGKV_GROUP_ITEM_COST;
         for (uint32_t kvh = 0; kvh < c->n_kv_heads; kvh++) {
-            if (b >= n_cta || (uint64_t)b * cost / n_cta >= at + head) { at += head; continue; }
-            for (uint32_t rt = 0; rt < nrt; rt++) {
-                const uint64_t end = at + tgkv_group_item_tiles(p, s, rt) + TGKV_GROUP_ITEM_COST;
+            if (b >= n_cta || (uint64_t)b * cost / n_cta >= done + head) { done += head; continue; }
+            for (uint32_t at = 0; at < n; at++) {
+                const uint64_t end = done + tgkv_group_item_tiles(&sh, s, at) + TGKV_GROUP_ITEM_COST;
                 for (; b < n_cta && (uint64_t)b * cost / n_cta < end; b++) {
-                    const uint64_t off = (uint64_t)b * cost / n_cta - at;
+                    const uint64_t off = (uint64_t)b * cost / n_cta - done;
                     start[b].seq = s;
                     start[b].kvh = kvh;
-                    start[b].rt = rt;
+                    start[b].at = at;
                     start[b].tile = off > TGKV_GROUP_ITEM_COST ? (uint32_t)(off - TGKV_GROUP_ITEM_COST) : 0;
                     if (start[b].tile) p->n_split++;
                 }
-                at = end;
+                done = end;
             }
         }
     }
     start[n_cta].seq = c->n_seq + 1;
-    start[n_cta].kvh = start[n_cta].rt = start[n_cta].tile = 0;
+    start[n_cta].kvh = start[n_cta].at = start[n_cta].tile = 0;
+    return 1;
+}
+
+/* q of a bf16 call as the kernel's row tiles read it. */
+static int encode_group_qmap(const TGKvGroupParams* p, CUtensorMap* out) {
+    if (!resolve_encode()) return 0;
+    const uint32_t g = p->n_heads / p->n_kv_heads;
+    cuuint64_t dims[3] = {p->head_dim, p->n_heads, p->tok0[p->n_seq]};
+    cuuint64_t strides[2] = {p->head_dim * 2ull, (uint64_t)p->n_heads * p->head_dim * 2};
+    cuuint32_t box[3] = {64, g, TGKV_GROUP_ROWS / g};
+    cuuint32_t estr[3] = {1, 1, 1};
+    CUresult r = g_encode(out, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, (void*)p->q, dims, strides, box, estr,
+                          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                          CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) {
+        set_err("cuTensorMapEncodeTiled (group q) failed (%d)", (int)r);
+        return 0;
+    }
     return 1;
 }
 
@@ -1189,5 +1215,6 @@ int tg_cuda_kv_group_attention(const TGCudaGroupCall* c, void* stream) {
     p.part_ml = p.part_o + group_rows(c->n_seq, c->n_heads) * c->head_dim;
     p.err = g_err_word;
     p.qscale = c->scale * 1.4426950408889634f;
+    if (c->act == 1 && !encode_group_qmap(&p, &p.qmap)) return 0;
     return launch_rc(tgkv_launch_group(&p, c->act, stream), "group attention");
 }

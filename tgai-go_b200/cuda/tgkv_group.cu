@@ -4,32 +4,32 @@
 // h * n_kv_heads / n_heads; out = softmax(q K^T * scale) V over both parts.
 //
 // group_kernel: persistent CTAs, one per SM, each with its stretch of the line
-// of K/V tiles that tgkv_group_plan.h cuts.  A piece is a row tile (128 query
-// rows of one KV head, one per TMEM lane) against a run of 128-position tiles,
-// in one pass: S = Q K^T, running maximum and sum in the log2 domain, O += P V.
-// Inside a CTA (320 threads):
-//   warps 0-7  softmax: TMEM lane r is row r, shared by warps r/32 and r/32 + 4,
-//              which take positions [0,64) and [64,128) of a tile; they exchange
-//              the tile's row maximum through shared memory.  Per piece they
-//              write Q into TMEM; per tile they read S, mask, exponentiate and
-//              write P over S; at the end they read O and write the rows, or
-//              leave them as a partial;
-//   warp 8     TMA: K and V tiles (64-dim boxes, 128-byte swizzle) into two rings,
-//              running ahead over the CTA's whole stretch;
-//   warp 9     the MMAs (one lane), A operand from TMEM: S into one of two
-//              buffers, so that the next tile's S is made while the softmax works
-//              on this one; PV with V as an MN-major operand.
+// of K/V tiles that tgkv_group_plan.h cuts.  A piece is an item (one or two row
+// tiles of 128 query rows of one KV head) against a run of 128-position K/V
+// tiles, in one pass: S = Q K^T, running maximum and sum in the log2 domain,
+// O += P V.  Two streams, each with its own S/P and O in TMEM and its own four
+// softmax warps (one thread per row), take turns on the tensor core: while one
+// stream's scores are exponentiated, the other's products run.
+//   wide pieces    (two row tiles) stream h has the rows of row tile h, and both
+//                  read every K/V tile: half the tile traffic per row;
+//   narrow pieces  (one row tile) both have the same rows and take alternate
+//                  tiles; their results join at the end of the piece.
+// Warps (384 threads): 0-3 and 4-7 the streams' softmax, 8 TMA (K/V tiles in
+// 64-dim boxes, 128-byte swizzle, into two rings that run ahead over the whole
+// stretch; Q of bf16 calls), 9 the MMAs (one lane).
 // TERMS is the number of bf16 terms of q and P: 1 with bf16 activations (q is
 // exact, P is rounded once, 2^-8 of a weight, as the output itself is), 2 with
-// fp32 ones (hi + lo, 16 mantissa bits; three terms of P would not fit the
+// fp32 ones (hi + lo, 16 mantissa bits; a third term of P has no room in the
 // columns S leaves free).  Scores, maxima, sums and O are fp32.
-// TMEM columns: S/P [0,128) and [128,256), O [256,256+HD), Q [384,384+TERMS*HD/2).
+// TMEM columns: S/P of stream h [128 h, 128 h + 128), P as bf16 pairs (hi at
+// +0, lo at +64); O of stream h [256 + 128 h, +HD).
 //
-// group_merge_kernel joins the partials of rows whose tiles more than one
+// group_merge kernels join the partials of rows whose tiles more than one
 // piece attended: no atomics, always in the same order.
 //
 // Every mbarrier wait is bounded; one that runs out sets the device error word
 // and the CTA ends without further waits on its own data.
+#include <cuda.h>
 #include <cuda_runtime.h>
 #include <math.h>
 #include <stdint.h>
@@ -43,30 +43,35 @@ namespace tgkv {
 namespace group {
 
 constexpr int kRows = TGKV_GROUP_ROWS, kPos = TGKV_GROUP_TILE;
-constexpr int kSoftmaxThreads = 256, kThreads = 320;
+constexpr int kThreads = 384;
 constexpr int kTmaWarp = 8, kMmaWarp = 9;
-constexpr uint32_t kBlock = 16384;              // 128 positions x 64 dims bf16: one box
-constexpr uint32_t TM_S = 0, TM_O = 256, TM_Q = 384, TM_COLS = 512;
+constexpr uint32_t kBlock = 16384;              // 128 rows x 64 bf16: one swizzled box
+constexpr uint32_t TM_S = 0, TM_O = 256, TM_COLS = 512;
 constexpr int kErrTimeout = 7;
+// Registers: the softmax threads hold 128 scores; the launch has 384 x 168.
+constexpr int kRegsSoftmax = 208, kRegsOther = 80;
+static_assert(256 * kRegsSoftmax + 128 * kRegsOther <= 384 * 168, "register split");
 
 template <int HD>
 struct Cfg {
-    static constexpr uint32_t kTile = (uint32_t)(HD / 64) * kBlock;    // one K or V tile
-    static constexpr int kStages = HD == 128 ? 3 : 6;                  // per ring: 192 KB in all
-    static constexpr uint32_t OFF_K = 0, OFF_V = kStages * kTile;
-    static constexpr uint32_t OFF_BAR = 2 * kStages * kTile;
+    static constexpr uint32_t kTile = (uint32_t)(HD / 64) * kBlock;    // one K, V or Q tile
+    static constexpr int kStages = HD == 128 ? 2 : 4;                  // per ring: 128 KB in all
+    static constexpr uint32_t OFF_K = 0, OFF_V = kStages * kTile, OFF_Q = 2 * kStages * kTile;
+    static constexpr uint32_t OFF_BAR = OFF_Q + 2 * kTile;             // Q: two row tiles, or hi and lo
     static constexpr int B_KFULL = 0, B_KEMPTY = kStages, B_VFULL = 2 * kStages, B_VEMPTY = 3 * kStages;
-    static constexpr int B_SFULL = 4 * kStages;      // [2] S of the tile in the buffer is in TMEM
-    static constexpr int B_PFULL = B_SFULL + 2;      // [2] its P is written (256 arrivals)
-    static constexpr int B_PVDONE = B_PFULL + 2;     // one phase per tile: its PV is complete
-    static constexpr int B_QREADY = B_PVDONE + 1;    // one phase per piece: Q is in TMEM (256)
-    static constexpr uint32_t OFF_X = OFF_BAR + 32 * 8;                // [2][2][128] maxima
-    static constexpr uint32_t OFF_L = OFF_X + 4 * kRows * 4;           // [2][128] sums
-    static constexpr uint32_t OFF_SLOT = OFF_L + 2 * kRows * 4;
-    static constexpr uint32_t SMEM = OFF_SLOT + 16 + 1024;             // slack to align the base
-    static_assert(B_QREADY < 32 && SMEM <= 232448, "shared memory per CTA");
+    static constexpr int B_SFULL = 4 * kStages;      // [2] a stream's S is in TMEM
+    static constexpr int B_PFULL = B_SFULL + 2;      // [2] its P is written, its O rescaled (128 arrivals)
+    static constexpr int B_PVDONE = B_PFULL + 2;     // [2] its PV is complete
+    static constexpr int B_QFULL = B_PVDONE + 2;     // a piece's Q is in shared memory
+    static constexpr int B_QEMPTY = B_QFULL + 1;     // every S of a piece is complete
+    static constexpr uint32_t OFF_ML = OFF_BAR + 32 * 8;               // [2 streams][128] (m, l)
+    static constexpr uint32_t OFF_SLOT = OFF_ML + 2 * kRows * 8;
+    static constexpr uint32_t OFF_TAB = OFF_SLOT + 16;                 // tok0, old_len
+    static constexpr uint32_t SMEM = OFF_TAB + (2 * TGKV_MAX_ITEMS + 1) * 4 + 1024;    // slack: alignment
+    static_assert(B_QEMPTY < 32 && SMEM <= 232448, "shared memory per CTA");
 };
 
+// The two warps (streams 0 and 1) of a TMEM lane quarter.
 __device__ __forceinline__ void pair_sync(int quarter) {
     asm volatile("bar.sync %0, 64;" ::"r"(1 + quarter) : "memory");
 }
@@ -76,27 +81,42 @@ __device__ __forceinline__ float hi_f(uint32_t x) { return __uint_as_float(x & 0
 __device__ __forceinline__ TGKvGroupPos start_of(const TGKvGroupParams& p, uint32_t b) {
     return TGKvGroupPos{p.start[4 * b], p.start[4 * b + 1], p.start[4 * b + 2], p.start[4 * b + 3]};
 }
+__device__ __forceinline__ TGKvGroupShape shape_of(const TGKvGroupParams& p, const uint32_t* old_len,
+                                                   const uint32_t* tok0) {
+    const uint32_t tpt = kRows / (p.n_heads / p.n_kv_heads);
+    return TGKvGroupShape{p.n_seq, p.n_kv_heads, p.prefix_len, p.share, tpt, tpt * p.pair, old_len, tok0};
+}
 
-// The pieces of a CTA's stretch, one after another.
+// The pieces of a CTA's stretch, one after another.  With `most` > 0 an item's
+// tiles come in pieces of at most that many (their results add up in a slot).
 struct Pieces {
     TGKvGroupPos at, end;
-    uint32_t j0, j1, nt;                         // tiles [j0, j1) of the item's nt
-    __device__ Pieces(const TGKvGroupParams& p, uint32_t cta) : at(start_of(p, cta)), end(start_of(p, cta + 1)) {
-        set(p);
+    uint32_t j0, j1;                             // tiles [j0, j1) of the item
+    uint32_t nt, first;                          // the item's tiles; where this CTA began with it
+    __device__ Pieces(const TGKvGroupShape& s, TGKvGroupPos a, TGKvGroupPos e, uint32_t most) : at(a), end(e) {
+        set(s, most);
     }
     __device__ bool more() const { return j0 < j1; }
-    __device__ void next(const TGKvGroupParams& p) {
+    __device__ void next(const TGKvGroupShape& s, uint32_t most) {
+        const uint32_t stop = tgkv_group_same_item(at, end) ? end.tile : nt;
+        if (j1 < stop) {                         // more of the same item
+            j0 = j1;
+            j1 = most && stop - j0 > most ? j0 + most : stop;
+            return;
+        }
         if (tgkv_group_same_item(at, end)) { j0 = j1; return; }
-        at = tgkv_group_next_item(&p, at);
-        set(p);
+        at = tgkv_group_next_item(&s, at);
+        set(s, most);
     }
+    // the last piece of the item in this CTA
+    __device__ bool last() const { return j1 == (tgkv_group_same_item(at, end) ? end.tile : nt); }
 
 private:
-    __device__ void set(const TGKvGroupParams& p) {
-        const bool last = tgkv_group_same_item(at, end);
-        j0 = at.tile;
-        nt = at.seq <= p.n_seq ? tgkv_group_item_tiles(&p, at.seq, at.rt) : 0;
-        j1 = last ? end.tile : nt;
+    __device__ void set(const TGKvGroupShape& s, uint32_t most) {
+        first = j0 = at.tile;
+        nt = at.seq <= s.n_seq ? tgkv_group_item_tiles(&s, at.seq, at.at) : 0;
+        const uint32_t stop = tgkv_group_same_item(at, end) ? end.tile : nt;
+        j1 = most && stop - j0 > most ? j0 + most : stop;
     }
 };
 
@@ -137,45 +157,45 @@ __global__ void __launch_bounds__(256) group_append_kernel(const __grid_constant
     asm volatile("fence.proxy.async.global;" ::: "memory");
 }
 
-// 32 or 16 32-bit TMEM columns from registers.
-__device__ __forceinline__ void tmem_st(uint32_t addr, const uint32_t (&w)[32]) { tmem_st32(addr, w); }
-__device__ __forceinline__ void tmem_st(uint32_t addr, const uint32_t (&w)[16]) { tmem_st16(addr, w); }
+// 32 consecutive TMEM columns x 4 into v, all loads in flight at once.
+struct Scores { uint32_t c[4][32]; };
+__device__ __forceinline__ void load_scores(uint32_t taddr, Scores& s) {
+    tmem_ld32(taddr, s.c[0]);
+    tmem_ld32(taddr + 32, s.c[1]);
+    tmem_ld32(taddr + 64, s.c[2]);
+    tmem_ld32(taddr + 96, s.c[3]);
+    tmem_wait_ld(s.c[0], s.c[1]);
+    tmem_wait_ld(s.c[2], s.c[3]);
+}
 
-// This thread's HD / 2 head dims of its query row, as bf16 words (two dims
-// each) into TMEM: term t at columns TM_Q + t * HD / 2.
-template <typename T, int HD, int TERMS>
-__device__ __forceinline__ void load_q(const TGKvGroupParams& p, bool valid, uint64_t row, int hf, uint32_t taddr) {
-    constexpr int W = HD / 4;                    // words of half a row
-    uint32_t w[TERMS][W];
-    const T* src = reinterpret_cast<const T*>(p.q) + row * HD + hf * (HD / 2);
-    if constexpr (TERMS == 1) {
+template <bool MASK>
+__device__ __forceinline__ float max32(const uint32_t (&v)[32], int lim) {
+    float a[8];
 #pragma unroll
-        for (int i = 0; i < W / 4; ++i) {
-            const uint4 x = valid ? reinterpret_cast<const uint4*>(src)[i] : make_uint4(0, 0, 0, 0);
-            w[0][4 * i] = x.x; w[0][4 * i + 1] = x.y; w[0][4 * i + 2] = x.z; w[0][4 * i + 3] = x.w;
-        }
-    } else {
+    for (int i = 0; i < 8; ++i) {
+        a[i] = -INFINITY;
 #pragma unroll
-        for (int i = 0; i < W / 2; ++i) {
-            const float4 x = valid ? reinterpret_cast<const float4*>(src)[i] : make_float4(0.f, 0.f, 0.f, 0.f);
-            const uint32_t h0 = cvt_bf16x2(x.x, x.y), h1 = cvt_bf16x2(x.z, x.w);
-            w[0][2 * i] = h0;
-            w[0][2 * i + 1] = h1;
-            w[TERMS - 1][2 * i] = cvt_bf16x2(x.x - lo_f(h0), x.y - hi_f(h0));
-            w[TERMS - 1][2 * i + 1] = cvt_bf16x2(x.z - lo_f(h1), x.w - hi_f(h1));
+        for (int k = 0; k < 4; ++k) {
+            const float x = __uint_as_float(v[4 * i + k]);
+            a[i] = fmaxf(a[i], (!MASK || 4 * i + k < lim) ? x : -INFINITY);
         }
     }
 #pragma unroll
-    for (int t = 0; t < TERMS; ++t) tmem_st(taddr + TM_Q + t * (HD / 2) + hf * W, w[t]);
+    for (int w = 4; w >= 1; w >>= 1)
+#pragma unroll
+        for (int i = 0; i < w; ++i) a[i] = fmaxf(a[i], a[i + w]);
+    return a[0];
 }
 
-// P = 2^(s * scale - msc) of 32 positions, packed as bf16 words: hi (and, with two
-// terms, the rounding residuals lo); the fp32 values add up in l.  Positions at or
+// P = 2^(s * scale - msc) of 32 positions as bf16 words (two positions each) into
+// the TMEM columns from `col` on: hi there and, with two terms, the rounding
+// residuals lo 64 columns behind; the fp32 values add up in l.  Positions at or
 // behind lim get 0.
 template <int TERMS, bool MASK>
 __device__ __forceinline__ void exp32(const uint32_t (&v)[32], float scale, float msc, int lim, float2& l,
-                                      uint32_t* ph, uint32_t* pl) {
+                                      uint32_t col) {
     const float2 sc = make_float2(scale, scale), nm = make_float2(-msc, -msc);
+    uint32_t ph[16], pl[16];
 #pragma unroll
     for (int c = 0; c < 16; ++c) {
         const float2 d = __ffma2_rn(make_float2(__uint_as_float(v[2 * c]), __uint_as_float(v[2 * c + 1])), sc, nm);
@@ -192,28 +212,71 @@ __device__ __forceinline__ void exp32(const uint32_t (&v)[32], float scale, floa
             pl[c] = cvt_bf16x2(r.x, r.y);
         }
     }
+    tmem_st16(col, ph);
+    if (TERMS == 2) tmem_st16(col + 64, pl);
 }
 
-template <bool MASK>
-__device__ __forceinline__ float max32(const uint32_t (&v)[32], int lim) {
-    float a[8];
+// 16 consecutive columns of this thread's TMEM lane.
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_wait_ld16(uint32_t (&r)[16]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                   "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]),
+                   "+r"(r[15])::"memory");
+}
+
+// Half a query row of fp32 (64-dim halves of HD dims) as hi and lo bf16 words into
+// the two Q tiles: row r of a box is 128 bytes, its 16-byte chunk c at c ^ (r % 8).
+template <int HD>
+__device__ __forceinline__ void store_q_terms(const float* src, bool valid, unsigned char* q, int r, int half) {
+    constexpr int D = HD / 2;                    // dims of this thread
 #pragma unroll
-    for (int i = 0; i < 8; ++i) a[i] = -INFINITY;
-#pragma unroll
-    for (int i = 0; i < 32; ++i) {
-        const float x = __uint_as_float(v[i]);
-        a[i & 7] = fmaxf(a[i & 7], (!MASK || i < lim) ? x : -INFINITY);
+    for (int c = 0; c < D / 8; ++c) {
+        float4 x = make_float4(0.f, 0.f, 0.f, 0.f), y = x;
+        if (valid) {
+            x = reinterpret_cast<const float4*>(src)[2 * c];
+            y = reinterpret_cast<const float4*>(src)[2 * c + 1];
+        }
+        const uint4 h = make_uint4(cvt_bf16x2(x.x, x.y), cvt_bf16x2(x.z, x.w), cvt_bf16x2(y.x, y.y), cvt_bf16x2(y.z, y.w));
+        const uint4 l = make_uint4(cvt_bf16x2(x.x - lo_f(h.x), x.y - hi_f(h.x)), cvt_bf16x2(x.z - lo_f(h.y), x.w - hi_f(h.y)),
+                                   cvt_bf16x2(y.x - lo_f(h.z), y.y - hi_f(h.z)), cvt_bf16x2(y.z - lo_f(h.w), y.w - hi_f(h.w)));
+        const int d = half * D + 8 * c, chunk = ((d & 63) >> 3) ^ (r & 7);
+        unsigned char* at = q + (d >> 6) * kBlock + r * 128 + chunk * 16;
+        *reinterpret_cast<uint4*>(at) = h;
+        *reinterpret_cast<uint4*>(at + (HD / 64) * kBlock) = l;
     }
+}
+
+// N dims of an output row, scaled, in the output type.
+template <typename T, int N>
+__device__ __forceinline__ void store_out(T* dst, const float (&o)[N], float inv) {
+    if constexpr (sizeof(T) == 4) {
 #pragma unroll
-    for (int w = 4; w >= 1; w >>= 1)
+        for (int i = 0; i < N; i += 4)
+            *reinterpret_cast<float4*>(dst + i) = make_float4(o[i] * inv, o[i + 1] * inv, o[i + 2] * inv, o[i + 3] * inv);
+    } else {
 #pragma unroll
-        for (int i = 0; i < w; ++i) a[i] = fmaxf(a[i], a[i + w]);
-    return a[0];
+        for (int i = 0; i < N; i += 8)
+            *reinterpret_cast<uint4*>(dst + i) =
+                make_uint4(cvt_bf16x2(o[i] * inv, o[i + 1] * inv), cvt_bf16x2(o[i + 2] * inv, o[i + 3] * inv),
+                           cvt_bf16x2(o[i + 4] * inv, o[i + 5] * inv), cvt_bf16x2(o[i + 6] * inv, o[i + 7] * inv));
+    }
 }
 
 template <typename T, int HD>
 __global__ void __launch_bounds__(kThreads, 1) group_kernel(const __grid_constant__ TGKvGroupParams p) {
     constexpr int TERMS = sizeof(T) == 4 ? 2 : 1;
+    // With two terms (fp32 results) an accumulator takes at most 8 tiles, 128 steps of
+    // 16 positions: the tensor core's fp32 sums round towards zero, and the sums of
+    // longer runs would lose more bits than the two terms keep.
+    constexpr uint32_t kMost = TERMS == 2 ? 16 : 0;
     using C = Cfg<HD>;
     extern __shared__ unsigned char smem_raw[];
     unsigned char* base =
@@ -221,10 +284,14 @@ __global__ void __launch_bounds__(kThreads, 1) group_kernel(const __grid_constan
     const uint32_t sbase = smem_addr(base);
     uint64_t* bar = reinterpret_cast<uint64_t*>(base + C::OFF_BAR);
     uint32_t* tslot = reinterpret_cast<uint32_t*>(base + C::OFF_SLOT);
-    float* sm_x = reinterpret_cast<float*>(base + C::OFF_X);
-    float* sm_l = reinterpret_cast<float*>(base + C::OFF_L);
+    uint32_t* tok0 = reinterpret_cast<uint32_t*>(base + C::OFF_TAB);
+    uint32_t* old_len = tok0 + p.n_seq + 1;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
+    for (uint32_t i = tid; i <= p.n_seq; i += kThreads) {
+        tok0[i] = p.tok0[i];
+        if (i < p.n_seq) old_len[i] = p.old_len[i];
+    }
     if (tid == 0) {
         for (int i = 0; i < C::kStages; ++i) {
             mbar_init(&bar[C::B_KFULL + i], 1);
@@ -232,12 +299,13 @@ __global__ void __launch_bounds__(kThreads, 1) group_kernel(const __grid_constan
             mbar_init(&bar[C::B_VFULL + i], 1);
             mbar_init(&bar[C::B_VEMPTY + i], 1);
         }
-        for (int i = 0; i < 2; ++i) {
-            mbar_init(&bar[C::B_SFULL + i], 1);
-            mbar_init(&bar[C::B_PFULL + i], kSoftmaxThreads);
+        for (int h = 0; h < 2; ++h) {
+            mbar_init(&bar[C::B_SFULL + h], 1);
+            mbar_init(&bar[C::B_PFULL + h], 128);
+            mbar_init(&bar[C::B_PVDONE + h], 1);
         }
-        mbar_init(&bar[C::B_PVDONE], 1);
-        mbar_init(&bar[C::B_QREADY], kSoftmaxThreads);
+        mbar_init(&bar[C::B_QFULL], TERMS == 2 ? 256 : 1);
+        mbar_init(&bar[C::B_QEMPTY], 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == kMmaWarp) {
@@ -248,257 +316,299 @@ __global__ void __launch_bounds__(kThreads, 1) group_kernel(const __grid_constan
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *tslot;
-    const uint32_t G = p.n_heads / p.n_kv_heads, tpt = kRows / G;
-    const uint32_t total_rows = p.tok0[p.n_seq] * p.n_heads;
+    const uint32_t G = p.n_heads / p.n_kv_heads;
+    const TGKvGroupShape sh = shape_of(p, old_len, tok0);
     // Everything above overlaps the previous kernel on the stream.
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
-    Pieces pc(p, blockIdx.x);
-    if (warp == kTmaWarp) {
-        if (lane == 0) {
-            uint32_t n = 0;                      // tiles issued
+    Pieces pc(sh, start_of(p, blockIdx.x), start_of(p, blockIdx.x + 1), kMost);
+    if (warp >= 8) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsOther));
+        if (warp == kTmaWarp && lane == 0) {
+            uint32_t nk = 0, nv = 0, it = 0;     // K and V tiles and pieces issued
             bool ok = true;
-            for (; ok && pc.more(); pc.next(p)) {
-                const uint32_t npre = tgkv_group_prefix_tiles(&p, pc.at.seq);
+            for (; ok && pc.more(); pc.next(sh, kMost)) {
+                const uint32_t seq = pc.at.seq, npre = tgkv_group_prefix_tiles(&sh, seq);
+                const uint32_t t0 = pc.at.at * sh.item_tokens;
+                const bool wide = TERMS == 1 && tgkv_group_tokens(&sh, seq) - t0 > sh.tpt;
                 const int x = (int)(pc.at.kvh * HD);
-                for (uint32_t j = pc.j0; j < pc.j1; ++j, ++n) {
+                for (uint32_t j = pc.j0; j < pc.j1; ++j) {
                     const bool own = j >= npre;
-                    const uint64_t map = p.tmaps + 128ull * (own ? pc.at.seq - 1 : p.n_seq);
+                    const uint64_t map = p.tmaps + 128ull * (own ? seq - 1 : p.n_seq);
                     const int y = (int)((own ? j - npre : j) * kPos);
-                    const uint32_t s = n % C::kStages, ph = (n / C::kStages - 1) & 1u;
-                    if (n >= C::kStages && !(ok = mbar_wait(&bar[C::B_KEMPTY + s], ph))) break;
+                    const uint32_t s = nk % C::kStages, ph = (nk / C::kStages - 1) & 1u;
+                    if (nk >= C::kStages && !(ok = mbar_wait(&bar[C::B_KEMPTY + s], ph))) break;
                     mbar_arrive_expect_tx(&bar[C::B_KFULL + s], C::kTile);
                     for (int b = 0; b < HD / 64; ++b)
                         tma_load_3d(base + C::OFF_K + s * C::kTile + b * kBlock, map, x + 64 * b, y, 0,
                                     &bar[C::B_KFULL + s]);
-                    if (n >= C::kStages && !mbar_wait(&bar[C::B_VEMPTY + s], ph)) {
-                        // the K copy just issued lands before the CTA ends
-                        mbar_wait(&bar[C::B_KFULL + s], (n / C::kStages) & 1u);
-                        ok = false;
-                        break;
+                    ++nk;
+                    if (TERMS == 1 && j == pc.j0) {
+                        // the piece's Q, once the last piece's scores are made
+                        if (it > 0 && !(ok = mbar_wait(&bar[C::B_QEMPTY], (it - 1) & 1u))) break;
+                        const uint32_t box = 64 * 2 * G * sh.tpt;
+                        mbar_arrive_expect_tx(&bar[C::B_QFULL], box * (HD / 64) * (wide ? 2 : 1));
+                        const int tok = (int)((seq ? tok0[seq - 1] : 0) + t0);
+                        for (int h = 0; h < (wide ? 2 : 1); ++h)
+                            for (int b = 0; b < HD / 64; ++b)
+                                tma_load_3d(base + C::OFF_Q + h * C::kTile + b * kBlock,
+                                            reinterpret_cast<uint64_t>(&p.qmap), 64 * b, (int)(pc.at.kvh * G),
+                                            tok + h * (int)sh.tpt, &bar[C::B_QFULL]);
+                        ++it;
                     }
+                    if (nv >= C::kStages && !(ok = mbar_wait(&bar[C::B_VEMPTY + s], ph))) break;
                     mbar_arrive_expect_tx(&bar[C::B_VFULL + s], C::kTile);
                     for (int b = 0; b < HD / 64; ++b)
                         tma_load_3d(base + C::OFF_V + s * C::kTile + b * kBlock, map, x + 64 * b, y, 1,
                                     &bar[C::B_VFULL + s]);
+                    ++nv;
                 }
             }
-            if (!ok) atomicExch(p.err, kErrTimeout);
             // every copy has landed before the CTA may end (at once in a normal run)
-            for (uint32_t i = n > C::kStages ? n - C::kStages : 0; i < n; ++i) {
-                const uint32_t s = i % C::kStages, ph = (i / C::kStages) & 1u;
-                if (!mbar_wait(&bar[C::B_KFULL + s], ph) || !mbar_wait(&bar[C::B_VFULL + s], ph))
-                    atomicExch(p.err, kErrTimeout);
-            }
-        }
-        __syncwarp();
-    } else if (warp == kMmaWarp) {
-        if (lane == 0) {
+            for (uint32_t i = nk > C::kStages ? nk - C::kStages : 0; i < nk; ++i)
+                ok = mbar_wait(&bar[C::B_KFULL + i % C::kStages], (i / C::kStages) & 1u) && ok;
+            for (uint32_t i = nv > C::kStages ? nv - C::kStages : 0; i < nv; ++i)
+                ok = mbar_wait(&bar[C::B_VFULL + i % C::kStages], (i / C::kStages) & 1u) && ok;
+            if (TERMS == 1 && it > 0) ok = mbar_wait(&bar[C::B_QFULL], (it - 1) & 1u) && ok;
+            if (!ok) atomicExch(p.err, kErrTimeout);
+        } else if (warp == kMmaWarp && lane == 0) {
             constexpr uint32_t id_s = umma_idesc_bf16(kRows, kPos, 0, 0);
             constexpr uint32_t id_pv = umma_idesc_bf16(kRows, HD, 0, 1);
-            // S of tile n into buffer n % 2: head dims 16 ks .. +15 of Q term t are the 8
-            // columns at t * HD / 2 + 8 ks; K is K-major
-            auto issue_s = [&](uint32_t n) -> bool {
-                const uint32_t s = n % C::kStages, b = n & 1u;
-                if (!mbar_wait(&bar[C::B_KFULL + s], (n / C::kStages) & 1u)) return false;
+            // Step k of a piece belongs to stream k % 2; its K/V tile is g0 + k / 2 (wide, both
+            // streams read it) or g0 + k (narrow).
+            uint32_t g0 = 0, it = 0;             // K/V tiles of earlier pieces; pieces
+            uint32_t done0 = 0, done1 = 0;       // PVs issued per stream
+            bool ok = true;
+            // S into stream h's buffer, once its last PV has read the P there
+            auto issue_s = [&](uint32_t h, uint32_t g, bool wide, bool last) -> bool {
+                const uint32_t n = h ? done1 : done0, s = g % C::kStages;
+                if (n > 0 && !mbar_wait(&bar[C::B_PVDONE + h], (n - 1) & 1u)) return false;
+                if (!mbar_wait(&bar[C::B_KFULL + s], (g / C::kStages) & 1u)) return false;
                 tc_fence_after();
                 const uint64_t kd = umma_desc_sw128(sbase + C::OFF_K + s * C::kTile, 16, 1024);
+                const uint64_t qd = umma_desc_sw128(sbase + C::OFF_Q + (wide && h ? C::kTile : 0u), 16, 1024);
 #pragma unroll
                 for (uint32_t i = 0; i < TERMS * (HD / 16); ++i) {
                     const uint32_t t = i / (HD / 16), ks = i % (HD / 16);
-                    const uint32_t bo = (ks >> 2) * kBlock + (ks & 3u) * 32u;
-                    umma_ts(tmem + TM_S + b * 128u, tmem + TM_Q + t * (HD / 2) + ks * 8u, kd + (bo >> 4), id_s, i != 0);
+                    const uint32_t off = (ks >> 2) * kBlock + (ks & 3u) * 32u;
+                    umma_ss(tmem + TM_S + h * 128u, qd + ((t * C::kTile + off) >> 4), kd + (off >> 4), id_s, i != 0);
                 }
-                umma_commit(&bar[C::B_KEMPTY + s]);
-                umma_commit(&bar[C::B_SFULL + b]);
+                if (!wide || h) umma_commit(&bar[C::B_KEMPTY + s]);
+                if (last) umma_commit(&bar[C::B_QEMPTY]);
+                umma_commit(&bar[C::B_SFULL + h]);
                 return true;
             };
-            uint32_t n = 0, it = 0;
-            bool ok = true;
-            for (; ok && pc.more(); pc.next(p), ++it) {
-                const uint32_t end = n + (pc.j1 - pc.j0), first = n;
-                ok = mbar_wait(&bar[C::B_QREADY], it & 1u);
+            for (; ok && pc.more(); pc.next(sh, kMost), ++it) {
+                const bool wide = TERMS == 1 && tgkv_group_tokens(&sh, pc.at.seq) - pc.at.at * sh.item_tokens > sh.tpt;
+                const uint32_t tiles = pc.j1 - pc.j0, steps = wide ? 2 * tiles : tiles;
+                ok = mbar_wait(&bar[C::B_QFULL], it & 1u);
                 tc_fence_after();
-                ok = ok && issue_s(n);
-                if (n + 1 < end) ok = ok && issue_s(n + 1);
-                for (; ok && n < end; ++n) {
-                    const uint32_t s = n % C::kStages, b = n & 1u;
-                    ok = mbar_wait(&bar[C::B_PFULL + b], (n >> 1) & 1u) &&
-                         mbar_wait(&bar[C::B_VFULL + s], (n / C::kStages) & 1u);
+                ok = ok && issue_s(0, g0, wide, steps == 1);
+                if (steps > 1) ok = ok && issue_s(1, wide ? g0 : g0 + 1, wide, steps == 2);
+                for (uint32_t k = 0; ok && k < steps; ++k) {
+                    const uint32_t h = k & 1u, g = g0 + (wide ? k >> 1 : k), s = g % C::kStages;
+                    const uint32_t n = h ? done1 : done0;
+                    ok = mbar_wait(&bar[C::B_PFULL + h], n & 1u) &&
+                         mbar_wait(&bar[C::B_VFULL + s], (g / C::kStages) & 1u);
                     if (!ok) break;
                     tc_fence_after();
-                    // P of positions 16 kk .. +15: 8 columns of half kk / 4, which holds its hi
-                    // words first and its lo words 32 columns behind.  V is MN-major: 64-dim
-                    // blocks 16 KB apart, 8-position groups 1 KB apart.
+                    // P of positions 16 kk .. +15: 8 columns.  V is MN-major: 64-dim blocks 16 KB
+                    // apart, 8-position groups 1 KB apart.
                     const uint64_t vd = umma_desc_sw128(sbase + C::OFF_V + s * C::kTile, kBlock, 1024);
 #pragma unroll
                     for (uint32_t i = 0; i < TERMS * 8; ++i) {
                         const uint32_t t = i >> 3, kk = i & 7u;
-                        const uint32_t a = tmem + TM_S + b * 128u + (kk >> 2) * 64u + t * 32u + (kk & 3u) * 8u;
-                        umma_ts(tmem + TM_O, a, vd + ((kk * 16u * 128u) >> 4), id_pv, n != first || i != 0);
+                        umma_ts(tmem + TM_O + h * 128u, tmem + TM_S + h * 128u + t * 64u + kk * 8u,
+                                vd + ((kk * 16u * 128u) >> 4), id_pv, k > 1 || i != 0);
                     }
-                    umma_commit(&bar[C::B_VEMPTY + s]);
-                    umma_commit(&bar[C::B_PVDONE]);
-                    if (n + 2 < end) {
-                        // S of tile n + 2 goes where PV of tile n reads P
-                        ok = mbar_wait(&bar[C::B_PVDONE], n & 1u);
-                        tc_fence_after();
-                        ok = ok && issue_s(n + 2);
-                    }
+                    if (!wide || h) umma_commit(&bar[C::B_VEMPTY + s]);
+                    umma_commit(&bar[C::B_PVDONE + h]);
+                    if (h) ++done1;
+                    else ++done0;
+                    if (k + 2 < steps) ok = issue_s(h, g0 + (wide ? (k + 2) >> 1 : k + 2), wide, k + 3 == steps);
                 }
+                g0 += tiles;
             }
             if (!ok) atomicExch(p.err, kErrTimeout);
         }
         __syncwarp();
     } else {
-        const int quarter = warp & 3, hf = warp >> 2, r = quarter * 32 + lane;
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoftmax));
+        const int quarter = warp & 3, h = warp >> 2, r = quarter * 32 + lane;
         const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16);
+        const uint32_t ts = lanes + TM_S + (uint32_t)h * 128u, to = lanes + TM_O + (uint32_t)h * 128u;
+        float2* ml = reinterpret_cast<float2*>(base + C::OFF_ML);
         const float scale = p.qscale;
-        const uint32_t tok = (uint32_t)r / G, sub = (uint32_t)r % G;
-        uint32_t n = 0;
+        const uint32_t rtok = (uint32_t)r / G, sub = (uint32_t)r % G;
+        const uint32_t total_rows = tok0[p.n_seq] * p.n_heads;
+        uint32_t g0 = 0, it = 0, n = 0;          // K/V tiles of earlier pieces; pieces; this stream's steps
         bool ok = true;
-        // Both warps of a pair meet at a named barrier every tile, so neither
-        // leaves early: after a failed wait a warp only keeps the barrier count.
-        for (; pc.more(); pc.next(p)) {
-            const uint32_t seq = pc.at.seq, npre = tgkv_group_prefix_tiles(&p, seq);
-            const uint32_t t0 = pc.at.rt * tpt, ntok = min(tpt, tgkv_group_tokens(&p, seq) - t0);
-            const uint32_t own_rows = seq ? tgkv_group_own_rows(&p, seq, pc.at.rt) : 0;
-            const uint32_t own_min = seq ? p.old_len[seq - 1] + t0 + 1 : 0;      // rows its first token sees
-            const bool valid = tok < ntok;
-            const uint64_t row = (uint64_t)((seq ? p.tok0[seq - 1] : 0) + t0 + tok) * p.n_heads + pc.at.kvh * G + sub;
-            load_q<T, HD, TERMS>(p, valid, row, hf, lanes);
-            tmem_wait_st();
-            tc_fence_before();
-            mbar_arrive(&bar[C::B_QREADY]);
+        // Both warps of a pair meet at named barriers, so neither leaves early:
+        // after a failed wait a warp only keeps the barriers' counts.
+        for (; pc.more(); pc.next(sh, kMost), ++it) {
+            const uint32_t seq = pc.at.seq, npre = tgkv_group_prefix_tiles(&sh, seq);
+            const uint32_t t0 = pc.at.at * sh.item_tokens, left = tgkv_group_tokens(&sh, seq) - t0;
+            const bool wide = TERMS == 1 && left > sh.tpt;
+            const uint32_t tb = wide && h ? sh.tpt : 0;                       // this stream's first token of the item
+            const uint32_t ntok = min(sh.tpt, left - tb);
+            const bool valid = rtok < ntok;
+            const bool busy = (uint32_t)(quarter * 32) < ntok * G;            // the warp has rows
+            const uint32_t own_rows = seq ? tgkv_group_own_rows(&sh, seq, pc.at.at) : 0;
+            const uint32_t own_min = seq ? old_len[seq - 1] + t0 + tb + 1 : 0;   // rows the stream's first token sees
+            const uint64_t row = (uint64_t)((seq ? tok0[seq - 1] : 0) + t0 + tb + rtok) * p.n_heads + pc.at.kvh * G + sub;
+            const uint32_t tiles = pc.j1 - pc.j0, steps = wide ? 2 * tiles : tiles;
+            if constexpr (TERMS == 2) {
+                if (ok && it > 0) ok = __all_sync(0xffffffffu, mbar_wait(&bar[C::B_QEMPTY], (it - 1) & 1u));
+                store_q_terms<HD>(reinterpret_cast<const float*>(p.q) + row * HD + h * (HD / 2), valid,
+                                  base + C::OFF_Q, r, h);
+                fence_proxy_async_smem();
+                mbar_arrive(&bar[C::B_QFULL]);
+            }
 
             float m = -INFINITY;                 // running maximum of the raw scores
             float2 l2 = make_float2(0.f, 0.f);
-            for (uint32_t j = pc.j0; j < pc.j1; ++j, ++n) {
-                const uint32_t b = n & 1u, s = n % C::kStages;
+            for (uint32_t k = (uint32_t)h; k < steps; k += 2, ++n) {
+                const uint32_t t = wide ? k >> 1 : k, j = pc.j0 + t, g = g0 + t;
                 const bool own = j >= npre;
                 const uint32_t pos = (own ? j - npre : j) * kPos;
-                const uint32_t rows = own ? own_rows : p.prefix_len;             // rows some query of the tile sees
+                const uint32_t rows = own ? own_rows : p.prefix_len;             // rows some query of the item sees
                 const bool mask = pos + kPos > (own ? own_min : p.prefix_len);
-                const int lim = (int)((own ? own_min + min(tok, ntok - 1) : p.prefix_len) - pos) - hf * 64;
-                const uint32_t sp = lanes + TM_S + b * 128u + (uint32_t)hf * 64u;
-                if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&bar[C::B_SFULL + b], (n >> 1) & 1u));
+                if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&bar[C::B_SFULL + h], n & 1u));
                 if (ok) tc_fence_after();
-                if (ok && pos + kPos > rows && hf == 0) {
-                    // V rows that no query of this tile sees may hold anything; P is 0 there, but
-                    // 0 * Inf is NaN, so they are cleared before PV reads them
-                    ok = __all_sync(0xffffffffu, mbar_wait(&bar[C::B_VFULL + s], (n / C::kStages) & 1u));
-                    if (ok && pos + (uint32_t)r >= rows)
+                if (ok && pos + kPos > rows && (!wide || h == 0)) {
+                    // V rows that no query of the item sees may hold anything; P is 0 there, but
+                    // 0 * Inf is NaN, so they are cleared before a PV reads them (in wide pieces
+                    // stream 0's comes first)
+                    const uint32_t s = g % C::kStages;
+                    ok = __all_sync(0xffffffffu, mbar_wait(&bar[C::B_VFULL + s], (g / C::kStages) & 1u));
+                    if (ok)
+                        for (uint32_t y = rows - pos + ((uint32_t)r >> 3); y < kPos; y += 16)
 #pragma unroll
-                        for (int c = 0; c < HD / 64; ++c)
-#pragma unroll
-                            for (int q = 0; q < 8; ++q)
-                                *reinterpret_cast<uint4*>(base + C::OFF_V + s * C::kTile + c * kBlock + r * 128 +
-                                                          q * 16) = make_uint4(0u, 0u, 0u, 0u);
+                            for (int c = 0; c < HD / 64; ++c)
+                                *reinterpret_cast<uint4*>(base + C::OFF_V + s * C::kTile + c * kBlock + y * 128 +
+                                                          (r & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
+                    __syncwarp();
                     fence_proxy_async_smem();
                 }
-                uint32_t va[32], vb[32];
-                float tm = -INFINITY;
-                if (ok) {
-                    tmem_ld32(sp, va);
-                    tmem_ld32(sp + 32, vb);
-                    tmem_wait_ld(va, vb);
-                    tm = mask ? fmaxf(max32<true>(va, lim), max32<true>(vb, lim - 32))
-                              : fmaxf(max32<false>(va, 0), max32<false>(vb, 0));
-                }
-                float* x = sm_x + b * 2 * kRows;
-                x[hf * kRows + r] = tm;
-                pair_sync(quarter);
-                tm = fmaxf(tm, x[(hf ^ 1) * kRows + r]);
-                if (ok) {
+                if (ok && busy) {
+                    Scores v;
+                    load_scores(ts, v);
+                    const int lim = (int)((own ? own_min + min(rtok, ntok - 1) : p.prefix_len) - pos);
+                    float tm;
+                    if (mask)
+                        tm = fmaxf(fmaxf(max32<true>(v.c[0], lim), max32<true>(v.c[1], lim - 32)),
+                                   fmaxf(max32<true>(v.c[2], lim - 64), max32<true>(v.c[3], lim - 96)));
+                    else
+                        tm = fmaxf(fmaxf(max32<false>(v.c[0], 0), max32<false>(v.c[1], 0)),
+                                   fmaxf(max32<false>(v.c[2], 0), max32<false>(v.c[3], 0)));
                     // the running maximum moves only when exceeded by more than 2^8
                     const bool grow = (tm - m) * scale > 8.f;
-                    float alpha = 1.f;
-                    if (grow) {
-                        alpha = m == -INFINITY ? 0.f : ex2_approx((m - tm) * scale);
-                        m = tm;
-                        l2.x *= alpha;
-                        l2.y *= alpha;
-                    }
-                    if (j > pc.j0 && __any_sync(0xffffffffu, grow)) {
-                        ok = __all_sync(0xffffffffu, mbar_wait(&bar[C::B_PVDONE], (n - 1) & 1u));
-                        if (ok) {
-                            tc_fence_after();
+                    const float alpha = !grow ? 1.f : m == -INFINITY ? 0.f : ex2_approx((m - tm) * scale);
+                    if (grow) m = tm;
+                    l2.x *= alpha;
+                    l2.y *= alpha;
+                    if (k > 1 && __any_sync(0xffffffffu, grow)) {
+                        // (the stream's last PV was complete before this S was made)
 #pragma unroll
-                            for (int c = 0; c < HD / 64; ++c) {
-                                uint32_t o[32];
-                                const uint32_t oc = lanes + TM_O + (uint32_t)hf * (HD / 2) + c * 32;
-                                tmem_ld32(oc, o);
-                                tmem_wait_ld(o);
+                        for (int c = 0; c < HD / 16; ++c) {
+                            uint32_t o[16];
+                            tmem_ld16(to + c * 16, o);
+                            tmem_wait_ld16(o);
 #pragma unroll
-                                for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
-                                tmem_st32(oc, o);
-                            }
+                            for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+                            tmem_st16(to + c * 16, o);
                         }
                     }
-                }
-                if (ok) {
                     const float msc = m == -INFINITY ? 0.f : m * scale;
-                    uint32_t ph[32], pl[32];
                     if (mask) {
-                        exp32<TERMS, true>(va, scale, msc, lim, l2, ph, pl);
-                        exp32<TERMS, true>(vb, scale, msc, lim - 32, l2, ph + 16, pl + 16);
+#pragma unroll
+                        for (int c = 0; c < 4; ++c) exp32<TERMS, true>(v.c[c], scale, msc, lim - 32 * c, l2, ts + 16 * c);
                     } else {
-                        exp32<TERMS, false>(va, scale, msc, 0, l2, ph, pl);
-                        exp32<TERMS, false>(vb, scale, msc, 0, l2, ph + 16, pl + 16);
+#pragma unroll
+                        for (int c = 0; c < 4; ++c) exp32<TERMS, false>(v.c[c], scale, msc, 0, l2, ts + 16 * c);
                     }
-                    tmem_st32(sp, ph);
-                    if (TERMS == 2) tmem_st32(sp + 32, pl);
+                    tmem_wait_st();
                 }
-                tmem_wait_st();
                 tc_fence_before();
-                mbar_arrive(&bar[C::B_PFULL + b]);
+                mbar_arrive(&bar[C::B_PFULL + h]);
             }
-            // the rows' sums over both halves, and O once the last PV is complete
-            sm_l[hf * kRows + r] = l2.x + l2.y;
-            pair_sync(quarter);
-            const float l = sm_l[r] + sm_l[kRows + r];
-            if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&bar[C::B_PVDONE], (n - 1) & 1u));
+            g0 += tiles;
+
+            // ---- the piece's rows: out, or a partial
+            const bool mine = (uint32_t)h < steps;                               // this stream had a tile
+            if (ok && mine) ok = __all_sync(0xffffffffu, mbar_wait(&bar[C::B_PVDONE + h], (n - 1) & 1u));
             if (ok) tc_fence_after();
-            const bool whole = pc.j0 == 0 && pc.j1 == pc.nt && !p.share;
+            float l = l2.x + l2.y, msc = m * scale;                              // -inf if nothing was seen
+            float w0 = 1.f, w1 = 0.f;                                            // weights of the streams' O
+            if (!wide) {
+                // both streams have the same rows: join (m, l), then each brings out half of the
+                // head dims from both O
+                ml[h * kRows + r] = make_float2(msc, l);
+                tc_fence_before();
+                pair_sync(quarter);
+                tc_fence_after();
+                const float2 a = ml[r], b = ml[kRows + r];
+                msc = fmaxf(a.x, b.x);
+                w0 = a.x == -INFINITY ? 0.f : ex2_approx(a.x - msc);
+                w1 = b.x == -INFINITY ? 0.f : ex2_approx(b.x - msc);
+                l = a.y * w0 + b.y * w1;
+            }
+            const bool whole = pc.first == 0 && pc.j1 == pc.nt && !p.share;
+            const bool again = pc.j0 > pc.first;                                 // adds to the item's earlier piece here
+            const uint32_t irow = (wide ? (uint32_t)h * kRows : 0u) + (uint32_t)r;
             uint64_t slot;
-            if (pc.j0 > 0 || !p.share) slot = (uint64_t)p.cta_rows + 256u * blockIdx.x + (pc.j0 > 0 ? 0u : 128u) + r;
+            if (pc.first > 0 || !p.share) slot = (uint64_t)p.cta_rows + 512u * blockIdx.x + (pc.first > 0 ? 0u : 256u) + irow;
             else slot = (seq ? total_rows : 0u) + row;
+            float keep = 0.f, mine_w = 1.f;                                      // weights of the slot and of this piece
+            float2* slot_ml = reinterpret_cast<float2*>(p.part_ml) + slot;
+            if (TERMS == 2 && again && valid) {
+                const float2 old = *slot_ml;
+                const float M = fmaxf(old.x, msc);
+                keep = old.x == -INFINITY ? 0.f : ex2_approx(old.x - M);
+                mine_w = msc == -INFINITY ? 0.f : ex2_approx(msc - M);
+                l = l * mine_w + old.y * keep;
+                msc = M;
+                w0 *= mine_w;
+                w1 *= mine_w;
+            }
+            if (TERMS == 2 && again) pair_sync(quarter);                         // both warps have read the slot's (m, l)
             const float inv = 1.f / l;
-#pragma unroll
-            for (int c = 0; c < HD / 64; ++c) {
-                uint32_t o[32];
-                if (ok) {
-                    tmem_ld32(lanes + TM_O + (uint32_t)hf * (HD / 2) + c * 32, o);
-                    tmem_wait_ld(o);
-                }
-                if (!ok || !valid) continue;
-                const uint32_t col = (uint32_t)hf * (HD / 2) + c * 32;
-                if (!whole) {
-                    uint4* dst = reinterpret_cast<uint4*>(p.part_o + slot * HD + col);
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) dst[i] = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
-                } else if constexpr (TERMS == 2) {
-                    float4* dst = reinterpret_cast<float4*>(reinterpret_cast<float*>(p.out) + row * HD + col);
-#pragma unroll
-                    for (int i = 0; i < 8; ++i)
-                        dst[i] = make_float4(__uint_as_float(o[4 * i]) * inv, __uint_as_float(o[4 * i + 1]) * inv,
-                                             __uint_as_float(o[4 * i + 2]) * inv, __uint_as_float(o[4 * i + 3]) * inv);
-                } else {
-                    uint4* dst = reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(p.out) + row * HD + col);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        uint32_t w[4];
-#pragma unroll
-                        for (int k = 0; k < 4; ++k)
-                            w[k] = cvt_bf16x2(__uint_as_float(o[8 * i + 2 * k]) * inv,
-                                              __uint_as_float(o[8 * i + 2 * k + 1]) * inv);
-                        dst[i] = make_uint4(w[0], w[1], w[2], w[3]);
+            const int c0 = wide ? 0 : h * (HD / 32), c1 = wide ? HD / 16 : c0 + HD / 32;   // columns 16 c .. +15
+            const uint32_t oa = wide ? to : lanes + TM_O;
+#pragma unroll 2
+            for (int c = c0; c < c1; ++c) {
+                uint32_t x[16], y[16];
+                __syncwarp();                    // tcgen05.ld is warp-collective
+                if (ok && busy) {
+                    tmem_ld16(oa + c * 16, x);
+                    if (!wide && steps > 1) {
+                        tmem_ld16(oa + 128 + c * 16, y);
+                        tmem_wait_ld16(y);
                     }
+                    tmem_wait_ld16(x);
+                }
+                if (ok && valid) {
+                    float o[16];
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        o[i] = w0 == 0.f ? 0.f : __uint_as_float(x[i]) * w0;
+                        if (w1 != 0.f) o[i] = fmaf(__uint_as_float(y[i]), w1, o[i]);
+                    }
+                    float* part = p.part_o + slot * HD + c * 16;
+                    if (TERMS == 2 && again)
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) o[i] = fmaf(part[i], keep, o[i]);
+                    if (whole) store_out<T, 16>(reinterpret_cast<T*>(p.out) + row * HD + c * 16, o, inv);
+                    else store_out<float, 16>(part, o, 1.f);
                 }
             }
-            if (ok && valid && !whole && hf == 0)
-                *reinterpret_cast<float2*>(p.part_ml + slot * 2) = make_float2(m * scale, l);
+            if (ok && valid && !whole && (wide || h == 0)) *slot_ml = make_float2(msc, l);
+            if (!wide) {
+                // the other stream has read this one's O and (m, l), and both the slot's rows are written
+                tc_fence_before();
+                pair_sync(quarter);
+            }
         }
         if (!ok && lane == 0) atomicExch(p.err, kErrTimeout);
     }
@@ -567,8 +677,13 @@ __device__ __forceinline__ void add_continued(const TGKvGroupParams& p, Acc<HD>&
         if (!tgkv_group_same_item(s, it)) break;
         const TGKvGroupPos e = start_of(p, b + 1);
         if (tgkv_group_same_item(s, e) && s.tile == e.tile) continue;            // an empty stretch
-        acc.add(p, (uint64_t)p.cta_rows + 256u * b + r, lane);
+        acc.add(p, (uint64_t)p.cta_rows + 512u * b + r, lane);
     }
+}
+
+// The row of an item that head `sub` of its KV head's group has for token t of it.
+__device__ __forceinline__ uint32_t item_row(const TGKvGroupShape& sh, uint32_t t, uint32_t G, uint32_t sub) {
+    return t / sh.tpt * kRows + t % sh.tpt * G + sub;
 }
 
 // share: every query row, from its prefix part and its own part.
@@ -579,19 +694,21 @@ __global__ void __launch_bounds__(256) group_merge_parts_kernel(const __grid_con
     const uint32_t row = blockIdx.x * 8 + (threadIdx.x >> 5), total = p.tok0[p.n_seq] * p.n_heads;
     const int lane = threadIdx.x & 31;
     if (row >= total) return;
-    const uint32_t G = p.n_heads / p.n_kv_heads, tpt = kRows / G;
+    const uint32_t G = p.n_heads / p.n_kv_heads;
+    const TGKvGroupShape sh = shape_of(p, p.old_len, p.tok0);
     const uint32_t t = row / p.n_heads, h = row % p.n_heads, kvh = h / G, sub = h % G;
     const uint32_t i = seq_of(p, t), own = t - p.tok0[i];
     Acc<HD> acc;
     acc.add(p, row, lane);
-    add_continued<HD>(p, acc, TGKvGroupPos{0, kvh, t / tpt, 0}, t % tpt * G + sub, lane);
+    add_continued<HD>(p, acc, TGKvGroupPos{0, kvh, t / sh.item_tokens, 0}, item_row(sh, t % sh.item_tokens, G, sub), lane);
     acc.add(p, (uint64_t)total + row, lane);
-    add_continued<HD>(p, acc, TGKvGroupPos{i + 1, kvh, own / tpt, 0}, own % tpt * G + sub, lane);
+    add_continued<HD>(p, acc, TGKvGroupPos{i + 1, kvh, own / sh.item_tokens, 0},
+                      item_row(sh, own % sh.item_tokens, G, sub), lane);
     acc.template store<T>(p, row, lane);
 }
 
 // joined: the rows of items that several CTAs worked on.  Block (b, y) merges
-// rows 16 y .. +15 of the item that CTA b leaves unfinished and began itself.
+// query rows 16 y .. +15 of the item that CTA b leaves unfinished and began itself.
 template <typename T, int HD>
 __global__ void __launch_bounds__(256) group_merge_split_kernel(const __grid_constant__ TGKvGroupParams p) {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -602,16 +719,16 @@ __global__ void __launch_bounds__(256) group_merge_split_kernel(const __grid_con
     if (e.seq > p.n_seq || e.tile == 0 || (tgkv_group_same_item(s, e) && s.tile > 0)) return;
     TGKvGroupPos it = e;
     it.tile = 0;
-    const uint32_t G = p.n_heads / p.n_kv_heads, tpt = kRows / G, t0 = it.rt * tpt;
-    const uint32_t ntok = min(tpt, tgkv_group_tokens(&p, it.seq) - t0);
+    const uint32_t G = p.n_heads / p.n_kv_heads;
+    const TGKvGroupShape sh = shape_of(p, p.old_len, p.tok0);
+    const uint32_t t0 = it.at * sh.item_tokens, ntok = min(sh.item_tokens, tgkv_group_tokens(&sh, it.seq) - t0);
     const int lane = threadIdx.x & 31;
-    for (uint32_t r = blockIdx.y * 16 + (threadIdx.x >> 5); r < blockIdx.y * 16 + 16; r += 8) {
-        if (r >= ntok * G) continue;
+    for (uint32_t x = blockIdx.y * 16 + (threadIdx.x >> 5); x < blockIdx.y * 16 + 16 && x < ntok * G; x += 8) {
+        const uint32_t t = x / G, sub = x % G, r = item_row(sh, t, G, sub);
         Acc<HD> acc;
-        acc.add(p, (uint64_t)p.cta_rows + 256u * b + 128u + r, lane);
+        acc.add(p, (uint64_t)p.cta_rows + 512u * b + 256u + r, lane);
         add_continued<HD>(p, acc, it, r, lane);
-        const uint64_t row = (uint64_t)(p.tok0[it.seq - 1] + t0 + r / G) * p.n_heads + it.kvh * G + r % G;
-        acc.template store<T>(p, row, lane);
+        acc.template store<T>(p, (uint64_t)(p.tok0[it.seq - 1] + t0 + t) * p.n_heads + it.kvh * G + sub, lane);
     }
 }
 
@@ -659,7 +776,7 @@ int launch(const TGKvGroupParams* p, cudaStream_t st) {
     if (p->share)
         e = launch_pdl(group_merge_parts_kernel<T, HD>, dim3((total * p->n_heads + 7) / 8), 256, 0, st, p);
     else if (p->n_split)
-        e = launch_pdl(group_merge_split_kernel<T, HD>, dim3(p->n_cta, 8), 256, 0, st, p);
+        e = launch_pdl(group_merge_split_kernel<T, HD>, dim3(p->n_cta, 8 * p->pair), 256, 0, st, p);
     return (int)e;
 }
 

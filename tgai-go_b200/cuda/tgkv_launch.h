@@ -201,6 +201,9 @@ typedef struct {
 /* ---- groups of caches with a shared prefix (tgkv_group.cu); the plan is in
  * tgkv_group_plan.h ---- */
 typedef struct {
+    /* bf16 activations: q as a 3-D map (head_dim, n_heads, tokens), 128-byte
+     * swizzle, box (64, G, 128 / G): 64 head dims of a row tile */
+    CUtensorMap qmap;
     const TGKvRowCache* table;   /* device: the n_seq caches, then the prefix cache */
     uint64_t    tmaps;           /* device: their tensor maps (128 bytes each; box 64 dims x
                                   * 128 positions, 128-byte swizzle) */
@@ -216,11 +219,11 @@ typedef struct {
     uint32_t n_seq, n_heads, n_kv_heads, head_dim;
     uint32_t prefix_len;
     float    qscale;             /* softmax scale * log2(e) */
-    uint32_t share, n_cta;
+    uint32_t share, pair, n_cta;
     uint32_t cta_rows;           /* first partial row of the CTAs' slots: CTA b's rows are
-                                  * cta_rows + 256 b + (0: the item it continues, 128: the one
-                                  * it leaves unfinished) + r; below it, with share, query row x's
-                                  * prefix part at x and own part at total rows + x */
+                                  * cta_rows + 512 b + (0: the item it continues, 256: the one
+                                  * it leaves unfinished) + row of the item; below it, with share,
+                                  * query row x's prefix part at x and own part at total + x */
     uint32_t n_split;            /* CTAs that continue an item */
     uint32_t old_len[TGKV_MAX_ITEMS];       /* own rows before the call's tokens */
     uint32_t tok0[TGKV_MAX_ITEMS + 1];      /* first packed token of each sequence; the total */
