@@ -7,22 +7,27 @@
 // of K/V tiles that tgkv_group_plan.h cuts.  A piece is an item (one or two row
 // tiles of 128 query rows of one KV head) against a run of 128-position K/V
 // tiles, in one pass: S = Q K^T, running maximum and sum in the log2 domain,
-// O += P V.  Two streams, each with its own S/P and O in TMEM and its own four
-// softmax warps (one thread per row), take turns on the tensor core: while one
-// stream's scores are exponentiated, the other's products run.
+// O += P V, 64 positions (half a tile) at a time.  Two streams, each with its
+// own O and two S/P buffers in TMEM, its own four softmax warps (one thread per
+// row) and its own MMA warp, run side by side:
 //   wide pieces    (two row tiles) stream h has the rows of row tile h, and both
 //                  read every K/V tile: half the tile traffic per row;
 //   narrow pieces  (one row tile) both have the same rows and take alternate
 //                  tiles; their results join at the end of the piece.
+// With two buffers the scores of a stream's next half tile are made while the
+// softmax works on this one, so the softmax warps hardly wait: the kernel is
+// bound by their instructions and the exponentials (16 a cycle and SM) beside
+// the tensor core (128 x 128 x HD of each product takes 4 HD cycles; scores 1.5
+// times that, since 64-column products read Q from shared memory twice).
 // Warps (384 threads): 0-3 and 4-7 the streams' softmax, 8 TMA (K/V tiles in
 // 64-dim boxes, 128-byte swizzle, into two rings that run ahead over the whole
-// stretch; Q of bf16 calls), 9 the MMAs (one lane).
+// stretch; Q of bf16 calls), 9 and 10 the streams' MMAs (one lane each).
 // TERMS is the number of bf16 terms of q and P: 1 with bf16 activations (q is
 // exact, P is rounded once, 2^-8 of a weight, as the output itself is), 2 with
 // fp32 ones (hi + lo, 16 mantissa bits; a third term of P has no room in the
 // columns S leaves free).  Scores, maxima, sums and O are fp32.
-// TMEM columns: S/P of stream h [128 h, 128 h + 128), P as bf16 pairs (hi at
-// +0, lo at +64); O of stream h [256 + 128 h, +HD).
+// TMEM columns: buffer b of stream h [128 h + 64 b, +64), P there as bf16 pairs
+// (hi at +0, lo at +32); O of stream h [256 + 128 h, +HD).
 //
 // group_merge kernels join the partials of rows whose tiles more than one
 // piece attended: no atomics, always in the same order.
@@ -48,9 +53,7 @@ constexpr int kTmaWarp = 8, kMmaWarp = 9;
 constexpr uint32_t kBlock = 16384;              // 128 rows x 64 bf16: one swizzled box
 constexpr uint32_t TM_S = 0, TM_O = 256, TM_COLS = 512;
 constexpr int kErrTimeout = 7;
-// Registers: the softmax threads hold 128 scores; the launch has 384 x 168.
-constexpr int kRegsSoftmax = 208, kRegsOther = 80;
-static_assert(256 * kRegsSoftmax + 128 * kRegsOther <= 384 * 168, "register split");
+constexpr int kSub = 64;                        // positions of one S: half a tile
 
 template <int HD>
 struct Cfg {
@@ -59,15 +62,17 @@ struct Cfg {
     static constexpr uint32_t OFF_K = 0, OFF_V = kStages * kTile, OFF_Q = 2 * kStages * kTile;
     static constexpr uint32_t OFF_BAR = OFF_Q + 2 * kTile;             // Q: two row tiles, or hi and lo
     static constexpr int B_KFULL = 0, B_KEMPTY = kStages, B_VFULL = 2 * kStages, B_VEMPTY = 3 * kStages;
-    static constexpr int B_SFULL = 4 * kStages;      // [2] a stream's S is in TMEM
-    static constexpr int B_PFULL = B_SFULL + 2;      // [2] its P is written, its O rescaled (128 arrivals)
-    static constexpr int B_PVDONE = B_PFULL + 2;     // [2] its PV is complete
-    static constexpr int B_QFULL = B_PVDONE + 2;     // a piece's Q is in shared memory
+    static constexpr int B_SFULL = 4 * kStages;      // [2 streams][2 buffers] S is in TMEM
+    static constexpr int B_PFULL = B_SFULL + 4;      // [2][2] its P is written, O rescaled (128 arrivals)
+    static constexpr int B_PVDONE = B_PFULL + 4;     // [2] one phase per half tile: its PV is complete
+    static constexpr int B_ODONE = B_PVDONE + 2;     // [2] one phase per piece with steps: O is complete
+    static constexpr int B_QFULL = B_ODONE + 2;      // a piece's Q is in shared memory
     static constexpr int B_QEMPTY = B_QFULL + 1;     // every S of a piece is complete
     static constexpr uint32_t OFF_ML = OFF_BAR + 32 * 8;               // [2 streams][128] (m, l)
     static constexpr uint32_t OFF_SLOT = OFF_ML + 2 * kRows * 8;
     static constexpr uint32_t OFF_TAB = OFF_SLOT + 16;                 // tok0, old_len
-    static constexpr uint32_t SMEM = OFF_TAB + (2 * TGKV_MAX_ITEMS + 1) * 4 + 1024;    // slack: alignment
+    static constexpr uint32_t OFF_STG = (OFF_TAB + (2 * TGKV_MAX_ITEMS + 1) * 4 + 127) / 128 * 128;
+    static constexpr uint32_t SMEM = OFF_STG + 8 * 2048 + 1024;        // 2 KB per softmax warp; slack: alignment
     static_assert(B_QEMPTY < 32 && SMEM <= 232448, "shared memory per CTA");
 };
 
@@ -120,6 +125,21 @@ private:
     }
 };
 
+// What a piece's tiles see: shared by the MMA and softmax warps.
+struct PieceRows {
+    uint32_t npre, prefix_len, own_rows;         // prefix tiles; rows some query of the item sees of each part
+    bool wide;
+    __device__ PieceRows(const TGKvGroupShape& s, const Pieces& pc, int terms)
+        : npre(tgkv_group_prefix_tiles(&s, pc.at.seq)), prefix_len(s.prefix_len),
+          own_rows(pc.at.seq ? tgkv_group_own_rows(&s, pc.at.seq, pc.at.at) : 0),
+          wide(terms == 1 && tgkv_group_tokens(&s, pc.at.seq) - pc.at.at * s.item_tokens > s.tpt) {}
+    __device__ bool own(uint32_t j) const { return j >= npre; }
+    __device__ uint32_t pos(uint32_t j) const { return (j >= npre ? j - npre : j) * kPos; }
+    __device__ uint32_t rows(uint32_t j) const { return j >= npre ? own_rows : prefix_len; }
+    // 64-position halves of tile j that hold rows
+    __device__ uint32_t halves(uint32_t j) const { return rows(j) - pos(j) > kSub ? 2 : 1; }
+};
+
 // The sequence of packed token t: the last one whose first token is at or
 // before t among those with tokens.
 __device__ __forceinline__ uint32_t seq_of(const TGKvGroupParams& p, uint32_t t) {
@@ -157,17 +177,6 @@ __global__ void __launch_bounds__(256) group_append_kernel(const __grid_constant
     asm volatile("fence.proxy.async.global;" ::: "memory");
 }
 
-// 32 consecutive TMEM columns x 4 into v, all loads in flight at once.
-struct Scores { uint32_t c[4][32]; };
-__device__ __forceinline__ void load_scores(uint32_t taddr, Scores& s) {
-    tmem_ld32(taddr, s.c[0]);
-    tmem_ld32(taddr + 32, s.c[1]);
-    tmem_ld32(taddr + 64, s.c[2]);
-    tmem_ld32(taddr + 96, s.c[3]);
-    tmem_wait_ld(s.c[0], s.c[1]);
-    tmem_wait_ld(s.c[2], s.c[3]);
-}
-
 template <bool MASK>
 __device__ __forceinline__ float max32(const uint32_t (&v)[32], int lim) {
     float a[8];
@@ -189,7 +198,7 @@ __device__ __forceinline__ float max32(const uint32_t (&v)[32], int lim) {
 
 // P = 2^(s * scale - msc) of 32 positions as bf16 words (two positions each) into
 // the TMEM columns from `col` on: hi there and, with two terms, the rounding
-// residuals lo 64 columns behind; the fp32 values add up in l.  Positions at or
+// residuals lo 32 columns behind; the fp32 values add up in l.  Positions at or
 // behind lim get 0.
 template <int TERMS, bool MASK>
 __device__ __forceinline__ void exp32(const uint32_t (&v)[32], float scale, float msc, int lim, float2& l,
@@ -213,7 +222,7 @@ __device__ __forceinline__ void exp32(const uint32_t (&v)[32], float scale, floa
         }
     }
     tmem_st16(col, ph);
-    if (TERMS == 2) tmem_st16(col + 64, pl);
+    if (TERMS == 2) tmem_st16(col + 32, pl);
 }
 
 // 16 consecutive columns of this thread's TMEM lane.
@@ -254,29 +263,13 @@ __device__ __forceinline__ void store_q_terms(const float* src, bool valid, unsi
     }
 }
 
-// N dims of an output row, scaled, in the output type.
-template <typename T, int N>
-__device__ __forceinline__ void store_out(T* dst, const float (&o)[N], float inv) {
-    if constexpr (sizeof(T) == 4) {
-#pragma unroll
-        for (int i = 0; i < N; i += 4)
-            *reinterpret_cast<float4*>(dst + i) = make_float4(o[i] * inv, o[i + 1] * inv, o[i + 2] * inv, o[i + 3] * inv);
-    } else {
-#pragma unroll
-        for (int i = 0; i < N; i += 8)
-            *reinterpret_cast<uint4*>(dst + i) =
-                make_uint4(cvt_bf16x2(o[i] * inv, o[i + 1] * inv), cvt_bf16x2(o[i + 2] * inv, o[i + 3] * inv),
-                           cvt_bf16x2(o[i + 4] * inv, o[i + 5] * inv), cvt_bf16x2(o[i + 6] * inv, o[i + 7] * inv));
-    }
-}
-
 template <typename T, int HD>
 __global__ void __launch_bounds__(kThreads, 1) group_kernel(const __grid_constant__ TGKvGroupParams p) {
     constexpr int TERMS = sizeof(T) == 4 ? 2 : 1;
-    // With two terms (fp32 results) an accumulator takes at most 8 tiles, 128 steps of
+    // With two terms (fp32 results) an accumulator takes at most 16 tiles, 256 steps of
     // 16 positions: the tensor core's fp32 sums round towards zero, and the sums of
     // longer runs would lose more bits than the two terms keep.
-    constexpr uint32_t kMost = TERMS == 2 ? 16 : 0;
+    constexpr uint32_t kMost = TERMS == 2 ? 32 : 0;
     using C = Cfg<HD>;
     extern __shared__ unsigned char smem_raw[];
     unsigned char* base =
@@ -295,17 +288,20 @@ __global__ void __launch_bounds__(kThreads, 1) group_kernel(const __grid_constan
     if (tid == 0) {
         for (int i = 0; i < C::kStages; ++i) {
             mbar_init(&bar[C::B_KFULL + i], 1);
-            mbar_init(&bar[C::B_KEMPTY + i], 1);
+            mbar_init(&bar[C::B_KEMPTY + i], 2);
             mbar_init(&bar[C::B_VFULL + i], 1);
-            mbar_init(&bar[C::B_VEMPTY + i], 1);
+            mbar_init(&bar[C::B_VEMPTY + i], 2);
         }
         for (int h = 0; h < 2; ++h) {
-            mbar_init(&bar[C::B_SFULL + h], 1);
-            mbar_init(&bar[C::B_PFULL + h], 128);
+            for (int b = 0; b < 2; ++b) {
+                mbar_init(&bar[C::B_SFULL + 2 * h + b], 1);
+                mbar_init(&bar[C::B_PFULL + 2 * h + b], 128);
+            }
             mbar_init(&bar[C::B_PVDONE + h], 1);
+            mbar_init(&bar[C::B_ODONE + h], 1);
         }
         mbar_init(&bar[C::B_QFULL], TERMS == 2 ? 256 : 1);
-        mbar_init(&bar[C::B_QEMPTY], 1);
+        mbar_init(&bar[C::B_QEMPTY], 2);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == kMmaWarp) {
@@ -324,7 +320,6 @@ __global__ void __launch_bounds__(kThreads, 1) group_kernel(const __grid_constan
 
     Pieces pc(sh, start_of(p, blockIdx.x), start_of(p, blockIdx.x + 1), kMost);
     if (warp >= 8) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsOther));
         if (warp == kTmaWarp && lane == 0) {
             uint32_t nk = 0, nv = 0, it = 0;     // K and V tiles and pieces issued
             bool ok = true;
@@ -372,69 +367,101 @@ __global__ void __launch_bounds__(kThreads, 1) group_kernel(const __grid_constan
                 ok = mbar_wait(&bar[C::B_VFULL + i % C::kStages], (i / C::kStages) & 1u) && ok;
             if (TERMS == 1 && it > 0) ok = mbar_wait(&bar[C::B_QFULL], (it - 1) & 1u) && ok;
             if (!ok) atomicExch(p.err, kErrTimeout);
-        } else if (warp == kMmaWarp && lane == 0) {
-            constexpr uint32_t id_s = umma_idesc_bf16(kRows, kPos, 0, 0);
+        } else if ((warp == kMmaWarp || warp == kMmaWarp + 1) && lane == 0) {
+            // One warp per stream.  Step k of a piece belongs to stream k % 2; its K/V tile is
+            // g0 + k / 2 (wide) or g0 + k (narrow), in one or two halves.  S runs two halves ahead
+            // of PV: PV of a half as soon as its P is there, then the S of the half after next
+            // into the same buffer.  Both warps pass every phase of the rings and of Q, in order,
+            // so that a parity always means the phase it is waited for: a tile or a Q that a
+            // stream does not use, it releases when it sees it.
+            constexpr uint32_t id_s = umma_idesc_bf16(kRows, kSub, 0, 0);
             constexpr uint32_t id_pv = umma_idesc_bf16(kRows, HD, 0, 1);
-            // Step k of a piece belongs to stream k % 2; its K/V tile is g0 + k / 2 (wide, both
-            // streams read it) or g0 + k (narrow).
+            const uint32_t h = (uint32_t)(warp - kMmaWarp);
             uint32_t g0 = 0, it = 0;             // K/V tiles of earlier pieces; pieces
-            uint32_t done0 = 0, done1 = 0;       // PVs issued per stream
+            uint32_t ns = 0, np = 0;             // this stream's S and PV issued
+            uint32_t ks = 0, vs = 0;             // tiles passed in each ring
             bool ok = true;
-            // S into stream h's buffer, once its last PV has read the P there
-            auto issue_s = [&](uint32_t h, uint32_t g, bool wide, bool last) -> bool {
-                const uint32_t n = h ? done1 : done0, s = g % C::kStages;
-                if (n > 0 && !mbar_wait(&bar[C::B_PVDONE + h], (n - 1) & 1u)) return false;
-                if (!mbar_wait(&bar[C::B_KFULL + s], (g / C::kStages) & 1u)) return false;
-                tc_fence_after();
-                const uint64_t kd = umma_desc_sw128(sbase + C::OFF_K + s * C::kTile, 16, 1024);
-                const uint64_t qd = umma_desc_sw128(sbase + C::OFF_Q + (wide && h ? C::kTile : 0u), 16, 1024);
-#pragma unroll
-                for (uint32_t i = 0; i < TERMS * (HD / 16); ++i) {
-                    const uint32_t t = i / (HD / 16), ks = i % (HD / 16);
-                    const uint32_t off = (ks >> 2) * kBlock + (ks & 3u) * 32u;
-                    umma_ss(tmem + TM_S + h * 128u, qd + ((t * C::kTile + off) >> 4), kd + (off >> 4), id_s, i != 0);
+            auto pass = [&](int full, int empty, uint32_t& seen, uint32_t g) {
+                for (; ok && seen < g; ++seen) {
+                    ok = mbar_wait(&bar[full + seen % C::kStages], (seen / C::kStages) & 1u);
+                    mbar_arrive(&bar[empty + seen % C::kStages]);
                 }
-                if (!wide || h) umma_commit(&bar[C::B_KEMPTY + s]);
-                if (last) umma_commit(&bar[C::B_QEMPTY]);
-                umma_commit(&bar[C::B_SFULL + h]);
-                return true;
             };
             for (; ok && pc.more(); pc.next(sh, kMost), ++it) {
-                const bool wide = TERMS == 1 && tgkv_group_tokens(&sh, pc.at.seq) - pc.at.at * sh.item_tokens > sh.tpt;
-                const uint32_t tiles = pc.j1 - pc.j0, steps = wide ? 2 * tiles : tiles;
+                const PieceRows pr(sh, pc, TERMS);
+                const uint32_t tiles = pc.j1 - pc.j0, steps = pr.wide ? 2 * tiles : tiles;
                 ok = mbar_wait(&bar[C::B_QFULL], it & 1u);
                 tc_fence_after();
-                ok = ok && issue_s(0, g0, wide, steps == 1);
-                if (steps > 1) ok = ok && issue_s(1, wide ? g0 : g0 + 1, wide, steps == 2);
-                for (uint32_t k = 0; ok && k < steps; ++k) {
-                    const uint32_t h = k & 1u, g = g0 + (wide ? k >> 1 : k), s = g % C::kStages;
-                    const uint32_t n = h ? done1 : done0;
-                    ok = mbar_wait(&bar[C::B_PFULL + h], n & 1u) &&
-                         mbar_wait(&bar[C::B_VFULL + s], (g / C::kStages) & 1u);
-                    if (!ok) break;
+                if (h >= steps) mbar_arrive(&bar[C::B_QEMPTY]);
+                const uint64_t qd = umma_desc_sw128(sbase + C::OFF_Q + (pr.wide && h ? C::kTile : 0u), 16, 1024);
+                uint32_t sk = h, shalf = 0;      // the next S: step, half
+                auto issue_s = [&]() {
+                    const uint32_t t = pr.wide ? sk >> 1 : sk, g = g0 + t, s = g % C::kStages, b = ns & 1u;
+                    if (shalf == 0) {
+                        pass(C::B_KFULL, C::B_KEMPTY, ks, g);
+                        ok = ok && mbar_wait(&bar[C::B_KFULL + s], (g / C::kStages) & 1u);
+                    }
+                    if (!ok) return;
                     tc_fence_after();
+                    const uint64_t kd =
+                        umma_desc_sw128(sbase + C::OFF_K + s * C::kTile + shalf * (kSub * 128u), 16, 1024);
+#pragma unroll
+                    for (uint32_t i = 0; i < TERMS * (HD / 16); ++i) {
+                        const uint32_t q = i / (HD / 16), d = i % (HD / 16);
+                        const uint32_t off = (d >> 2) * kBlock + (d & 3u) * 32u;
+                        umma_ss(tmem + TM_S + h * 128u + b * 64u, qd + ((q * C::kTile + off) >> 4), kd + (off >> 4), id_s,
+                                i != 0);
+                    }
+                    umma_commit(&bar[C::B_SFULL + 2 * h + b]);
+                    ++ns;
+                    if (++shalf < pr.halves(pc.j0 + t)) return;
+                    umma_commit(&bar[C::B_KEMPTY + s]);
+                    ks = g + 1;
+                    shalf = 0;
+                    sk += 2;
+                    if (sk >= steps) umma_commit(&bar[C::B_QEMPTY]);
+                    if (!pr.wide && sk - 1 < steps) pass(C::B_KFULL, C::B_KEMPTY, ks, g + 2);
+                };
+                if (ok && sk < steps) issue_s();
+                if (ok && sk < steps) issue_s();
+                for (uint32_t k = h; ok && k < steps; k += 2) {
+                    const uint32_t t = pr.wide ? k >> 1 : k, g = g0 + t, s = g % C::kStages;
+                    pass(C::B_VFULL, C::B_VEMPTY, vs, g);
                     // P of positions 16 kk .. +15: 8 columns.  V is MN-major: 64-dim blocks 16 KB
                     // apart, 8-position groups 1 KB apart.
                     const uint64_t vd = umma_desc_sw128(sbase + C::OFF_V + s * C::kTile, kBlock, 1024);
+                    const uint32_t halves = pr.halves(pc.j0 + t);
+                    for (uint32_t half = 0; ok && half < halves; ++half, ++np) {
+                        const uint32_t b = np & 1u;
+                        ok = mbar_wait(&bar[C::B_PFULL + 2 * h + b], (np >> 1) & 1u) &&
+                             (half || mbar_wait(&bar[C::B_VFULL + s], (g / C::kStages) & 1u));
+                        if (!ok) break;
+                        tc_fence_after();
 #pragma unroll
-                    for (uint32_t i = 0; i < TERMS * 8; ++i) {
-                        const uint32_t t = i >> 3, kk = i & 7u;
-                        umma_ts(tmem + TM_O + h * 128u, tmem + TM_S + h * 128u + t * 64u + kk * 8u,
-                                vd + ((kk * 16u * 128u) >> 4), id_pv, k > 1 || i != 0);
+                        for (uint32_t i = 0; i < TERMS * 4; ++i) {
+                            const uint32_t q = i >> 2, kk = i & 3u;
+                            umma_ts(tmem + TM_O + h * 128u, tmem + TM_S + h * 128u + b * 64u + q * 32u + kk * 8u,
+                                    vd + (((4 * half + kk) * 16u * 128u) >> 4), id_pv, k > 1 || half || i != 0);
+                        }
+                        umma_commit(&bar[C::B_PVDONE + h]);
+                        if (half + 1 == halves) {
+                            umma_commit(&bar[C::B_VEMPTY + s]);
+                            vs = g + 1;
+                            if (k + 2 >= steps) umma_commit(&bar[C::B_ODONE + h]);
+                        }
+                        // the next S goes where this PV reads P
+                        ok = mbar_wait(&bar[C::B_PVDONE + h], np & 1u);
+                        if (ok && sk < steps) issue_s();
                     }
-                    if (!wide || h) umma_commit(&bar[C::B_VEMPTY + s]);
-                    umma_commit(&bar[C::B_PVDONE + h]);
-                    if (h) ++done1;
-                    else ++done0;
-                    if (k + 2 < steps) ok = issue_s(h, g0 + (wide ? (k + 2) >> 1 : k + 2), wide, k + 3 == steps);
                 }
                 g0 += tiles;
+                pass(C::B_KFULL, C::B_KEMPTY, ks, g0);
+                pass(C::B_VFULL, C::B_VEMPTY, vs, g0);
             }
             if (!ok) atomicExch(p.err, kErrTimeout);
         }
         __syncwarp();
     } else {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoftmax));
         const int quarter = warp & 3, h = warp >> 2, r = quarter * 32 + lane;
         const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16);
         const uint32_t ts = lanes + TM_S + (uint32_t)h * 128u, to = lanes + TM_O + (uint32_t)h * 128u;
@@ -442,20 +469,21 @@ __global__ void __launch_bounds__(kThreads, 1) group_kernel(const __grid_constan
         const float scale = p.qscale;
         const uint32_t rtok = (uint32_t)r / G, sub = (uint32_t)r % G;
         const uint32_t total_rows = tok0[p.n_seq] * p.n_heads;
-        uint32_t g0 = 0, it = 0, n = 0;          // K/V tiles of earlier pieces; pieces; this stream's steps
+        uint32_t g0 = 0, it = 0, n = 0, nd = 0;  // K/V tiles of earlier pieces; pieces; this stream's halves, O's
         bool ok = true;
         // Both warps of a pair meet at named barriers, so neither leaves early:
         // after a failed wait a warp only keeps the barriers' counts.
         for (; pc.more(); pc.next(sh, kMost), ++it) {
-            const uint32_t seq = pc.at.seq, npre = tgkv_group_prefix_tiles(&sh, seq);
+            const uint32_t seq = pc.at.seq;
+            const PieceRows pr(sh, pc, TERMS);
+            const bool wide = pr.wide;
             const uint32_t t0 = pc.at.at * sh.item_tokens, left = tgkv_group_tokens(&sh, seq) - t0;
-            const bool wide = TERMS == 1 && left > sh.tpt;
             const uint32_t tb = wide && h ? sh.tpt : 0;                       // this stream's first token of the item
             const uint32_t ntok = min(sh.tpt, left - tb);
             const bool valid = rtok < ntok;
             const bool busy = (uint32_t)(quarter * 32) < ntok * G;            // the warp has rows
-            const uint32_t own_rows = seq ? tgkv_group_own_rows(&sh, seq, pc.at.at) : 0;
             const uint32_t own_min = seq ? old_len[seq - 1] + t0 + tb + 1 : 0;   // rows the stream's first token sees
+            const uint32_t own_mine = own_min + min(rtok, ntok - 1);             // rows this thread's token sees
             const uint64_t row = (uint64_t)((seq ? tok0[seq - 1] : 0) + t0 + tb + rtok) * p.n_heads + pc.at.kvh * G + sub;
             const uint32_t tiles = pc.j1 - pc.j0, steps = wide ? 2 * tiles : tiles;
             if constexpr (TERMS == 2) {
@@ -468,76 +496,86 @@ __global__ void __launch_bounds__(kThreads, 1) group_kernel(const __grid_constan
 
             float m = -INFINITY;                 // running maximum of the raw scores
             float2 l2 = make_float2(0.f, 0.f);
-            for (uint32_t k = (uint32_t)h; k < steps; k += 2, ++n) {
-                const uint32_t t = wide ? k >> 1 : k, j = pc.j0 + t, g = g0 + t;
-                const bool own = j >= npre;
-                const uint32_t pos = (own ? j - npre : j) * kPos;
-                const uint32_t rows = own ? own_rows : p.prefix_len;             // rows some query of the item sees
-                const bool mask = pos + kPos > (own ? own_min : p.prefix_len);
-                if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&bar[C::B_SFULL + h], n & 1u));
-                if (ok) tc_fence_after();
-                if (ok && pos + kPos > rows && (!wide || h == 0)) {
-                    // V rows that no query of the item sees may hold anything; P is 0 there, but
-                    // 0 * Inf is NaN, so they are cleared before a PV reads them (in wide pieces
-                    // stream 0's comes first)
-                    const uint32_t s = g % C::kStages;
-                    ok = __all_sync(0xffffffffu, mbar_wait(&bar[C::B_VFULL + s], (g / C::kStages) & 1u));
-                    if (ok)
-                        for (uint32_t y = rows - pos + ((uint32_t)r >> 3); y < kPos; y += 16)
+            for (uint32_t k = (uint32_t)h; k < steps; k += 2) {
+                const uint32_t t = wide ? k >> 1 : k, j = pc.j0 + t;
+                const uint32_t rows = pr.rows(j) - pr.pos(j);                    // of the tile, that some query sees
+                const uint32_t all = (pr.own(j) ? own_min : p.prefix_len) - pr.pos(j);         // that every query sees
+                const int lim = (int)((pr.own(j) ? own_mine : p.prefix_len) - pr.pos(j));      // that this thread's sees
+                const bool mask = (int)all < kPos;
+                const uint32_t halves = rows > kSub ? 2 : 1;
+#pragma unroll 1
+                for (uint32_t half = 0; half < halves; ++half, ++n) {
+                    const uint32_t b = n & 1u, tsb = ts + b * 64u;
+                    const int lm = lim - (int)(half * kSub);
+                    if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&bar[C::B_SFULL + 2 * h + b], (n >> 1) & 1u));
+                    if (ok && half == 0 && rows < kPos) {
+                        // V rows that no query of the item sees may hold anything; P is 0 there, but
+                        // 0 * Inf is NaN, so they are cleared before this stream's PV reads them (in
+                        // wide pieces by both streams: either may be first).  Only after this S is there has
+                        // the stage's last tile been used, so that the parity means this tile.
+                        const uint32_t g = g0 + t, s = g % C::kStages;
+                        ok = __all_sync(0xffffffffu, mbar_wait(&bar[C::B_VFULL + s], (g / C::kStages) & 1u));
+                        if (ok)
+                            for (uint32_t y = rows + ((uint32_t)r >> 3); y < kPos; y += 16)
 #pragma unroll
-                            for (int c = 0; c < HD / 64; ++c)
-                                *reinterpret_cast<uint4*>(base + C::OFF_V + s * C::kTile + c * kBlock + y * 128 +
-                                                          (r & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
-                    __syncwarp();
-                    fence_proxy_async_smem();
-                }
-                if (ok && busy) {
-                    Scores v;
-                    load_scores(ts, v);
-                    const int lim = (int)((own ? own_min + min(rtok, ntok - 1) : p.prefix_len) - pos);
-                    float tm;
-                    if (mask)
-                        tm = fmaxf(fmaxf(max32<true>(v.c[0], lim), max32<true>(v.c[1], lim - 32)),
-                                   fmaxf(max32<true>(v.c[2], lim - 64), max32<true>(v.c[3], lim - 96)));
-                    else
-                        tm = fmaxf(fmaxf(max32<false>(v.c[0], 0), max32<false>(v.c[1], 0)),
-                                   fmaxf(max32<false>(v.c[2], 0), max32<false>(v.c[3], 0)));
-                    // the running maximum moves only when exceeded by more than 2^8
-                    const bool grow = (tm - m) * scale > 8.f;
-                    const float alpha = !grow ? 1.f : m == -INFINITY ? 0.f : ex2_approx((m - tm) * scale);
-                    if (grow) m = tm;
-                    l2.x *= alpha;
-                    l2.y *= alpha;
-                    if (k > 1 && __any_sync(0xffffffffu, grow)) {
-                        // (the stream's last PV was complete before this S was made)
+                                for (int c = 0; c < HD / 64; ++c)
+                                    *reinterpret_cast<uint4*>(base + C::OFF_V + s * C::kTile + c * kBlock + y * 128 +
+                                                              (r & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
+                        __syncwarp();
+                        fence_proxy_async_smem();
+                    }
+                    if (ok && busy) {
+                        tc_fence_after();
+                        uint32_t va[32], vb[32];
+                        tmem_ld32(tsb, va);
+                        tmem_ld32(tsb + 32, vb);
+                        tmem_wait_ld(va, vb);
+                        const float tm = mask ? fmaxf(max32<true>(va, lm), max32<true>(vb, lm - 32))
+                                              : fmaxf(max32<false>(va, 0), max32<false>(vb, 0));
+                        // the running maximum moves only when exceeded by more than 2^8
+                        const bool grow = (tm - m) * scale > 8.f;
+                        if (__any_sync(0xffffffffu, grow)) {
+                            const float alpha = !grow ? 1.f : m == -INFINITY ? 0.f : ex2_approx((m - tm) * scale);
+                            if (grow) m = tm;
+                            l2.x *= alpha;
+                            l2.y *= alpha;
+                            if (k > 1 || half) {
+                                // O holds the earlier halves: all of them, then scale it
+                                ok = __all_sync(0xffffffffu, mbar_wait(&bar[C::B_PVDONE + h], (n - 1) & 1u));
+                                if (ok) {
+                                    tc_fence_after();
+#pragma unroll 1
+                                    for (int c = 0; c < HD / 16; ++c) {
+                                        uint32_t o[16];
+                                        tmem_ld16(to + c * 16, o);
+                                        tmem_wait_ld16(o);
 #pragma unroll
-                        for (int c = 0; c < HD / 16; ++c) {
-                            uint32_t o[16];
-                            tmem_ld16(to + c * 16, o);
-                            tmem_wait_ld16(o);
-#pragma unroll
-                            for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
-                            tmem_st16(to + c * 16, o);
+                                        for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+                                        tmem_st16(to + c * 16, o);
+                                    }
+                                }
+                            }
                         }
+                        const float msc = m == -INFINITY ? 0.f : m * scale;
+                        if (mask) {
+                            exp32<TERMS, true>(va, scale, msc, lm, l2, tsb);
+                            exp32<TERMS, true>(vb, scale, msc, lm - 32, l2, tsb + 16);
+                        } else {
+                            exp32<TERMS, false>(va, scale, msc, 0, l2, tsb);
+                            exp32<TERMS, false>(vb, scale, msc, 0, l2, tsb + 16);
+                        }
+                        tmem_wait_st();
                     }
-                    const float msc = m == -INFINITY ? 0.f : m * scale;
-                    if (mask) {
-#pragma unroll
-                        for (int c = 0; c < 4; ++c) exp32<TERMS, true>(v.c[c], scale, msc, lim - 32 * c, l2, ts + 16 * c);
-                    } else {
-#pragma unroll
-                        for (int c = 0; c < 4; ++c) exp32<TERMS, false>(v.c[c], scale, msc, 0, l2, ts + 16 * c);
-                    }
-                    tmem_wait_st();
+                    tc_fence_before();
+                    mbar_arrive(&bar[C::B_PFULL + 2 * h + b]);
                 }
-                tc_fence_before();
-                mbar_arrive(&bar[C::B_PFULL + h]);
             }
             g0 += tiles;
 
             // ---- the piece's rows: out, or a partial
             const bool mine = (uint32_t)h < steps;                               // this stream had a tile
-            if (ok && mine) ok = __all_sync(0xffffffffu, mbar_wait(&bar[C::B_PVDONE + h], (n - 1) & 1u));
+            if (ok && mine) ok = __all_sync(0xffffffffu, mbar_wait(&bar[C::B_ODONE + h], nd & 1u));
+            if (mine) ++nd;
             if (ok) tc_fence_after();
             float l = l2.x + l2.y, msc = m * scale;                              // -inf if nothing was seen
             float w0 = 1.f, w1 = 0.f;                                            // weights of the streams' O
@@ -560,52 +598,112 @@ __global__ void __launch_bounds__(kThreads, 1) group_kernel(const __grid_constan
             uint64_t slot;
             if (pc.first > 0 || !p.share) slot = (uint64_t)p.cta_rows + 512u * blockIdx.x + (pc.first > 0 ? 0u : 256u) + irow;
             else slot = (seq ? total_rows : 0u) + row;
-            float keep = 0.f, mine_w = 1.f;                                      // weights of the slot and of this piece
+            float keep = 0.f;                                                    // weight of the slot's earlier sum
             float2* slot_ml = reinterpret_cast<float2*>(p.part_ml) + slot;
-            if (TERMS == 2 && again && valid) {
-                const float2 old = *slot_ml;
-                const float M = fmaxf(old.x, msc);
-                keep = old.x == -INFINITY ? 0.f : ex2_approx(old.x - M);
-                mine_w = msc == -INFINITY ? 0.f : ex2_approx(msc - M);
-                l = l * mine_w + old.y * keep;
-                msc = M;
-                w0 *= mine_w;
-                w1 *= mine_w;
+            if (TERMS == 2 && again) {
+                if (valid) {
+                    const float2 old = *slot_ml;
+                    const float M = fmaxf(old.x, msc), w = msc == -INFINITY ? 0.f : ex2_approx(msc - M);
+                    keep = old.x == -INFINITY ? 0.f : ex2_approx(old.x - M);
+                    l = l * w + old.y * keep;
+                    msc = M;
+                    w0 *= w;
+                    w1 *= w;
+                }
+                pair_sync(quarter);                                              // both warps have read the slot's (m, l)
             }
-            if (TERMS == 2 && again) pair_sync(quarter);                         // both warps have read the slot's (m, l)
-            const float inv = 1.f / l;
-            const int c0 = wide ? 0 : h * (HD / 32), c1 = wide ? HD / 16 : c0 + HD / 32;   // columns 16 c .. +15
-            const uint32_t oa = wide ? to : lanes + TM_O;
-#pragma unroll 2
-            for (int c = c0; c < c1; ++c) {
-                uint32_t x[16], y[16];
-                __syncwarp();                    // tcgen05.ld is warp-collective
-                if (ok && busy) {
+            const float inv = whole ? 1.f / l : 1.f;
+            w0 *= inv;
+            w1 *= inv;
+            keep *= inv;
+            if (ok && busy) {
+                // 64 bytes of each row at a time through the warp's 2 KB of shared memory, so that
+                // four lanes write a row's 64 bytes: 16-byte part q of row x lies at x * 64 + (q ^
+                // (x / 2 % 4)) * 16, free of bank conflicts both ways
+                unsigned char* stg = base + C::OFF_STG + warp * 2048;
+                const uint32_t part = (uint32_t)lane & 3u;
+                uint64_t dst[4];                                                 // rows lane / 4 + 8 i
+                float kp[4];
+                const uint64_t mine_row = valid ? (whole ? row : slot) : ~0ull;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    dst[i] = __shfl_sync(0xffffffffu, mine_row, (lane >> 2) + 8 * i);
+                    kp[i] = TERMS == 2 ? __shfl_sync(0xffffffffu, keep, (lane >> 2) + 8 * i) : 0.f;
+                }
+                const uint64_t cta_slot = (uint64_t)p.cta_rows + 512u * blockIdx.x + 256u;   // a whole item's earlier sums
+                auto flush = [&](const uint4 (&w)[4], unsigned char* out, uint32_t row_bytes, uint32_t off, bool add) {
+#pragma unroll
+                    for (int q = 0; q < 4; ++q)
+                        *reinterpret_cast<uint4*>(stg + lane * 64 + ((q ^ (lane >> 1)) & 3) * 16) = w[q];
+                    __syncwarp();
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const uint32_t x = (uint32_t)(lane >> 2) + 8u * i;
+                        uint4 y = *reinterpret_cast<const uint4*>(stg + x * 64 + ((part ^ (x >> 1)) & 3u) * 16);
+                        if (dst[i] == ~0ull) continue;
+                        if (TERMS == 2 && add) {
+                            const float4 o = *reinterpret_cast<const float4*>(
+                                reinterpret_cast<const unsigned char*>(p.part_o) +
+                                (whole ? cta_slot + x : dst[i]) * row_bytes + off + part * 16);
+                            y = make_uint4(__float_as_uint(fmaf(o.x, kp[i], __uint_as_float(y.x))),
+                                           __float_as_uint(fmaf(o.y, kp[i], __uint_as_float(y.y))),
+                                           __float_as_uint(fmaf(o.z, kp[i], __uint_as_float(y.z))),
+                                           __float_as_uint(fmaf(o.w, kp[i], __uint_as_float(y.w))));
+                        }
+                        *reinterpret_cast<uint4*>(out + dst[i] * row_bytes + off + part * 16) = y;
+                    }
+                    __syncwarp();
+                };
+                // 16 columns of the row's sums (columns 16 c ..), joined and scaled
+                const uint32_t oa = wide ? to : lanes + TM_O;
+                auto take = [&](int c, float (&o)[16]) {
+                    uint32_t x[16], y[16];
                     tmem_ld16(oa + c * 16, x);
                     if (!wide && steps > 1) {
                         tmem_ld16(oa + 128 + c * 16, y);
                         tmem_wait_ld16(y);
                     }
                     tmem_wait_ld16(x);
-                }
-                if (ok && valid) {
-                    float o[16];
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
                         o[i] = w0 == 0.f ? 0.f : __uint_as_float(x[i]) * w0;
                         if (w1 != 0.f) o[i] = fmaf(__uint_as_float(y[i]), w1, o[i]);
                     }
-                    float* part = p.part_o + slot * HD + c * 16;
-                    if (TERMS == 2 && again)
+                };
+                const int c0 = wide ? 0 : h * (HD / 32), c1 = wide ? HD / 16 : c0 + HD / 32;
+                if (TERMS == 1 && whole) {
+#pragma unroll 1
+                    for (int c = c0; c < c1; c += 2) {
+                        float o[16];
+                        uint4 w[4];
 #pragma unroll
-                        for (int i = 0; i < 16; ++i) o[i] = fmaf(part[i], keep, o[i]);
-                    if (whole) store_out<T, 16>(reinterpret_cast<T*>(p.out) + row * HD + c * 16, o, inv);
-                    else store_out<float, 16>(part, o, 1.f);
+                        for (int k = 0; k < 2; ++k) {
+                            take(c + k, o);
+#pragma unroll
+                            for (int q = 0; q < 2; ++q)
+                                w[2 * k + q] = make_uint4(cvt_bf16x2(o[8 * q], o[8 * q + 1]), cvt_bf16x2(o[8 * q + 2], o[8 * q + 3]),
+                                                          cvt_bf16x2(o[8 * q + 4], o[8 * q + 5]), cvt_bf16x2(o[8 * q + 6], o[8 * q + 7]));
+                        }
+                        flush(w, reinterpret_cast<unsigned char*>(p.out), HD * 2, c * 32, false);
+                    }
+                } else {
+#pragma unroll 1
+                    for (int c = c0; c < c1; ++c) {
+                        float o[16];
+                        uint4 w[4];
+                        take(c, o);
+#pragma unroll
+                        for (int q = 0; q < 4; ++q)
+                            w[q] = make_uint4(__float_as_uint(o[4 * q]), __float_as_uint(o[4 * q + 1]),
+                                              __float_as_uint(o[4 * q + 2]), __float_as_uint(o[4 * q + 3]));
+                        flush(w, reinterpret_cast<unsigned char*>(whole ? p.out : (void*)p.part_o), HD * 4, c * 64, again);
+                    }
                 }
+                if (valid && !whole && (wide || h == 0)) *slot_ml = make_float2(msc, l);
             }
-            if (ok && valid && !whole && (wide || h == 0)) *slot_ml = make_float2(msc, l);
             if (!wide) {
                 // the other stream has read this one's O and (m, l), and both the slot's rows are written
+                __syncwarp();
                 tc_fence_before();
                 pair_sync(quarter);
             }
