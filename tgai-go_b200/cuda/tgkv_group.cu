@@ -7,18 +7,19 @@
 // of K/V tiles that tgkv_group_plan.h cuts.  A piece is an item (one or two row
 // tiles of 128 query rows of one KV head) against a run of 128-position K/V
 // tiles, in one pass: S = Q K^T, running maximum and sum in the log2 domain,
-// O += P V, 64 positions (half a tile) at a time.  Two streams, each with its
-// own O and two S/P buffers in TMEM, its own four softmax warps (one thread per
-// row) and its own MMA warp, run side by side:
+// O += P V, 64 positions (half a tile) at a time.  Two streams, each with its own
+// O and two S/P buffers of 64 positions in TMEM, its own four softmax warps (one
+// thread per row) and its own MMA warp, run side by side:
 //   wide pieces    (two row tiles) stream h has the rows of row tile h, and both
-//                  read every K/V tile: half the tile traffic per row;
+//                  read every K/V tile: half the tile traffic per row.  The scores
+//                  of the half after next are made as soon as a buffer's P has
+//                  been used, while the softmax works on the other buffer;
 //   narrow pieces  (one row tile) both have the same rows and take alternate
-//                  tiles; their results join at the end of the piece.
-// With two buffers the scores of a stream's next half tile are made while the
-// softmax works on this one, so the softmax warps hardly wait: the kernel is
-// bound by their instructions and the exponentials (16 a cycle and SM) beside
-// the tensor core (128 x 128 x HD of each product takes 4 HD cycles; scores 1.5
-// times that, since 64-column products read Q from shared memory twice).
+//                  tiles; their results join at the end of the piece.  A tile's
+//                  scores are made at once: a 64-column product reads as much of Q
+//                  as one of 128 and takes as long (524 of 512 cycles), and here
+//                  the other stream fills the wait.
+// A tile with at most 64 rows is one half.
 // Warps (384 threads): 0-3 and 4-7 the streams' softmax, 8 TMA (K/V tiles in
 // 64-dim boxes, 128-byte swizzle, into two rings that run ahead over the whole
 // stretch; Q of bf16 calls), 9 and 10 the streams' MMAs (one lane each).
@@ -53,7 +54,7 @@ constexpr int kTmaWarp = 8, kMmaWarp = 9;
 constexpr uint32_t kBlock = 16384;              // 128 rows x 64 bf16: one swizzled box
 constexpr uint32_t TM_S = 0, TM_O = 256, TM_COLS = 512;
 constexpr int kErrTimeout = 7;
-constexpr int kSub = 64;                        // positions of one S: half a tile
+constexpr int kSub = 64;                        // half a tile
 
 template <int HD>
 struct Cfg {
@@ -62,11 +63,11 @@ struct Cfg {
     static constexpr uint32_t OFF_K = 0, OFF_V = kStages * kTile, OFF_Q = 2 * kStages * kTile;
     static constexpr uint32_t OFF_BAR = OFF_Q + 2 * kTile;             // Q: two row tiles, or hi and lo
     static constexpr int B_KFULL = 0, B_KEMPTY = kStages, B_VFULL = 2 * kStages, B_VEMPTY = 3 * kStages;
-    static constexpr int B_SFULL = 4 * kStages;      // [2 streams][2 buffers] S is in TMEM
-    static constexpr int B_PFULL = B_SFULL + 4;      // [2][2] its P is written, O rescaled (128 arrivals)
-    static constexpr int B_PVDONE = B_PFULL + 4;     // [2] one phase per half tile: its PV is complete
-    static constexpr int B_ODONE = B_PVDONE + 2;     // [2] one phase per piece with steps: O is complete
-    static constexpr int B_QFULL = B_ODONE + 2;      // a piece's Q is in shared memory
+    // [2 streams][2 halves], one phase per tile each:
+    static constexpr int B_SFULL = 4 * kStages;      // S is in TMEM
+    static constexpr int B_PFULL = B_SFULL + 4;      // its P is written, O rescaled (128 arrivals)
+    static constexpr int B_PVDONE = B_PFULL + 4;     // its PV is complete
+    static constexpr int B_QFULL = B_PVDONE + 4;      // a piece's Q is in shared memory
     static constexpr int B_QEMPTY = B_QFULL + 1;     // every S of a piece is complete
     static constexpr uint32_t OFF_ML = OFF_BAR + 32 * 8;               // [2 streams][128] (m, l)
     static constexpr uint32_t OFF_SLOT = OFF_ML + 2 * kRows * 8;
@@ -177,29 +178,51 @@ __global__ void __launch_bounds__(256) group_append_kernel(const __grid_constant
     asm volatile("fence.proxy.async.global;" ::: "memory");
 }
 
+// The larger of three; NaN if one is, so that a NaN score reaches the row's maximum
+// and with it all its weights.
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
 template <bool MASK>
 __device__ __forceinline__ float max32(const uint32_t (&v)[32], int lim) {
-    float a[8];
+    float a[4];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
+    for (int i = 0; i < 4; ++i) {
         a[i] = -INFINITY;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            const float x = __uint_as_float(v[4 * i + k]);
-            a[i] = fmaxf(a[i], (!MASK || 4 * i + k < lim) ? x : -INFINITY);
+        for (int k = 0; k < 8; k += 2) {
+            const float x = __uint_as_float(v[8 * i + k]), y = __uint_as_float(v[8 * i + k + 1]);
+            a[i] = max3(a[i], (!MASK || 8 * i + k < lim) ? x : -INFINITY, (!MASK || 8 * i + k + 1 < lim) ? y : -INFINITY);
         }
     }
-#pragma unroll
-    for (int w = 4; w >= 1; w >>= 1)
-#pragma unroll
-        for (int i = 0; i < w; ++i) a[i] = fmaxf(a[i], a[i + w]);
-    return a[0];
+    return max3(max3(a[0], a[1], a[2]), a[3], a[3]);
+}
+
+// 2^x of two values on the FMA units, x <= 2^20: x = n + f with n the nearest
+// integer (adding and taking off 1.5 * 2^23) and |f| <= 1/2, 2^f by the cubic of
+// least relative error there (a weighted least-squares fit iterated to the minimax:
+// 7.5e-5, a fiftieth of the bf16 rounding that follows), n added to the exponent.
+// Below 2^-125 it gives 2^-125.
+__device__ __forceinline__ float2 exp2_fma(float2 x) {
+    constexpr float M = 12582912.f;
+    x = make_float2(fmaxf(x.x, -125.f), fmaxf(x.y, -125.f));
+    const float2 t = __fadd2_rn(x, make_float2(M, M));
+    const float2 f = __fadd2_rn(x, __ffma2_rn(t, make_float2(-1.f, -1.f), make_float2(M, M)));
+    float2 r = __ffma2_rn(f, make_float2(0.05517166852f, 0.05517166852f), make_float2(0.2426111251f, 0.2426111251f));
+    r = __ffma2_rn(r, f, make_float2(0.6932609677f, 0.6932609677f));
+    r = __ffma2_rn(r, f, make_float2(0.9999280572f, 0.9999280572f));
+    return make_float2(__int_as_float(__float_as_int(r.x) + (__float_as_int(t.x) << 23)),
+                       __int_as_float(__float_as_int(r.y) + (__float_as_int(t.y) << 23)));
 }
 
 // P = 2^(s * scale - msc) of 32 positions as bf16 words (two positions each) into
 // the TMEM columns from `col` on: hi there and, with two terms, the rounding
 // residuals lo 32 columns behind; the fp32 values add up in l.  Positions at or
-// behind lim get 0.
+// behind lim get 0.  One term: kFmaPairs of 8 pairs take exp2_fma, since the
+// exponential unit (16 a cycle and SM) would bound the kernel.
+constexpr int kFmaPairs = 3;
 template <int TERMS, bool MASK>
 __device__ __forceinline__ void exp32(const uint32_t (&v)[32], float scale, float msc, int lim, float2& l,
                                       uint32_t col) {
@@ -208,14 +231,15 @@ __device__ __forceinline__ void exp32(const uint32_t (&v)[32], float scale, floa
 #pragma unroll
     for (int c = 0; c < 16; ++c) {
         const float2 d = __ffma2_rn(make_float2(__uint_as_float(v[2 * c]), __uint_as_float(v[2 * c + 1])), sc, nm);
-        float p0 = ex2_approx(d.x), p1 = ex2_approx(d.y);
+        float2 pp;
+        if (TERMS == 1 && (c & 7) >= 8 - kFmaPairs) pp = exp2_fma(d);
+        else pp = make_float2(ex2_approx(d.x), ex2_approx(d.y));
         if (MASK) {
-            p0 = 2 * c < lim ? p0 : 0.f;
-            p1 = 2 * c + 1 < lim ? p1 : 0.f;
+            pp.x = 2 * c < lim ? pp.x : 0.f;
+            pp.y = 2 * c + 1 < lim ? pp.y : 0.f;
         }
-        const float2 pp = make_float2(p0, p1);
         l = __fadd2_rn(l, pp);
-        ph[c] = cvt_bf16x2(p0, p1);
+        ph[c] = cvt_bf16x2(pp.x, pp.y);
         if (TERMS == 2) {
             const float2 r = __ffma2_rn(make_float2(lo_f(ph[c]), hi_f(ph[c])), make_float2(-1.f, -1.f), pp);
             pl[c] = cvt_bf16x2(r.x, r.y);
@@ -292,13 +316,10 @@ __global__ void __launch_bounds__(kThreads, 1) group_kernel(const __grid_constan
             mbar_init(&bar[C::B_VFULL + i], 1);
             mbar_init(&bar[C::B_VEMPTY + i], 2);
         }
-        for (int h = 0; h < 2; ++h) {
-            for (int b = 0; b < 2; ++b) {
-                mbar_init(&bar[C::B_SFULL + 2 * h + b], 1);
-                mbar_init(&bar[C::B_PFULL + 2 * h + b], 128);
-            }
-            mbar_init(&bar[C::B_PVDONE + h], 1);
-            mbar_init(&bar[C::B_ODONE + h], 1);
+        for (int i = 0; i < 4; ++i) {
+            mbar_init(&bar[C::B_SFULL + i], 1);
+            mbar_init(&bar[C::B_PFULL + i], 128);
+            mbar_init(&bar[C::B_PVDONE + i], 1);
         }
         mbar_init(&bar[C::B_QFULL], TERMS == 2 ? 256 : 1);
         mbar_init(&bar[C::B_QEMPTY], 2);
@@ -369,16 +390,13 @@ __global__ void __launch_bounds__(kThreads, 1) group_kernel(const __grid_constan
             if (!ok) atomicExch(p.err, kErrTimeout);
         } else if ((warp == kMmaWarp || warp == kMmaWarp + 1) && lane == 0) {
             // One warp per stream.  Step k of a piece belongs to stream k % 2; its K/V tile is
-            // g0 + k / 2 (wide) or g0 + k (narrow), in one or two halves.  S runs two halves ahead
-            // of PV: PV of a half as soon as its P is there, then the S of the half after next
-            // into the same buffer.  Both warps pass every phase of the rings and of Q, in order,
-            // so that a parity always means the phase it is waited for: a tile or a Q that a
-            // stream does not use, it releases when it sees it.
-            constexpr uint32_t id_s = umma_idesc_bf16(kRows, kSub, 0, 0);
-            constexpr uint32_t id_pv = umma_idesc_bf16(kRows, HD, 0, 1);
+            // g0 + k / 2 (wide) or g0 + k (narrow).  PV of a half as soon as its P is there, then
+            // the next step's S into the buffer: half by half (wide) or at once behind the second
+            // half (narrow).  Both warps pass every phase of the rings and of Q, in order, so that
+            // a parity always means the phase it is waited for: a tile or a Q that a stream does
+            // not use, it releases when it sees it.
             const uint32_t h = (uint32_t)(warp - kMmaWarp);
-            uint32_t g0 = 0, it = 0;             // K/V tiles of earlier pieces; pieces
-            uint32_t ns = 0, np = 0;             // this stream's S and PV issued
+            uint32_t g0 = 0, it = 0, n = 0;      // K/V tiles of earlier pieces; pieces; this stream's steps
             uint32_t ks = 0, vs = 0;             // tiles passed in each ring
             bool ok = true;
             auto pass = [&](int full, int empty, uint32_t& seen, uint32_t g) {
@@ -394,64 +412,66 @@ __global__ void __launch_bounds__(kThreads, 1) group_kernel(const __grid_constan
                 tc_fence_after();
                 if (h >= steps) mbar_arrive(&bar[C::B_QEMPTY]);
                 const uint64_t qd = umma_desc_sw128(sbase + C::OFF_Q + (pr.wide && h ? C::kTile : 0u), 16, 1024);
-                uint32_t sk = h, shalf = 0;      // the next S: step, half
-                auto issue_s = [&]() {
-                    const uint32_t t = pr.wide ? sk >> 1 : sk, g = g0 + t, s = g % C::kStages, b = ns & 1u;
-                    if (shalf == 0) {
+                // S of step k's half (both halves with half 2); half 0 or 2 comes first for a tile
+                auto issue_s = [&](uint32_t k, uint32_t half) {
+                    const uint32_t t = pr.wide ? k >> 1 : k, g = g0 + t, s = g % C::kStages;
+                    if (half != 1) {
                         pass(C::B_KFULL, C::B_KEMPTY, ks, g);
                         ok = ok && mbar_wait(&bar[C::B_KFULL + s], (g / C::kStages) & 1u);
                     }
                     if (!ok) return;
                     tc_fence_after();
-                    const uint64_t kd =
-                        umma_desc_sw128(sbase + C::OFF_K + s * C::kTile + shalf * (kSub * 128u), 16, 1024);
+                    const uint32_t halves = pr.halves(pc.j0 + t), b = half & 1u;
+                    if (b < halves) {
+                        const uint32_t id = umma_idesc_bf16(kRows, half == 2 && halves == 2 ? kPos : kSub, 0, 0);
+                        const uint64_t kd = umma_desc_sw128(sbase + C::OFF_K + s * C::kTile + b * (kSub * 128u), 16, 1024);
 #pragma unroll
-                    for (uint32_t i = 0; i < TERMS * (HD / 16); ++i) {
-                        const uint32_t q = i / (HD / 16), d = i % (HD / 16);
-                        const uint32_t off = (d >> 2) * kBlock + (d & 3u) * 32u;
-                        umma_ss(tmem + TM_S + h * 128u + b * 64u, qd + ((q * C::kTile + off) >> 4), kd + (off >> 4), id_s,
-                                i != 0);
+                        for (uint32_t i = 0; i < TERMS * (HD / 16); ++i) {
+                            const uint32_t q = i / (HD / 16), d = i % (HD / 16);
+                            const uint32_t off = (d >> 2) * kBlock + (d & 3u) * 32u;
+                            umma_ss(tmem + TM_S + h * 128u + b * 64u, qd + ((q * C::kTile + off) >> 4), kd + (off >> 4), id,
+                                    i != 0);
+                        }
                     }
                     umma_commit(&bar[C::B_SFULL + 2 * h + b]);
-                    ++ns;
-                    if (++shalf < pr.halves(pc.j0 + t)) return;
+                    if (half == 0) return;
+                    if (half == 2) umma_commit(&bar[C::B_SFULL + 2 * h + 1]);
                     umma_commit(&bar[C::B_KEMPTY + s]);
                     ks = g + 1;
-                    shalf = 0;
-                    sk += 2;
-                    if (sk >= steps) umma_commit(&bar[C::B_QEMPTY]);
-                    if (!pr.wide && sk - 1 < steps) pass(C::B_KFULL, C::B_KEMPTY, ks, g + 2);
+                    if (k + 2 >= steps) umma_commit(&bar[C::B_QEMPTY]);
+                    if (!pr.wide && k + 1 < steps) pass(C::B_KFULL, C::B_KEMPTY, ks, g + 2);
                 };
-                if (ok && sk < steps) issue_s();
-                if (ok && sk < steps) issue_s();
-                for (uint32_t k = h; ok && k < steps; k += 2) {
+                if (ok && h < steps) issue_s(h, pr.wide ? 0 : 2);
+                if (ok && pr.wide) issue_s(h, 1);
+                for (uint32_t k = h; ok && k < steps; k += 2, ++n) {
                     const uint32_t t = pr.wide ? k >> 1 : k, g = g0 + t, s = g % C::kStages;
+                    const uint32_t halves = pr.halves(pc.j0 + t);
+                    const bool more = k + 2 < steps;
+                    constexpr uint32_t id_pv = umma_idesc_bf16(kRows, HD, 0, 1);
                     pass(C::B_VFULL, C::B_VEMPTY, vs, g);
                     // P of positions 16 kk .. +15: 8 columns.  V is MN-major: 64-dim blocks 16 KB
                     // apart, 8-position groups 1 KB apart.
                     const uint64_t vd = umma_desc_sw128(sbase + C::OFF_V + s * C::kTile, kBlock, 1024);
-                    const uint32_t halves = pr.halves(pc.j0 + t);
-                    for (uint32_t half = 0; ok && half < halves; ++half, ++np) {
-                        const uint32_t b = np & 1u;
-                        ok = mbar_wait(&bar[C::B_PFULL + 2 * h + b], (np >> 1) & 1u) &&
-                             (half || mbar_wait(&bar[C::B_VFULL + s], (g / C::kStages) & 1u));
+                    for (uint32_t b = 0; ok && b < 2; ++b) {
+                        ok = mbar_wait(&bar[C::B_PFULL + 2 * h + b], n & 1u) &&
+                             (b || mbar_wait(&bar[C::B_VFULL + s], (g / C::kStages) & 1u));
                         if (!ok) break;
                         tc_fence_after();
+                        if (b < halves)
 #pragma unroll
-                        for (uint32_t i = 0; i < TERMS * 4; ++i) {
-                            const uint32_t q = i >> 2, kk = i & 3u;
-                            umma_ts(tmem + TM_O + h * 128u, tmem + TM_S + h * 128u + b * 64u + q * 32u + kk * 8u,
-                                    vd + (((4 * half + kk) * 16u * 128u) >> 4), id_pv, k > 1 || half || i != 0);
-                        }
-                        umma_commit(&bar[C::B_PVDONE + h]);
-                        if (half + 1 == halves) {
+                            for (uint32_t i = 0; i < TERMS * 4; ++i) {
+                                const uint32_t q = i >> 2, kk = i & 3u;
+                                umma_ts(tmem + TM_O + h * 128u, tmem + TM_S + h * 128u + b * 64u + q * 32u + kk * 8u,
+                                        vd + (((4 * b + kk) * 16u * 128u) >> 4), id_pv, k > 1 || b || i != 0);
+                            }
+                        umma_commit(&bar[C::B_PVDONE + 2 * h + b]);
+                        if (b) {
                             umma_commit(&bar[C::B_VEMPTY + s]);
                             vs = g + 1;
-                            if (k + 2 >= steps) umma_commit(&bar[C::B_ODONE + h]);
                         }
                         // the next S goes where this PV reads P
-                        ok = mbar_wait(&bar[C::B_PVDONE + h], np & 1u);
-                        if (ok && sk < steps) issue_s();
+                        if (pr.wide || b) ok = mbar_wait(&bar[C::B_PVDONE + 2 * h + b], n & 1u);
+                        if (ok && more && (pr.wide || b)) issue_s(k + 2, pr.wide ? b : 2);
                     }
                 }
                 g0 += tiles;
@@ -469,7 +489,7 @@ __global__ void __launch_bounds__(kThreads, 1) group_kernel(const __grid_constan
         const float scale = p.qscale;
         const uint32_t rtok = (uint32_t)r / G, sub = (uint32_t)r % G;
         const uint32_t total_rows = tok0[p.n_seq] * p.n_heads;
-        uint32_t g0 = 0, it = 0, n = 0, nd = 0;  // K/V tiles of earlier pieces; pieces; this stream's halves, O's
+        uint32_t g0 = 0, it = 0, n = 0;          // K/V tiles of earlier pieces; pieces; this stream's steps
         bool ok = true;
         // Both warps of a pair meet at named barriers, so neither leaves early:
         // after a failed wait a warp only keeps the barriers' counts.
@@ -504,15 +524,16 @@ __global__ void __launch_bounds__(kThreads, 1) group_kernel(const __grid_constan
                 const bool mask = (int)all < kPos;
                 const uint32_t halves = rows > kSub ? 2 : 1;
 #pragma unroll 1
-                for (uint32_t half = 0; half < halves; ++half, ++n) {
-                    const uint32_t b = n & 1u, tsb = ts + b * 64u;
-                    const int lm = lim - (int)(half * kSub);
-                    if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&bar[C::B_SFULL + 2 * h + b], (n >> 1) & 1u));
-                    if (ok && half == 0 && rows < kPos) {
+                for (uint32_t b = 0; b < 2; ++b) {
+                    const uint32_t tsb = ts + b * 64u;
+                    const int lm = lim - (int)(b * kSub);
+                    if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&bar[C::B_SFULL + 2 * h + b], n & 1u));
+                    if (ok && b == 0 && rows < kPos) {
                         // V rows that no query of the item sees may hold anything; P is 0 there, but
                         // 0 * Inf is NaN, so they are cleared before this stream's PV reads them (in
-                        // wide pieces by both streams: either may be first).  Only after this S is there has
-                        // the stage's last tile been used, so that the parity means this tile.
+                        // wide pieces by both streams: either may be first).  Only after this S is
+                        // there has the stage's last tile been used, so that the parity means this
+                        // tile.
                         const uint32_t g = g0 + t, s = g % C::kStages;
                         ok = __all_sync(0xffffffffu, mbar_wait(&bar[C::B_VFULL + s], (g / C::kStages) & 1u));
                         if (ok)
@@ -524,24 +545,25 @@ __global__ void __launch_bounds__(kThreads, 1) group_kernel(const __grid_constan
                         __syncwarp();
                         fence_proxy_async_smem();
                     }
-                    if (ok && busy) {
+                    if (ok && busy && b < halves) {
                         tc_fence_after();
                         uint32_t va[32], vb[32];
                         tmem_ld32(tsb, va);
                         tmem_ld32(tsb + 32, vb);
                         tmem_wait_ld(va, vb);
-                        const float tm = mask ? fmaxf(max32<true>(va, lm), max32<true>(vb, lm - 32))
-                                              : fmaxf(max32<false>(va, 0), max32<false>(vb, 0));
-                        // the running maximum moves only when exceeded by more than 2^8
-                        const bool grow = (tm - m) * scale > 8.f;
+                        const float tm = mask ? max3(-INFINITY, max32<true>(va, lm), max32<true>(vb, lm - 32))
+                                              : max3(-INFINITY, max32<false>(va, 0), max32<false>(vb, 0));
+                        // the running maximum moves only when exceeded by more than 2^8 (or NaN)
+                        const bool grow = !((tm - m) * scale <= 8.f);
                         if (__any_sync(0xffffffffu, grow)) {
                             const float alpha = !grow ? 1.f : m == -INFINITY ? 0.f : ex2_approx((m - tm) * scale);
                             if (grow) m = tm;
                             l2.x *= alpha;
                             l2.y *= alpha;
-                            if (k > 1 || half) {
+                            if (k > 1 || b) {
                                 // O holds the earlier halves: all of them, then scale it
-                                ok = __all_sync(0xffffffffu, mbar_wait(&bar[C::B_PVDONE + h], (n - 1) & 1u));
+                                ok = __all_sync(0xffffffffu,
+                                                mbar_wait(&bar[C::B_PVDONE + 2 * h + (b ^ 1u)], (b ? n : n - 1) & 1u));
                                 if (ok) {
                                     tc_fence_after();
 #pragma unroll 1
@@ -569,13 +591,13 @@ __global__ void __launch_bounds__(kThreads, 1) group_kernel(const __grid_constan
                     tc_fence_before();
                     mbar_arrive(&bar[C::B_PFULL + 2 * h + b]);
                 }
+                ++n;
             }
             g0 += tiles;
 
             // ---- the piece's rows: out, or a partial
             const bool mine = (uint32_t)h < steps;                               // this stream had a tile
-            if (ok && mine) ok = __all_sync(0xffffffffu, mbar_wait(&bar[C::B_ODONE + h], nd & 1u));
-            if (mine) ++nd;
+            if (ok && mine) ok = __all_sync(0xffffffffu, mbar_wait(&bar[C::B_PVDONE + 2 * h + 1], (n - 1) & 1u));
             if (ok) tc_fence_after();
             float l = l2.x + l2.y, msc = m * scale;                              // -inf if nothing was seen
             float w0 = 1.f, w1 = 0.f;                                            // weights of the streams' O
