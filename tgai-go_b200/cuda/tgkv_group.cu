@@ -200,29 +200,13 @@ __device__ __forceinline__ float max32(const uint32_t (&v)[32], int lim) {
     return max3(max3(a[0], a[1], a[2]), a[3], a[3]);
 }
 
-// 2^x of two values on the FMA units, x <= 2^20: x = n + f with n the nearest
-// integer (adding and taking off 1.5 * 2^23) and |f| <= 1/2, 2^f by the cubic of
-// least relative error there (a weighted least-squares fit iterated to the minimax:
-// 7.5e-5, a fiftieth of the bf16 rounding that follows), n added to the exponent.
-// Below 2^-125 it gives 2^-125.
-__device__ __forceinline__ float2 exp2_fma(float2 x) {
-    constexpr float M = 12582912.f;
-    x = make_float2(fmaxf(x.x, -125.f), fmaxf(x.y, -125.f));
-    const float2 t = __fadd2_rn(x, make_float2(M, M));
-    const float2 f = __fadd2_rn(x, __ffma2_rn(t, make_float2(-1.f, -1.f), make_float2(M, M)));
-    float2 r = __ffma2_rn(f, make_float2(0.05517166852f, 0.05517166852f), make_float2(0.2426111251f, 0.2426111251f));
-    r = __ffma2_rn(r, f, make_float2(0.6932609677f, 0.6932609677f));
-    r = __ffma2_rn(r, f, make_float2(0.9999280572f, 0.9999280572f));
-    return make_float2(__int_as_float(__float_as_int(r.x) + (__float_as_int(t.x) << 23)),
-                       __int_as_float(__float_as_int(r.y) + (__float_as_int(t.y) << 23)));
-}
-
 // P = 2^(s * scale - msc) of 32 positions as bf16 words (two positions each) into
 // the TMEM columns from `col` on: hi there and, with two terms, the rounding
 // residuals lo 32 columns behind; the fp32 values add up in l.  Positions at or
-// behind lim get 0.  One term: kFmaPairs of 8 pairs take exp2_fma, since the
-// exponential unit (16 a cycle and SM) would bound the kernel.
-constexpr int kFmaPairs = 3;
+// behind lim get 0.  (A part of the exponentials as a polynomial on the FMA units
+// measured no faster: 490 us with none to a quarter of them, 513 us with three
+// eighths, 4 prompts of 2000 tokens behind 2048; the streams' chain of products
+// bounds the kernel, not the exponential unit.)
 template <int TERMS, bool MASK>
 __device__ __forceinline__ void exp32(const uint32_t (&v)[32], float scale, float msc, int lim, float2& l,
                                       uint32_t col) {
@@ -231,9 +215,7 @@ __device__ __forceinline__ void exp32(const uint32_t (&v)[32], float scale, floa
 #pragma unroll
     for (int c = 0; c < 16; ++c) {
         const float2 d = __ffma2_rn(make_float2(__uint_as_float(v[2 * c]), __uint_as_float(v[2 * c + 1])), sc, nm);
-        float2 pp;
-        if (TERMS == 1 && (c & 7) >= 8 - kFmaPairs) pp = exp2_fma(d);
-        else pp = make_float2(ex2_approx(d.x), ex2_approx(d.y));
+        float2 pp = make_float2(ex2_approx(d.x), ex2_approx(d.y));
         if (MASK) {
             pp.x = 2 * c < lim ? pp.x : 0.f;
             pp.y = 2 * c + 1 < lim ? pp.y : 0.f;
