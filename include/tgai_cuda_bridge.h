@@ -233,10 +233,12 @@ typedef struct {
 uint64_t tg_cuda_kv_group_scratch_bytes(uint32_t n_seq, uint32_t n_heads, uint32_t head_dim);
 /* How a call's work is dealt to CTAs on a device of `sms` SMs (no launch, no
  * device needed): share 1 if the prefix is attended for all sequences' tokens
- * together, the CTAs, and where on the line of tiles each starts: n_cta + 1
- * records (sequence: 0 the shared prefix, i + 1 sequence i; KV head; item, of
- * 256 / G tokens with bf16 activations and 128 / G with fp32 ones, G = n_heads /
- * n_kv_heads; K/V tile of 128 positions), at most 161. */
+ * together; n_cta[2], the CTAs of the two kernels (0: full row tiles, 1: at most
+ * 16 query rows); and where on its line of tiles each CTA starts: starts +
+ * 644 * kernel holds n_cta + 1 records (sequence: 0 the shared prefix, i + 1
+ * sequence i; KV head; item, of 256 / G tokens with bf16 activations and 128 / G
+ * with fp32 ones on line 0, 16 / G and 10 / G on line 1, G = n_heads / n_kv_heads;
+ * K/V tile of 128 positions). */
 int tg_cuda_kv_group_plan(const TGCudaGroupCall* c, uint32_t sms, uint32_t* share, uint32_t* n_cta,
                           uint32_t* starts);
 int tg_cuda_kv_group_attention(const TGCudaGroupCall* c, void* stream);

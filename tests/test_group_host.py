@@ -107,53 +107,60 @@ def test_group_table_refuses(lib):
 
 
 def plan(lib, old, new, prefix, nh, nkv, act, sms):
-    """(share, CTA starts) of a call; the last start is the end of the line."""
+    """(share, CTA starts of the two kernels) of a call; the last start is what follows the line."""
     n = len(old)
     c = Call(act=act, n_seq=n, n_heads=nh, n_kv_heads=nkv, head_dim=64, prefix_len=prefix, old_len=(u32 * n)(*old),
              n_new=(u32 * n)(*new))
-    share, n_cta, starts = u32(), u32(), (u32 * (161 * 4))()
-    assert lib.tg_cuda_kv_group_plan(C.byref(c), sms, C.byref(share), C.byref(n_cta), starts), \
-        lib.tg_cuda_kv_last_error()
-    return share.value, [tuple(starts[4 * b:4 * b + 4]) for b in range(n_cta.value + 1)]
+    share, n_cta, starts = u32(), (u32 * 2)(), (u32 * (2 * 161 * 4))()
+    assert lib.tg_cuda_kv_group_plan(C.byref(c), sms, C.byref(share), n_cta, starts), lib.tg_cuda_kv_last_error()
+    return share.value, [[tuple(starts[644 * ln + 4 * b:644 * ln + 4 * b + 4]) for b in range(n_cta[ln] + 1)]
+                         if n_cta[ln] else [] for ln in range(2)]
 
 
-def line(old, new, prefix, nh, nkv, share, act):
-    """Every (item, tile) of the line in order, from the description of the cut alone."""
-    tpt = 128 // (nh // nkv) * (1 + act)
+def lines(old, new, prefix, nh, nkv, share, act):
+    """Every (item, tile) of the two lines in order, from the description of the cut alone."""
+    g = nh // nkv
+    heavy, light = 128 // g * (1 + act), (16 if act else 10) // g
+    own_light = max(new) <= light
+    pre_light = own_light and (not share or sum(new) <= light)
+    got = [[], []]
 
-    def row_tiles(seq, tokens, tiles_of):
-        return [(seq, h, r, j) for h in range(nkv) for r in range(-(-tokens // tpt)) for j in range(tiles_of(r))]
+    def add(line, seq, tokens, tiles_of):
+        per = light if line else heavy
+        got[line] += [(seq, h, r, j) for h in range(nkv) for r in range(-(-tokens // per)) for j in range(tiles_of(r, per))]
     pre = -(-prefix // 128)
-    got = row_tiles(0, sum(new), lambda r: pre) if share else []
+    if share:
+        add(int(pre_light), 0, sum(new), lambda r, per: pre)
     for i, (o, t) in enumerate(zip(old, new)):
-        got += row_tiles(i + 1, t, lambda r: (0 if share else pre) + -(-(o + min((r + 1) * tpt, t)) // 128))
+        add(int(own_light), i + 1, t, lambda r, per: (0 if share else pre) + -(-(o + min((r + 1) * per, t)) // 128))
     return got
 
 
 @pytest.mark.parametrize("old,new,prefix,nh,nkv,share", [
     ([0], [1], 0, 1, 1, 0), ([0], [1], 1, 1, 1, 0), ([5] * 64, [1] * 64, 32768, 32, 8, 1),
     ([100] * 1024, [1] * 1024, 300, 8, 8, 1), ([0, 3, 900], [0, 7, 0], 500, 12, 4, 0),
-    ([0] * 5, [0] * 5, 100, 4, 4, 0), ([0, 0], [5000, 1], 0, 16, 4, 0), ([10] * 12, [2, 9, 0, 4, 0, 8, 1, 1, 3, 5, 6, 7],
-                                                                       700, 16, 2, 1),
-    ([77] * 9, [40] * 9, 4000, 16, 4, 1), ([77] * 9, [60] * 9, 4000, 16, 4, 0), ([1], [3], 129, 128, 1, 0), ([200000], [1], 0, 7, 1, 0),
-    ([0] * 30, [600] * 30, 100, 32, 8, 0),
+    ([0] * 5, [0] * 5, 100, 4, 4, 0), ([0, 0], [5000, 1], 0, 16, 4, 0),
+    ([10] * 12, [2, 9, 0, 4, 0, 8, 1, 1, 3, 5, 6, 7], 700, 16, 2, 1), ([0, 9], [1, 1], 3000, 8, 8, 1),
+    ([77] * 9, [40] * 9, 4000, 16, 4, 1), ([77] * 9, [60] * 9, 4000, 16, 4, 0), ([1], [3], 129, 128, 1, 0),
+    ([200000], [1], 0, 7, 1, 0), ([0] * 30, [600] * 30, 100, 32, 8, 0), ([3, 0, 5], [2, 0, 1], 0, 8, 4, 0),
 ])
 @pytest.mark.parametrize("act", [0, 1])
 @pytest.mark.parametrize("sms", [148, 1, 7, 0])
-def test_plan_covers_the_line(lib, old, new, prefix, nh, nkv, share, sms, act):
-    """The CTAs' stretches are the line of tiles, cut in order into parts of about one size."""
+def test_plan_covers_the_lines(lib, old, new, prefix, nh, nkv, share, sms, act):
+    """The CTAs' stretches are the lines of tiles, cut in order into parts of about one size."""
     got_share, starts = plan(lib, old, new, prefix, nh, nkv, act, sms)
     assert got_share == share
-    tiles = line(old, new, prefix, nh, nkv, share, act)
-    if not tiles:
-        assert len(starts) == 1
-        return
-    index = {t: k for k, t in enumerate(tiles)}
-    cuts = [index[s] for s in starts[:-1]] + [len(tiles)]
-    assert starts[-1] == (len(old) + 1, 0, 0, 0)
-    assert cuts[0] == 0 and all(a <= b for a, b in zip(cuts, cuts[1:]))
-    n_cta = len(starts) - 1
-    assert n_cta == min(len(tiles), sms or 160)
-    items = len({t[:3] for t in tiles})
-    most = max(b - a + len({t[:3] for t in tiles[a:b]}) for a, b in zip(cuts, cuts[1:]))
-    assert most <= (len(tiles) + items) / n_cta + 3
+    for tiles, st in zip(lines(old, new, prefix, nh, nkv, share, act), starts):
+        if not tiles:
+            assert not st
+            continue
+        index = {t: k for k, t in enumerate(tiles)}
+        cuts = [index[s] for s in st[:-1]] + [len(tiles)]
+        after = min([i + 1 for i, t in enumerate(new) if t and i + 1 > tiles[-1][0]], default=len(new) + 1)
+        assert st[-1] == (after, 0, 0, 0)
+        assert cuts[0] == 0 and all(a <= b for a, b in zip(cuts, cuts[1:]))
+        n_cta = len(st) - 1
+        assert n_cta == min(len(tiles), sms or 160)
+        items = len({t[:3] for t in tiles})
+        most = max(b - a + len({t[:3] for t in tiles[a:b]}) for a, b in zip(cuts, cuts[1:]))
+        assert most <= (len(tiles) + items) / n_cta + 3

@@ -1064,17 +1064,56 @@ static uint64_t group_share_rows(uint32_t n_seq, uint32_t n_heads) {
     return 2 * (rows > 16384 ? rows : 16384);
 }
 static uint64_t group_rows(uint32_t n_seq, uint32_t n_heads) {
-    return group_share_rows(n_seq, n_heads) + 512ull * TGKV_GROUP_MAX_CTAS;
+    return group_share_rows(n_seq, n_heads) +
+           (2ull * 256 + 2 * TGKV_GROUP_LIGHT_ROWS) * TGKV_GROUP_MAX_CTAS;
 }
 uint64_t tg_cuda_kv_group_scratch_bytes(uint32_t n_seq, uint32_t n_heads, uint32_t head_dim) {
     return group_rows(n_seq, n_heads) * (head_dim + 2) * 4;
 }
 
-static TGKvGroupShape group_shape(const TGKvGroupParams* p) {
-    TGKvGroupShape s = {p->n_seq, p->n_kv_heads, p->prefix_len, p->share, 0, 0, p->old_len, p->tok0};
-    s.tpt = TGKV_GROUP_ROWS / (p->n_heads / p->n_kv_heads);
-    s.item_tokens = s.tpt * p->pair;
-    return s;
+/* The stretches of a line: the items of sequences [first, last] (0: the shared
+ * prefix) on up to `sms` CTAs. */
+static void plan_line(const TGKvGroupShape* sh, uint32_t first, uint32_t last, uint32_t sms, TGKvGroupLine* ln) {
+    ln->n_cta = ln->n_split = 0;
+    ln->item_tokens = sh->item_tokens;
+    uint64_t cost = 0, units = 0;
+    for (uint32_t s = tgkv_group_skip(sh, first); s <= last; s = tgkv_group_skip(sh, s + 1)) {
+        const uint32_t n = tgkv_group_items(sh, s);
+        uint64_t tiles = 0;
+        for (uint32_t at = 0; at < n; at++) tiles += tgkv_group_item_tiles(sh, s, at);
+        units += tiles * sh->n_kv_heads;
+        cost += (tiles + (uint64_t)n * TGKV_GROUP_ITEM_COST) * sh->n_kv_heads;
+    }
+    if (units == 0) return;
+    uint32_t n_cta = sms && sms < TGKV_GROUP_MAX_CTAS ? sms : TGKV_GROUP_MAX_CTAS;
+    if (units < n_cta) n_cta = (uint32_t)units;
+    ln->n_cta = n_cta;
+    TGKvGroupPos* start = (TGKvGroupPos*)ln->start;
+    uint32_t b = 0, s = tgkv_group_skip(sh, first);
+    uint64_t done = 0;                              /* cost before the current item */
+    for (; s <= last; s = tgkv_group_skip(sh, s + 1)) {
+        const uint32_t n = tgkv_group_items(sh, s);
+        uint64_t head = 0;                          /* cost of one KV head's items of s */
+        for (uint32_t at = 0; at < n; at++)
+            head += tgkv_group_item_tiles(sh, s, at) + TGKV_GROUP_ITEM_COST;
+        for (uint32_t kvh = 0; kvh < sh->n_kv_heads; kvh++) {
+            if (b >= n_cta || (uint64_t)b * cost / n_cta >= done + head) { done += head; continue; }
+            for (uint32_t at = 0; at < n; at++) {
+                const uint64_t end = done + tgkv_group_item_tiles(sh, s, at) + TGKV_GROUP_ITEM_COST;
+                for (; b < n_cta && (uint64_t)b * cost / n_cta < end; b++) {
+                    const uint64_t off = (uint64_t)b * cost / n_cta - done;
+                    start[b].seq = s;
+                    start[b].kvh = kvh;
+                    start[b].at = at;
+                    start[b].tile = off > TGKV_GROUP_ITEM_COST ? (uint32_t)(off - TGKV_GROUP_ITEM_COST) : 0;
+                    if (start[b].tile) ln->n_split++;
+                }
+                done = end;
+            }
+        }
+    }
+    start[n_cta].seq = s;                           /* what follows the line, or n_seq + 1 */
+    start[n_cta].kvh = start[n_cta].at = start[n_cta].tile = 0;
 }
 
 /* Checks a call and fills p's lengths, geometry and plan. */
@@ -1088,10 +1127,13 @@ static int plan_group(const TGCudaGroupCall* c, uint32_t sms, TGKvGroupParams* p
         return 0;
     }
     uint64_t total = 0;
+    uint32_t longest = 0, seqs = 0;
     for (uint32_t i = 0; i < c->n_seq; i++) {
         p->tok0[i] = (uint32_t)total;
         p->old_len[i] = c->old_len[i];
         total += c->n_new[i];
+        seqs += c->n_new[i] > 0;
+        if (c->n_new[i] > longest) longest = c->n_new[i];
         if (total * c->n_heads > 0x7fffffffull) {
             set_err("group: too many query rows (tokens x heads above 2^31 - 1)");
             return 0;
@@ -1101,64 +1143,46 @@ static int plan_group(const TGCudaGroupCall* c, uint32_t sms, TGKvGroupParams* p
             return 0;
         }
     }
+    const uint32_t g = c->n_heads / c->n_kv_heads, tpt = TGKV_GROUP_ROWS / g;
     p->tok0[c->n_seq] = (uint32_t)total;
     p->n_seq = c->n_seq;
     p->n_heads = c->n_heads;
     p->n_kv_heads = c->n_kv_heads;
     p->head_dim = c->head_dim;
     p->prefix_len = c->prefix_len;
-    p->n_cta = p->n_split = p->share = 0;
-    p->pair = c->act == 1 ? 2 : 1;
-    p->cta_rows = 0;
+    p->share = p->prefix_line = p->own_line = 0;
+    p->line[0].n_cta = p->line[1].n_cta = p->line[0].n_split = p->line[1].n_split = 0;
     if (total == 0) return 1;
-    TGKvGroupShape sh = group_shape(p);
-    /* Split when items over all sequences' tokens need at most 3/4 of the
-     * prefix passes that the sequences' own items make. */
-    uint64_t own_items = 0;
-    for (uint32_t i = 1; i <= c->n_seq; i++) own_items += tgkv_group_items(&sh, i);
-    if (c->prefix_len && 4 * ((total + sh.item_tokens - 1) / sh.item_tokens) <= 3 * own_items &&
-        2 * total * c->n_heads <= group_share_rows(c->n_seq, c->n_heads)) {
-        p->share = sh.share = 1;
-        p->cta_rows = (uint32_t)(2 * total * c->n_heads);
+    /* Light items when every sequence's rows fit one: the products' columns then
+     * are the rows there are, not 128.  (Three terms of 10 rows with fp32
+     * activations.) */
+    const uint32_t light_tokens = (c->act == 1 ? TGKV_GROUP_LIGHT_ROWS : 10u) / g;
+    const int own_light = longest <= light_tokens;
+    TGKvGroupShape heavy = {p->n_seq, p->n_kv_heads, p->prefix_len, 0, tpt, c->act == 1 ? 2 * tpt : tpt,
+                            p->old_len, p->tok0};
+    /* Split when items over all sequences' tokens need at most 3/4 of the prefix
+     * passes that the sequences' own items make. */
+    uint64_t own_items = seqs;
+    if (!own_light) {
+        own_items = 0;
+        for (uint32_t i = 1; i <= c->n_seq; i++) own_items += tgkv_group_items(&heavy, i);
     }
-    /* the line's cost: tiles, and TGKV_GROUP_ITEM_COST per item */
-    uint64_t cost = 0, units = 0;
-    for (uint32_t s = tgkv_group_skip(&sh, 0); s <= c->n_seq; s = tgkv_group_skip(&sh, s + 1)) {
-        const uint32_t n = tgkv_group_items(&sh, s);
-        uint64_t tiles = 0;
-        for (uint32_t at = 0; at < n; at++) tiles += tgkv_group_item_tiles(&sh, s, at);
-        units += tiles * c->n_kv_heads;
-        cost += (tiles + (uint64_t)n * TGKV_GROUP_ITEM_COST) * c->n_kv_heads;
+    if (c->prefix_len && 4 * ((total + heavy.item_tokens - 1) / heavy.item_tokens) <= 3 * own_items &&
+        2 * total * c->n_heads <= group_share_rows(c->n_seq, c->n_heads))
+        p->share = heavy.share = 1;
+    TGKvGroupShape light = heavy;
+    light.item_tokens = light_tokens;
+    const int all_light = own_light && (!p->share || total <= light_tokens);
+    p->own_line = own_light;
+    p->prefix_line = all_light;
+    if (!own_light) plan_line(&heavy, 0, c->n_seq, sms, &p->line[0]);
+    else if (all_light) plan_line(&light, 0, c->n_seq, sms, &p->line[1]);
+    else {
+        plan_line(&heavy, 0, 0, sms, &p->line[0]);
+        plan_line(&light, 1, c->n_seq, sms, &p->line[1]);
     }
-    uint32_t n_cta = sms && sms < TGKV_GROUP_MAX_CTAS ? sms : TGKV_GROUP_MAX_CTAS;
-    if (units < n_cta) n_cta = (uint32_t)units;
-    p->n_cta = n_cta;
-    TGKvGroupPos* start = (TGKvGroupPos*)p->start;
-    uint32_t b = 0;
-    uint64_t done = 0;                              /* cost before the current item */
-    for (uint32_t s = tgkv_group_skip(&sh, 0); s <= c->n_seq; s = tgkv_group_skip(&sh, s + 1)) {
-        const uint32_t n = tgkv_group_items(&sh, s);
-        uint64_t head = 0;                          /* cost of one KV head's items of s */
-        for (uint32_t at = 0; at < n; at++)
-            head += tgkv_group_item_tiles(&sh, s, at) + TGKV_GROUP_ITEM_COST;
-        for (uint32_t kvh = 0; kvh < c->n_kv_heads; kvh++) {
-            if (b >= n_cta || (uint64_t)b * cost / n_cta >= done + head) { done += head; continue; }
-            for (uint32_t at = 0; at < n; at++) {
-                const uint64_t end = done + tgkv_group_item_tiles(&sh, s, at) + TGKV_GROUP_ITEM_COST;
-                for (; b < n_cta && (uint64_t)b * cost / n_cta < end; b++) {
-                    const uint64_t off = (uint64_t)b * cost / n_cta - done;
-                    start[b].seq = s;
-                    start[b].kvh = kvh;
-                    start[b].at = at;
-                    start[b].tile = off > TGKV_GROUP_ITEM_COST ? (uint32_t)(off - TGKV_GROUP_ITEM_COST) : 0;
-                    if (start[b].tile) p->n_split++;
-                }
-                done = end;
-            }
-        }
-    }
-    start[n_cta].seq = c->n_seq + 1;
-    start[n_cta].kvh = start[n_cta].at = start[n_cta].tile = 0;
+    p->line[0].cta_rows = p->share ? (uint32_t)(2 * total * c->n_heads) : 0;
+    p->line[1].cta_rows = p->line[0].cta_rows + 2 * 256 * p->line[0].n_cta;
     return 1;
 }
 
@@ -1182,17 +1206,21 @@ static int encode_group_qmap(const TGKvGroupParams* p, CUtensorMap* out) {
 
 int tg_cuda_kv_group_plan(const TGCudaGroupCall* c, uint32_t sms, uint32_t* share, uint32_t* n_cta,
                           uint32_t* starts) {
-    static _Thread_local TGKvGroupParams p;    /* 11 KB: keep off the stack */
+    static _Thread_local TGKvGroupParams p;    /* 14 KB: keep off the stack */
     if (!share || !n_cta || !starts) { set_err("group: NULL pointer"); return 0; }
     if (!plan_group(c, sms, &p)) return 0;
     *share = p.share;
-    *n_cta = p.n_cta;
-    memcpy(starts, p.start, (p.n_cta + 1) * sizeof(TGKvGroupPos));
+    for (int l = 0; l < 2; l++) {
+        n_cta[l] = p.line[l].n_cta;
+        if (n_cta[l])
+            memcpy(starts + (size_t)l * (TGKV_GROUP_MAX_CTAS + 1) * 4, p.line[l].start,
+                   (n_cta[l] + 1) * sizeof(TGKvGroupPos));
+    }
     return 1;
 }
 
 int tg_cuda_kv_group_attention(const TGCudaGroupCall* c, void* stream) {
-    static _Thread_local TGKvGroupParams p;    /* 11 KB: keep off the stack */
+    static _Thread_local TGKvGroupParams p;    /* 14 KB: keep off the stack */
     if (!c || !c->table_dev || !c->scratch || !c->q || !c->out) {
         set_err("group: NULL pointer");
         return 0;
@@ -1204,7 +1232,7 @@ int tg_cuda_kv_group_attention(const TGCudaGroupCall* c, void* stream) {
     }
     if (!plan_group(c, (uint32_t)g_sm_count, &p)) return 0;
     if (!g_ready && !tg_cuda_kv_init()) return 0;
-    if (p.n_cta == 0) return 1;
+    if (p.line[0].n_cta + p.line[1].n_cta == 0) return 1;
     p.table = (const TGKvRowCache*)c->table_dev;
     p.tmaps = (uint64_t)(uintptr_t)c->table_dev + group_maps_offset(c->n_seq);
     p.q = c->q;

@@ -35,26 +35,24 @@
 //
 // Every mbarrier wait is bounded; one that runs out sets the device error word
 // and the CTA ends without further waits on its own data.
-#include <cuda.h>
-#include <cuda_runtime.h>
-#include <math.h>
-#include <stdint.h>
-#include <stdlib.h>
-
-#include "tgkv_group_plan.h"
-#include "tgkv_launch.h"
-#include "tgkv_ptx.cuh"
+#include "tgkv_group.cuh"
 
 namespace tgkv {
 namespace group {
 
-constexpr int kRows = TGKV_GROUP_ROWS, kPos = TGKV_GROUP_TILE;
 constexpr int kThreads = 384;
 constexpr int kTmaWarp = 8, kMmaWarp = 9;
-constexpr uint32_t kBlock = 16384;              // 128 rows x 64 bf16: one swizzled box
 constexpr uint32_t TM_S = 0, TM_O = 256, TM_COLS = 512;
-constexpr int kErrTimeout = 7;
 constexpr int kSub = 64;                        // half a tile
+
+// An item as this kernel works on it.
+struct PieceRows : ItemRows {
+    bool wide;                                   // two row tiles
+    __device__ PieceRows(const TGKvGroupShape& s, const Pieces& pc, int terms)
+        : ItemRows(s, pc), wide(terms == 1 && tokens > s.tpt) {}
+    // 64-position halves of tile j that hold rows
+    __device__ uint32_t halves(uint32_t j) const { return rows(j) - pos(j) > kSub ? 2 : 1; }
+};
 
 template <int HD>
 struct Cfg {
@@ -81,78 +79,6 @@ struct Cfg {
 __device__ __forceinline__ void pair_sync(int quarter) {
     asm volatile("bar.sync %0, 64;" ::"r"(1 + quarter) : "memory");
 }
-__device__ __forceinline__ float lo_f(uint32_t x) { return __uint_as_float(x << 16); }
-__device__ __forceinline__ float hi_f(uint32_t x) { return __uint_as_float(x & 0xffff0000u); }
-
-__device__ __forceinline__ TGKvGroupPos start_of(const TGKvGroupParams& p, uint32_t b) {
-    return TGKvGroupPos{p.start[4 * b], p.start[4 * b + 1], p.start[4 * b + 2], p.start[4 * b + 3]};
-}
-__device__ __forceinline__ TGKvGroupShape shape_of(const TGKvGroupParams& p, const uint32_t* old_len,
-                                                   const uint32_t* tok0) {
-    const uint32_t tpt = kRows / (p.n_heads / p.n_kv_heads);
-    return TGKvGroupShape{p.n_seq, p.n_kv_heads, p.prefix_len, p.share, tpt, tpt * p.pair, old_len, tok0};
-}
-
-// The pieces of a CTA's stretch, one after another.  With `most` > 0 an item's
-// tiles come in pieces of at most that many (their results add up in a slot).
-struct Pieces {
-    TGKvGroupPos at, end;
-    uint32_t j0, j1;                             // tiles [j0, j1) of the item
-    uint32_t nt, first;                          // the item's tiles; where this CTA began with it
-    __device__ Pieces(const TGKvGroupShape& s, TGKvGroupPos a, TGKvGroupPos e, uint32_t most) : at(a), end(e) {
-        set(s, most);
-    }
-    __device__ bool more() const { return j0 < j1; }
-    __device__ void next(const TGKvGroupShape& s, uint32_t most) {
-        const uint32_t stop = tgkv_group_same_item(at, end) ? end.tile : nt;
-        if (j1 < stop) {                         // more of the same item
-            j0 = j1;
-            j1 = most && stop - j0 > most ? j0 + most : stop;
-            return;
-        }
-        if (tgkv_group_same_item(at, end)) { j0 = j1; return; }
-        at = tgkv_group_next_item(&s, at);
-        set(s, most);
-    }
-    // the last piece of the item in this CTA
-    __device__ bool last() const { return j1 == (tgkv_group_same_item(at, end) ? end.tile : nt); }
-
-private:
-    __device__ void set(const TGKvGroupShape& s, uint32_t most) {
-        first = j0 = at.tile;
-        nt = at.seq <= s.n_seq ? tgkv_group_item_tiles(&s, at.seq, at.at) : 0;
-        const uint32_t stop = tgkv_group_same_item(at, end) ? end.tile : nt;
-        j1 = most && stop - j0 > most ? j0 + most : stop;
-    }
-};
-
-// What a piece's tiles see: shared by the MMA and softmax warps.
-struct PieceRows {
-    uint32_t npre, prefix_len, own_rows;         // prefix tiles; rows some query of the item sees of each part
-    bool wide;
-    __device__ PieceRows(const TGKvGroupShape& s, const Pieces& pc, int terms)
-        : npre(tgkv_group_prefix_tiles(&s, pc.at.seq)), prefix_len(s.prefix_len),
-          own_rows(pc.at.seq ? tgkv_group_own_rows(&s, pc.at.seq, pc.at.at) : 0),
-          wide(terms == 1 && tgkv_group_tokens(&s, pc.at.seq) - pc.at.at * s.item_tokens > s.tpt) {}
-    __device__ bool own(uint32_t j) const { return j >= npre; }
-    __device__ uint32_t pos(uint32_t j) const { return (j >= npre ? j - npre : j) * kPos; }
-    __device__ uint32_t rows(uint32_t j) const { return j >= npre ? own_rows : prefix_len; }
-    // 64-position halves of tile j that hold rows
-    __device__ uint32_t halves(uint32_t j) const { return rows(j) - pos(j) > kSub ? 2 : 1; }
-};
-
-// The sequence of packed token t: the last one whose first token is at or
-// before t among those with tokens.
-__device__ __forceinline__ uint32_t seq_of(const TGKvGroupParams& p, uint32_t t) {
-    uint32_t lo = 0, hi = p.n_seq;
-    while (hi - lo > 1) {
-        const uint32_t mid = (lo + hi) >> 1;
-        if (p.tok0[mid] <= t) lo = mid;
-        else hi = mid;
-    }
-    return lo;
-}
-
 // The packed rows of k_new / v_new into their caches, 8 elements per thread.
 template <typename T>
 __global__ void __launch_bounds__(256) group_append_kernel(const __grid_constant__ TGKvGroupParams p) {
@@ -178,13 +104,6 @@ __global__ void __launch_bounds__(256) group_append_kernel(const __grid_constant
     asm volatile("fence.proxy.async.global;" ::: "memory");
 }
 
-// The larger of three; NaN if one is, so that a NaN score reaches the row's maximum
-// and with it all its weights.
-__device__ __forceinline__ float max3(float a, float b, float c) {
-    float d;
-    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
-    return d;
-}
 template <bool MASK>
 __device__ __forceinline__ float max32(const uint32_t (&v)[32], int lim) {
     float a[4];
@@ -229,22 +148,6 @@ __device__ __forceinline__ void exp32(const uint32_t (&v)[32], float scale, floa
     }
     tmem_st16(col, ph);
     if (TERMS == 2) tmem_st16(col + 32, pl);
-}
-
-// 16 consecutive columns of this thread's TMEM lane.
-__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
-        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-        : "r"(taddr));
-}
-__device__ __forceinline__ void tmem_wait_ld16(uint32_t (&r)[16]) {
-    asm volatile("tcgen05.wait::ld.sync.aligned;"
-                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
-                   "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]),
-                   "+r"(r[15])::"memory");
 }
 
 // Half a query row of fp32 (64-dim halves of HD dims) as hi and lo bf16 words into
@@ -316,12 +219,12 @@ __global__ void __launch_bounds__(kThreads, 1) group_kernel(const __grid_constan
     tc_fence_after();
     const uint32_t tmem = *tslot;
     const uint32_t G = p.n_heads / p.n_kv_heads;
-    const TGKvGroupShape sh = shape_of(p, old_len, tok0);
+    const TGKvGroupShape sh = shape_of(p, 0, old_len, tok0);
     // Everything above overlaps the previous kernel on the stream.
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
-    Pieces pc(sh, start_of(p, blockIdx.x), start_of(p, blockIdx.x + 1), kMost);
+    Pieces pc(sh, start_of(p, 0, blockIdx.x), start_of(p, 0, blockIdx.x + 1), kMost);
     if (warp >= 8) {
         if (warp == kTmaWarp && lane == 0) {
             uint32_t nk = 0, nv = 0, it = 0;     // K and V tiles and pieces issued
@@ -600,7 +503,7 @@ __global__ void __launch_bounds__(kThreads, 1) group_kernel(const __grid_constan
             const bool again = pc.j0 > pc.first;                                 // adds to the item's earlier piece here
             const uint32_t irow = (wide ? (uint32_t)h * kRows : 0u) + (uint32_t)r;
             uint64_t slot;
-            if (pc.first > 0 || !p.share) slot = (uint64_t)p.cta_rows + 512u * blockIdx.x + (pc.first > 0 ? 0u : 256u) + irow;
+            if (pc.first > 0 || !p.share) slot = (uint64_t)p.line[0].cta_rows + 512u * blockIdx.x + (pc.first > 0 ? 0u : 256u) + irow;
             else slot = (seq ? total_rows : 0u) + row;
             float keep = 0.f;                                                    // weight of the slot's earlier sum
             float2* slot_ml = reinterpret_cast<float2*>(p.part_ml) + slot;
@@ -634,7 +537,7 @@ __global__ void __launch_bounds__(kThreads, 1) group_kernel(const __grid_constan
                     dst[i] = __shfl_sync(0xffffffffu, mine_row, (lane >> 2) + 8 * i);
                     kp[i] = TERMS == 2 ? __shfl_sync(0xffffffffu, keep, (lane >> 2) + 8 * i) : 0.f;
                 }
-                const uint64_t cta_slot = (uint64_t)p.cta_rows + 512u * blockIdx.x + 256u;   // a whole item's earlier sums
+                const uint64_t cta_slot = (uint64_t)p.line[0].cta_rows + 512u * blockIdx.x + 256u;   // a whole item's earlier sums
                 auto flush = [&](const uint4 (&w)[4], unsigned char* out, uint32_t row_bytes, uint32_t off, bool add) {
 #pragma unroll
                     for (int q = 0; q < 4; ++q)
@@ -764,22 +667,28 @@ struct Acc {
     }
 };
 
+// Partial rows a CTA of a line has: of the item it continues, then of the one it
+// leaves unfinished.
+__device__ __forceinline__ uint32_t slot_rows(int line) { return line ? TGKV_GROUP_LIGHT_ROWS : 2 * kRows; }
+
 // Adds the pieces of item `it` that continue it: those of the CTAs behind the one
 // with its tile 0.
 template <int HD>
-__device__ __forceinline__ void add_continued(const TGKvGroupParams& p, Acc<HD>& acc, TGKvGroupPos it, uint32_t r, int lane) {
-    uint32_t lo = 0, hi = p.n_cta;               // the last CTA that starts at or before the item
+__device__ __forceinline__ void add_continued(const TGKvGroupParams& p, int line, Acc<HD>& acc, TGKvGroupPos it, uint32_t r,
+                                              int lane) {
+    const uint32_t n = p.line[line].n_cta;
+    uint32_t lo = 0, hi = n;                     // the last CTA that starts at or before the item
     while (hi - lo > 1) {
         const uint32_t mid = (lo + hi) >> 1;
-        if (tgkv_group_le(start_of(p, mid), it)) lo = mid;
+        if (tgkv_group_le(start_of(p, line, mid), it)) lo = mid;
         else hi = mid;
     }
-    for (uint32_t b = lo + 1; b < p.n_cta; ++b) {
-        const TGKvGroupPos s = start_of(p, b);
+    for (uint32_t b = lo + 1; b < n; ++b) {
+        const TGKvGroupPos s = start_of(p, line, b);
         if (!tgkv_group_same_item(s, it)) break;
-        const TGKvGroupPos e = start_of(p, b + 1);
+        const TGKvGroupPos e = start_of(p, line, b + 1);
         if (tgkv_group_same_item(s, e) && s.tile == e.tile) continue;            // an empty stretch
-        acc.add(p, (uint64_t)p.cta_rows + 512u * b + r, lane);
+        acc.add(p, (uint64_t)p.line[line].cta_rows + 2u * slot_rows(line) * b + r, lane);
     }
 }
 
@@ -797,15 +706,17 @@ __global__ void __launch_bounds__(256) group_merge_parts_kernel(const __grid_con
     const int lane = threadIdx.x & 31;
     if (row >= total) return;
     const uint32_t G = p.n_heads / p.n_kv_heads;
-    const TGKvGroupShape sh = shape_of(p, p.old_len, p.tok0);
+    const int lp = p.prefix_line, lo = p.own_line;
+    const TGKvGroupShape sp = shape_of(p, lp, p.old_len, p.tok0), so = shape_of(p, lo, p.old_len, p.tok0);
     const uint32_t t = row / p.n_heads, h = row % p.n_heads, kvh = h / G, sub = h % G;
     const uint32_t i = seq_of(p, t), own = t - p.tok0[i];
     Acc<HD> acc;
     acc.add(p, row, lane);
-    add_continued<HD>(p, acc, TGKvGroupPos{0, kvh, t / sh.item_tokens, 0}, item_row(sh, t % sh.item_tokens, G, sub), lane);
+    add_continued<HD>(p, lp, acc, TGKvGroupPos{0, kvh, t / sp.item_tokens, 0}, item_row(sp, t % sp.item_tokens, G, sub),
+                      lane);
     acc.add(p, (uint64_t)total + row, lane);
-    add_continued<HD>(p, acc, TGKvGroupPos{i + 1, kvh, own / sh.item_tokens, 0},
-                      item_row(sh, own % sh.item_tokens, G, sub), lane);
+    add_continued<HD>(p, lo, acc, TGKvGroupPos{i + 1, kvh, own / so.item_tokens, 0},
+                      item_row(so, own % so.item_tokens, G, sub), lane);
     acc.template store<T>(p, row, lane);
 }
 
@@ -816,69 +727,49 @@ __global__ void __launch_bounds__(256) group_merge_split_kernel(const __grid_con
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const uint32_t b = blockIdx.x;
-    const TGKvGroupPos s = start_of(p, b), e = start_of(p, b + 1);
+    const int line = p.own_line;
+    const TGKvGroupPos s = start_of(p, line, b), e = start_of(p, line, b + 1);
     // the item that the next CTA continues, begun in this one
     if (e.seq > p.n_seq || e.tile == 0 || (tgkv_group_same_item(s, e) && s.tile > 0)) return;
     TGKvGroupPos it = e;
     it.tile = 0;
     const uint32_t G = p.n_heads / p.n_kv_heads;
-    const TGKvGroupShape sh = shape_of(p, p.old_len, p.tok0);
+    const TGKvGroupShape sh = shape_of(p, line, p.old_len, p.tok0);
     const uint32_t t0 = it.at * sh.item_tokens, ntok = min(sh.item_tokens, tgkv_group_tokens(&sh, it.seq) - t0);
     const int lane = threadIdx.x & 31;
     for (uint32_t x = blockIdx.y * 16 + (threadIdx.x >> 5); x < blockIdx.y * 16 + 16 && x < ntok * G; x += 8) {
         const uint32_t t = x / G, sub = x % G, r = item_row(sh, t, G, sub);
         Acc<HD> acc;
-        acc.add(p, (uint64_t)p.cta_rows + 512u * b + 256u + r, lane);
-        add_continued<HD>(p, acc, it, r, lane);
+        acc.add(p, (uint64_t)p.line[line].cta_rows + slot_rows(line) * (2 * b + 1) + r, lane);
+        add_continued<HD>(p, line, acc, it, r, lane);
         acc.template store<T>(p, (uint64_t)(p.tok0[it.seq - 1] + t0 + t) * p.n_heads + it.kvh * G + sub, lane);
     }
-}
-
-// Programmatic dependent launch (TGKV_PDL=0 turns it off): each kernel waits
-// (griddepcontrol.wait) before its first access to global memory.
-template <typename K>
-cudaError_t launch_pdl(K kernel, dim3 grid, int threads, uint32_t smem, cudaStream_t st, const TGKvGroupParams* p) {
-    static const bool pdl = [] {
-        const char* e = getenv("TGKV_PDL");
-        return !(e && e[0] == '0');
-    }();
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = grid;
-    cfg.blockDim = dim3(threads);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = st;
-    cudaLaunchAttribute at[1];
-    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = at;
-    cfg.numAttrs = pdl ? 1 : 0;
-    return cudaLaunchKernelEx(&cfg, kernel, *p);
 }
 
 template <typename T, int HD>
 int launch(const TGKvGroupParams* p, cudaStream_t st) {
     const uint32_t total = p->tok0[p->n_seq];
-    int dev = 0;
-    cudaError_t e = cudaGetDevice(&dev);
+    static bool done[64];
+    cudaError_t e = allow_smem(group_kernel<T, HD>, Cfg<HD>::SMEM, done);
     if (e != cudaSuccess) return (int)e;
-    static bool configured[64];                  // benign race: same value
-    if (dev < 0 || dev >= 64) return (int)cudaErrorInvalidDevice;
-    if (!configured[dev]) {
-        e = cudaFuncSetAttribute(group_kernel<T, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<HD>::SMEM);
-        if (e != cudaSuccess) return (int)e;
-        configured[dev] = true;
-    }
     if (p->k_new) {
         const uint64_t n = (uint64_t)total * (p->n_kv_heads * HD / 8);
         e = launch_pdl(group_append_kernel<T>, dim3((unsigned)((n + 255) / 256), 2), 256, 0, st, p);
         if (e != cudaSuccess) return (int)e;
     }
-    e = launch_pdl(group_kernel<T, HD>, dim3(p->n_cta), kThreads, Cfg<HD>::SMEM, st, p);
-    if (e != cudaSuccess) return (int)e;
+    if (p->line[0].n_cta) {
+        e = launch_pdl(group_kernel<T, HD>, dim3(p->line[0].n_cta), kThreads, Cfg<HD>::SMEM, st, p);
+        if (e != cudaSuccess) return (int)e;
+    }
+    if (p->line[1].n_cta) {
+        const int r = tgkv_launch_group_light(p, sizeof(T) == 2, (void*)st);
+        if (r) return r;
+    }
+    const TGKvGroupLine* own = &p->line[p->own_line];
     if (p->share)
         e = launch_pdl(group_merge_parts_kernel<T, HD>, dim3((total * p->n_heads + 7) / 8), 256, 0, st, p);
-    else if (p->n_split)
-        e = launch_pdl(group_merge_split_kernel<T, HD>, dim3(p->n_cta, 8 * p->pair), 256, 0, st, p);
+    else if (own->n_split)
+        e = launch_pdl(group_merge_split_kernel<T, HD>, dim3(own->n_cta, p->own_line ? 1 : 16), 256, 0, st, p);
     return (int)e;
 }
 

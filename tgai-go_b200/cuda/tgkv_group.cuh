@@ -1,0 +1,151 @@
+// tgkv_group.cuh -- device code shared by the kernels of tgkv_group.cu and
+// tgkv_group_light.cu: the pieces of a CTA's stretch (tgkv_group_plan.h), TMEM
+// access and the launch helper.
+#pragma once
+#include <cuda.h>
+#include <cuda_runtime.h>
+#include <math.h>
+#include <stdint.h>
+#include <stdlib.h>
+
+#include "tgkv_group_plan.h"
+#include "tgkv_launch.h"
+#include "tgkv_ptx.cuh"
+
+namespace tgkv {
+namespace group {
+
+constexpr int kRows = TGKV_GROUP_ROWS, kPos = TGKV_GROUP_TILE;
+constexpr uint32_t kBlock = 16384;              // 128 rows x 64 bf16: one swizzled box
+constexpr int kErrTimeout = 7;
+
+__device__ __forceinline__ float lo_f(uint32_t x) { return __uint_as_float(x << 16); }
+__device__ __forceinline__ float hi_f(uint32_t x) { return __uint_as_float(x & 0xffff0000u); }
+
+__device__ __forceinline__ TGKvGroupPos start_of(const TGKvGroupParams& p, int line, uint32_t b) {
+    const uint32_t* s = p.line[line].start + 4 * b;
+    return TGKvGroupPos{s[0], s[1], s[2], s[3]};
+}
+__device__ __forceinline__ TGKvGroupShape shape_of(const TGKvGroupParams& p, int line, const uint32_t* old_len,
+                                                   const uint32_t* tok0) {
+    return TGKvGroupShape{p.n_seq, p.n_kv_heads, p.prefix_len, p.share, kRows / (p.n_heads / p.n_kv_heads),
+                          p.line[line].item_tokens, old_len, tok0};
+}
+
+// The pieces of a CTA's stretch, one after another.  With `most` > 0 an item's
+// tiles come in pieces of at most that many (their results add up in a slot).
+struct Pieces {
+    TGKvGroupPos at, end;
+    uint32_t j0, j1;                             // tiles [j0, j1) of the item
+    uint32_t nt, first;                          // the item's tiles; where this CTA began with it
+    __device__ Pieces(const TGKvGroupShape& s, TGKvGroupPos a, TGKvGroupPos e, uint32_t most) : at(a), end(e) {
+        set(s, most);
+    }
+    __device__ bool more() const { return j0 < j1; }
+    __device__ void next(const TGKvGroupShape& s, uint32_t most) {
+        const uint32_t stop = tgkv_group_same_item(at, end) ? end.tile : nt;
+        if (j1 < stop) {                         // more of the same item
+            j0 = j1;
+            j1 = most && stop - j0 > most ? j0 + most : stop;
+            return;
+        }
+        if (tgkv_group_same_item(at, end)) { j0 = j1; return; }
+        at = tgkv_group_next_item(&s, at);
+        set(s, most);
+    }
+    // the last piece of the item in this CTA
+    __device__ bool last() const { return j1 == (tgkv_group_same_item(at, end) ? end.tile : nt); }
+
+private:
+    __device__ void set(const TGKvGroupShape& s, uint32_t most) {
+        first = j0 = at.tile;
+        nt = at.seq <= s.n_seq ? tgkv_group_item_tiles(&s, at.seq, at.at) : 0;
+        const uint32_t stop = tgkv_group_same_item(at, end) ? end.tile : nt;
+        j1 = most && stop - j0 > most ? j0 + most : stop;
+    }
+};
+
+// What an item's tiles see.
+struct ItemRows {
+    uint32_t npre, prefix_len, own_rows;         // prefix tiles; rows some query of the item sees of each part
+    uint32_t tokens;                             // of the item
+    __device__ ItemRows(const TGKvGroupShape& s, const Pieces& pc)
+        : npre(tgkv_group_prefix_tiles(&s, pc.at.seq)), prefix_len(s.prefix_len),
+          own_rows(pc.at.seq ? tgkv_group_own_rows(&s, pc.at.seq, pc.at.at) : 0),
+          tokens(min(s.item_tokens, tgkv_group_tokens(&s, pc.at.seq) - pc.at.at * s.item_tokens)) {}
+    __device__ bool own(uint32_t j) const { return j >= npre; }
+    __device__ uint32_t pos(uint32_t j) const { return (j >= npre ? j - npre : j) * kPos; }
+    __device__ uint32_t rows(uint32_t j) const { return j >= npre ? own_rows : prefix_len; }
+};
+
+// The sequence of packed token t: the last one whose first token is at or
+// before t among those with tokens.
+__device__ __forceinline__ uint32_t seq_of(const TGKvGroupParams& p, uint32_t t) {
+    uint32_t lo = 0, hi = p.n_seq;
+    while (hi - lo > 1) {
+        const uint32_t mid = (lo + hi) >> 1;
+        if (p.tok0[mid] <= t) lo = mid;
+        else hi = mid;
+    }
+    return lo;
+}
+
+// The larger of three; NaN if one is, so that a NaN score reaches the row's maximum
+// and with it all its weights.
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+// 16 consecutive columns of this thread's TMEM lane.
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_wait_ld16(uint32_t (&r)[16]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                   "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]),
+                   "+r"(r[15])::"memory");
+}
+
+// Programmatic dependent launch (TGKV_PDL=0 turns it off): each kernel waits
+// (griddepcontrol.wait) before its first access to global memory.
+template <typename K>
+cudaError_t launch_pdl(K kernel, dim3 grid, int threads, uint32_t smem, cudaStream_t st, const TGKvGroupParams* p) {
+    static const bool pdl = [] {
+        const char* e = getenv("TGKV_PDL");
+        return !(e && e[0] == '0');
+    }();
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = pdl ? 1 : 0;
+    return cudaLaunchKernelEx(&cfg, kernel, *p);
+}
+
+// The kernel's shared memory size, once per device.
+template <typename K>
+cudaError_t allow_smem(K kernel, uint32_t bytes, bool (&done)[64]) {
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
+    if (done[dev]) return cudaSuccess;           // benign race: same value
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    done[dev] = e == cudaSuccess;
+    return e;
+}
+
+}  // namespace group
+}  // namespace tgkv

@@ -3,9 +3,9 @@
  * the kernels (tgkv_group.cu).
  *
  * A row tile is up to 128 query rows of one KV head: 128 / G tokens times the G
- * query heads of that KV head.  An item is `pair` (1 or 2) consecutive row tiles
- * with the 128-position K/V tiles they attend.  There are two ways to cut a
- * call:
+ * query heads of that KV head.  An item is one or two consecutive row tiles, or
+ * (light) up to 16 query rows, with the 128-position K/V tiles they attend.
+ * There are two ways to cut a call:
  *   split   (share = 1) items over the packed tokens of all sequences attend the
  *           prefix ("sequence" 0 below), items of each sequence's own tokens
  *           attend its own cache, and a merge joins the two parts of every row:
@@ -13,13 +13,17 @@
  *           sequences they come from;
  *   joined  (share = 0) items of each sequence attend the prefix, then the own
  *           cache.
- * Items in order (sequence, KV head, place in the sequence) form one line of
+ * Items in order (sequence, KV head, place in the sequence) form a line of
  * tiles, which is cut into n_cta contiguous stretches of about the same cost
  * (tiles plus TGKV_GROUP_ITEM_COST per item).  A CTA's stretch is a run of
  * pieces: parts of an item's tiles.  Only a stretch's first piece can continue
  * an item and only its last piece can leave one unfinished, so partial results
  * need two slots of an item's rows per CTA (and, split, one row per query row
  * and part).
+ * Line 0 holds the items of tgkv_group.cu, line 1 those of tgkv_group_light.cu:
+ * the sequences' own items when none of them has more than the light rows (most
+ * decode steps), and with them the prefix's when all tokens together are that
+ * few.
  */
 #ifndef TGKV_GROUP_PLAN_H
 #define TGKV_GROUP_PLAN_H
@@ -41,7 +45,7 @@
 typedef struct {
     uint32_t n_seq, n_kv_heads, prefix_len, share;
     uint32_t tpt;                /* tokens of a row tile: 128 / G */
-    uint32_t item_tokens;        /* tokens of an item: pair * tpt */
+    uint32_t item_tokens;        /* tokens of an item */
     const uint32_t* old_len;     /* [n_seq] */
     const uint32_t* tok0;        /* [n_seq + 1] */
 } TGKvGroupShape;

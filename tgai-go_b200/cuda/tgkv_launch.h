@@ -201,6 +201,18 @@ typedef struct {
 /* ---- groups of caches with a shared prefix (tgkv_group.cu); the plan is in
  * tgkv_group_plan.h ---- */
 typedef struct {
+    uint32_t n_cta;
+    uint32_t item_tokens;        /* tokens of an item */
+    uint32_t n_split;            /* CTAs that continue an item */
+    uint32_t cta_rows;           /* first partial row of the CTAs' slots: CTA b has 2 S rows from
+                                  * cta_rows + 2 S b on, S for the item it continues, then S for
+                                  * the one it leaves unfinished; S = 256 on line 0,
+                                  * TGKV_GROUP_LIGHT_ROWS on line 1 */
+    uint32_t start[(TGKV_GROUP_MAX_CTAS + 1) * 4];  /* TGKvGroupPos of each CTA, and the end */
+} TGKvGroupLine;
+#define TGKV_GROUP_LIGHT_ROWS 16 /* query rows of a light item at most */
+
+typedef struct {
     /* bf16 activations: q as a 3-D map (head_dim, n_heads, tokens), 128-byte
      * swizzle, box (64, G, 128 / G): 64 head dims of a row tile */
     CUtensorMap qmap;
@@ -212,26 +224,25 @@ typedef struct {
     const void* v_new;
     void*       out;             /* as q */
     /* partial rows: [..][head_dim] unnormalised outputs and [..][2] (maximum,
-     * in the log2 domain, and sum of weights) */
+     * in the log2 domain, and sum of weights).  With share, query row x's prefix
+     * part is row x and its own part row total rows + x; then the CTAs' slots */
     float*      part_o;
     float*      part_ml;
     int32_t*    err;             /* device error word */
     uint32_t n_seq, n_heads, n_kv_heads, head_dim;
     uint32_t prefix_len;
     float    qscale;             /* softmax scale * log2(e) */
-    uint32_t share, pair, n_cta;
-    uint32_t cta_rows;           /* first partial row of the CTAs' slots: CTA b's rows are
-                                  * cta_rows + 512 b + (0: the item it continues, 256: the one
-                                  * it leaves unfinished) + row of the item; below it, with share,
-                                  * query row x's prefix part at x and own part at total + x */
-    uint32_t n_split;            /* CTAs that continue an item */
+    uint32_t share;
+    uint32_t prefix_line, own_line;   /* whose items the shared prefix's and the sequences' are */
+    uint32_t pad;
+    TGKvGroupLine line[2];
     uint32_t old_len[TGKV_MAX_ITEMS];       /* own rows before the call's tokens */
     uint32_t tok0[TGKV_MAX_ITEMS + 1];      /* first packed token of each sequence; the total */
-    uint32_t start[(TGKV_GROUP_MAX_CTAS + 1) * 4];  /* TGKvGroupPos of each CTA, and the end */
 } TGKvGroupParams;
 int tgkv_launch_fork(const TGKvForkParams* p, void* stream);
 int tgkv_launch_compact(const TGKvCompactParams* p, uint32_t cluster, void* stream);
-/* act: 0 fp32, 1 bf16 activations */
+/* act: 0 fp32, 1 bf16 activations; the second: line 1 alone */
+int tgkv_launch_group_light(const TGKvGroupParams* p, int act, void* stream);
 int tgkv_launch_group(const TGKvGroupParams* p, int act, void* stream);
 
 /* Launchers (tgkv_kernels.cu, tgkv_prefill.cu, tgkv_prefill_f32.cu).  Return 0
