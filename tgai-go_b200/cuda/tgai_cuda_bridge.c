@@ -1178,8 +1178,19 @@ static int plan_group(const TGCudaGroupCall* c, uint32_t sms, TGKvGroupParams* p
     if (!own_light) plan_line(&heavy, 0, c->n_seq, sms, &p->line[0]);
     else if (all_light) plan_line(&light, 0, c->n_seq, sms, &p->line[1]);
     else {
-        plan_line(&heavy, 0, 0, sms, &p->line[0]);
-        plan_line(&light, 1, c->n_seq, sms, &p->line[1]);
+        /* both lines at once, each on the SMs its work takes: a tile of line 0 about
+         * 1.2 us (2.3 us for two row tiles), one of line 1 1 us and an item 2 us more */
+        uint64_t w0 = 0, w1 = 0;
+        const uint64_t pre = tgkv_group_prefix_tiles(&heavy, 0), items = tgkv_group_items(&heavy, 0);
+        w0 = pre * items * (total > tpt && c->act == 1 ? 23 : 12);
+        for (uint32_t i = 1; i <= c->n_seq; i++)
+            if (c->n_new[i - 1]) w1 += 20 + 10ull * tgkv_group_item_tiles(&light, i, 0);
+        if (sms == 0 || sms > TGKV_GROUP_MAX_CTAS) sms = TGKV_GROUP_MAX_CTAS;
+        uint32_t n0 = (uint32_t)((sms * w0 + (w0 + w1) / 2) / (w0 + w1));
+        if (n0 < 1) n0 = 1;
+        if (n0 + 1 > sms) n0 = sms > 1 ? sms - 1 : 1;
+        plan_line(&heavy, 0, 0, n0, &p->line[0]);
+        plan_line(&light, 1, c->n_seq, sms > n0 ? sms - n0 : 1, &p->line[1]);
     }
     p->line[0].cta_rows = p->share ? (uint32_t)(2 * total * c->n_heads) : 0;
     p->line[1].cta_rows = p->line[0].cta_rows + 2 * 256 * p->line[0].n_cta;

@@ -36,11 +36,11 @@
 // Every mbarrier wait is bounded; one that runs out sets the device error word
 // and the CTA ends without further waits on its own data.
 #include "tgkv_group.cuh"
+#include "tgkv_group_light.cuh"
 
 namespace tgkv {
 namespace group {
 
-constexpr int kThreads = 384;
 constexpr int kTmaWarp = 8, kMmaWarp = 9;
 constexpr uint32_t TM_S = 0, TM_O = 256, TM_COLS = 512;
 constexpr int kSub = 64;                        // half a tile
@@ -82,16 +82,19 @@ __device__ __forceinline__ void pair_sync(int quarter) {
 // The packed rows of k_new / v_new into their caches, 8 elements per thread.
 template <typename T>
 __global__ void __launch_bounds__(256) group_append_kernel(const __grid_constant__ TGKvGroupParams p) {
+    __shared__ uint32_t tok0[TGKV_MAX_ITEMS + 1];
+    copy_table(tok0, p.tok0, p.n_seq + 1, threadIdx.x, 256);
+    __syncthreads();
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const uint32_t kv_dim = p.n_kv_heads * p.head_dim, vec = kv_dim / 8;
     const uint64_t x = (uint64_t)blockIdx.x * blockDim.x + threadIdx.x;
-    if (x >= (uint64_t)p.tok0[p.n_seq] * vec) return;
-    const uint32_t t = (uint32_t)(x / vec), e = (uint32_t)(x % vec) * 8, i = seq_of(p, t);
+    if (x >= (uint64_t)tok0[p.n_seq] * vec) return;
+    const uint32_t t = (uint32_t)(x / vec), e = (uint32_t)(x % vec) * 8, i = seq_of(tok0, p.n_seq, t);
     const T* src = reinterpret_cast<const T*>(blockIdx.y ? p.v_new : p.k_new) + (uint64_t)t * kv_dim + e;
     const TGKvRowCache c = p.table[i];
     uint16_t* dst = reinterpret_cast<uint16_t*>(c.base) +
-                    ((uint64_t)blockIdx.y * c.max_seq + p.old_len[i] + (t - p.tok0[i])) * kv_dim + e;
+                    ((uint64_t)blockIdx.y * c.max_seq + as_memory(p.old_len)[i] + (t - tok0[i])) * kv_dim + e;
     uint4 w;
     if constexpr (sizeof(T) == 4) {
         const float4 a = *reinterpret_cast<const float4*>(src), b = *reinterpret_cast<const float4*>(src + 4);
@@ -173,14 +176,13 @@ __device__ __forceinline__ void store_q_terms(const float* src, bool valid, unsi
 }
 
 template <typename T, int HD>
-__global__ void __launch_bounds__(kThreads, 1) group_kernel(const __grid_constant__ TGKvGroupParams p) {
+__device__ __forceinline__ void run(const TGKvGroupParams& p, uint32_t cta_index, unsigned char* smem_raw) {
     constexpr int TERMS = sizeof(T) == 4 ? 2 : 1;
     // With two terms (fp32 results) an accumulator takes at most 16 tiles, 256 steps of
     // 16 positions: the tensor core's fp32 sums round towards zero, and the sums of
     // longer runs would lose more bits than the two terms keep.
     constexpr uint32_t kMost = TERMS == 2 ? 32 : 0;
     using C = Cfg<HD>;
-    extern __shared__ unsigned char smem_raw[];
     unsigned char* base =
         reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     const uint32_t sbase = smem_addr(base);
@@ -190,10 +192,8 @@ __global__ void __launch_bounds__(kThreads, 1) group_kernel(const __grid_constan
     uint32_t* old_len = tok0 + p.n_seq + 1;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
-    for (uint32_t i = tid; i <= p.n_seq; i += kThreads) {
-        tok0[i] = p.tok0[i];
-        if (i < p.n_seq) old_len[i] = p.old_len[i];
-    }
+    copy_table(tok0, p.tok0, p.n_seq + 1, tid, kThreads);
+    copy_table(old_len, p.old_len, p.n_seq, tid, kThreads);
     if (tid == 0) {
         for (int i = 0; i < C::kStages; ++i) {
             mbar_init(&bar[C::B_KFULL + i], 1);
@@ -224,7 +224,7 @@ __global__ void __launch_bounds__(kThreads, 1) group_kernel(const __grid_constan
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
-    Pieces pc(sh, start_of(p, 0, blockIdx.x), start_of(p, 0, blockIdx.x + 1), kMost);
+    Pieces pc(sh, start_of(p, 0, cta_index), start_of(p, 0, cta_index + 1), kMost);
     if (warp >= 8) {
         if (warp == kTmaWarp && lane == 0) {
             uint32_t nk = 0, nv = 0, it = 0;     // K and V tiles and pieces issued
@@ -503,7 +503,7 @@ __global__ void __launch_bounds__(kThreads, 1) group_kernel(const __grid_constan
             const bool again = pc.j0 > pc.first;                                 // adds to the item's earlier piece here
             const uint32_t irow = (wide ? (uint32_t)h * kRows : 0u) + (uint32_t)r;
             uint64_t slot;
-            if (pc.first > 0 || !p.share) slot = (uint64_t)p.line[0].cta_rows + 512u * blockIdx.x + (pc.first > 0 ? 0u : 256u) + irow;
+            if (pc.first > 0 || !p.share) slot = (uint64_t)p.line[0].cta_rows + 512u * cta_index + (pc.first > 0 ? 0u : 256u) + irow;
             else slot = (seq ? total_rows : 0u) + row;
             float keep = 0.f;                                                    // weight of the slot's earlier sum
             float2* slot_ml = reinterpret_cast<float2*>(p.part_ml) + slot;
@@ -537,7 +537,7 @@ __global__ void __launch_bounds__(kThreads, 1) group_kernel(const __grid_constan
                     dst[i] = __shfl_sync(0xffffffffu, mine_row, (lane >> 2) + 8 * i);
                     kp[i] = TERMS == 2 ? __shfl_sync(0xffffffffu, keep, (lane >> 2) + 8 * i) : 0.f;
                 }
-                const uint64_t cta_slot = (uint64_t)p.line[0].cta_rows + 512u * blockIdx.x + 256u;   // a whole item's earlier sums
+                const uint64_t cta_slot = (uint64_t)p.line[0].cta_rows + 512u * cta_index + 256u;   // a whole item's earlier sums
                 auto flush = [&](const uint4 (&w)[4], unsigned char* out, uint32_t row_bytes, uint32_t off, bool add) {
 #pragma unroll
                     for (int q = 0; q < 4; ++q)
@@ -625,36 +625,72 @@ __global__ void __launch_bounds__(kThreads, 1) group_kernel(const __grid_constan
     }
 }
 
+// Both lines in one launch, each on its share of the SMs: what bounds line 1 is
+// HBM, what bounds line 0 is not.
+template <typename T, int HD>
+__global__ void __launch_bounds__(kThreads, 1) group_kernel(const __grid_constant__ TGKvGroupParams p) {
+    extern __shared__ unsigned char smem_raw[];
+    if (blockIdx.x < p.line[0].n_cta) run<T, HD>(p, blockIdx.x, smem_raw);
+    else light::run<T, HD>(p, blockIdx.x - p.line[0].n_cta, smem_raw);
+}
+
 // ------------------------------------------------------------------ merge
 // A row's result from its partials (o, m, l): sum 2^(m - M) o / sum 2^(m - M) l.
-// One warp per query row, HD / 32 dims per lane.
+// One warp per query row, HD / 32 dims per lane.  Lane i keeps partial i's (m, l)
+// and, up to 32 at a time, all partials' rows are in flight at once: the kernel's
+// time is a few memory latencies.
 template <int HD>
 struct Acc {
     static constexpr int D = HD / 32;
     float o[D], m, l;
-    __device__ Acc() : m(-INFINITY), l(0.f) {
+    uint32_t n;                                  // partials noted
+    uint64_t slot;                               // lane i: partial i's row
+    __device__ Acc() : m(-INFINITY), l(0.f), n(0), slot(0) {
 #pragma unroll
         for (int d = 0; d < D; ++d) o[d] = 0.f;
     }
-    __device__ void add(const TGKvGroupParams& p, uint64_t slot, int lane) {
-        const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + slot * 2);
-        float x[D];
-        if constexpr (D == 4) {
-            const float4 v = *reinterpret_cast<const float4*>(p.part_o + slot * HD + lane * 4);
-            x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
-        } else {
-            const float2 v = *reinterpret_cast<const float2*>(p.part_o + slot * HD + lane * 2);
-            x[0] = v.x; x[1] = v.y;
-        }
-        if (ml.x == -INFINITY) return;           // no position of that part was visible to the row
-        const float M = fmaxf(m, ml.x), a = m == -INFINITY ? 0.f : ex2_approx(m - M), b = ex2_approx(ml.x - M);
-        l = l * a + ml.y * b;
+    // Notes a partial row.
+    __device__ void add(const TGKvGroupParams& p, uint64_t s, int lane) {
+        if (lane == (int)n) slot = s;
+        if (++n == 32) flush(p, lane);
+    }
+    __device__ void flush(const TGKvGroupParams& p, int lane) {
+        const float2 ml = lane < (int)n ? *reinterpret_cast<const float2*>(p.part_ml + slot * 2)
+                                        : make_float2(-INFINITY, 0.f);
+        float M = ml.x;
 #pragma unroll
-        for (int d = 0; d < D; ++d) o[d] = o[d] * a + x[d] * b;
+        for (int w = 16; w >= 1; w >>= 1) M = max3(M, __shfl_xor_sync(0xffffffffu, M, w), m);
+        // (a part of which the row saw nothing has m = -inf and counts nothing)
+        const float w = ml.x == -INFINITY ? 0.f : ex2_approx(ml.x - M), a = m == -INFINITY ? 0.f : ex2_approx(m - M);
+        float L = w * ml.y;
+#pragma unroll
+        for (int k = 16; k >= 1; k >>= 1) L += __shfl_xor_sync(0xffffffffu, L, k);
+        l = l * a + L;
+#pragma unroll
+        for (int d = 0; d < D; ++d) o[d] *= a;
+#pragma unroll 8
+        for (uint32_t i = 0; i < n; ++i) {
+            const uint64_t s = __shfl_sync(0xffffffffu, slot, i);
+            const float wi = __shfl_sync(0xffffffffu, w, i);
+            const float* src = p.part_o + s * HD + lane * D;
+            if constexpr (D == 4) {
+                const float4 v = *reinterpret_cast<const float4*>(src);
+                o[0] += wi == 0.f ? 0.f : wi * v.x;
+                o[1] += wi == 0.f ? 0.f : wi * v.y;
+                o[2] += wi == 0.f ? 0.f : wi * v.z;
+                o[3] += wi == 0.f ? 0.f : wi * v.w;
+            } else {
+                const float2 v = *reinterpret_cast<const float2*>(src);
+                o[0] += wi == 0.f ? 0.f : wi * v.x;
+                o[1] += wi == 0.f ? 0.f : wi * v.y;
+            }
+        }
         m = M;
+        n = 0;
     }
     template <typename T>
-    __device__ void store(const TGKvGroupParams& p, uint64_t row, int lane) const {
+    __device__ void store(const TGKvGroupParams& p, uint64_t row, int lane) {
+        if (n) flush(p, lane);
         const float inv = 1.f / l;
         T* dst = reinterpret_cast<T*>(p.out) + row * HD + lane * D;
         if constexpr (sizeof(T) == 4) {
@@ -671,22 +707,31 @@ struct Acc {
 // leaves unfinished.
 __device__ __forceinline__ uint32_t slot_rows(int line) { return line ? TGKV_GROUP_LIGHT_ROWS : 2 * kRows; }
 
+// A line's starts, in shared memory.
+struct Starts {
+    uint32_t s[(TGKV_GROUP_MAX_CTAS + 1) * 4];
+    __device__ void copy(const TGKvGroupParams& p, int line) {
+        copy_table(s, p.line[line].start, (p.line[line].n_cta + 1) * 4, threadIdx.x, blockDim.x);
+    }
+    __device__ TGKvGroupPos at(uint32_t b) const { return TGKvGroupPos{s[4 * b], s[4 * b + 1], s[4 * b + 2], s[4 * b + 3]}; }
+};
+
 // Adds the pieces of item `it` that continue it: those of the CTAs behind the one
 // with its tile 0.
 template <int HD>
-__device__ __forceinline__ void add_continued(const TGKvGroupParams& p, int line, Acc<HD>& acc, TGKvGroupPos it, uint32_t r,
-                                              int lane) {
+__device__ __forceinline__ void add_continued(const TGKvGroupParams& p, int line, const Starts& st, Acc<HD>& acc,
+                                              TGKvGroupPos it, uint32_t r, int lane) {
     const uint32_t n = p.line[line].n_cta;
     uint32_t lo = 0, hi = n;                     // the last CTA that starts at or before the item
     while (hi - lo > 1) {
         const uint32_t mid = (lo + hi) >> 1;
-        if (tgkv_group_le(start_of(p, line, mid), it)) lo = mid;
+        if (tgkv_group_le(st.at(mid), it)) lo = mid;
         else hi = mid;
     }
     for (uint32_t b = lo + 1; b < n; ++b) {
-        const TGKvGroupPos s = start_of(p, line, b);
+        const TGKvGroupPos s = st.at(b);
         if (!tgkv_group_same_item(s, it)) break;
-        const TGKvGroupPos e = start_of(p, line, b + 1);
+        const TGKvGroupPos e = st.at(b + 1);
         if (tgkv_group_same_item(s, e) && s.tile == e.tile) continue;            // an empty stretch
         acc.add(p, (uint64_t)p.line[line].cta_rows + 2u * slot_rows(line) * b + r, lane);
     }
@@ -700,22 +745,28 @@ __device__ __forceinline__ uint32_t item_row(const TGKvGroupShape& sh, uint32_t 
 // share: every query row, from its prefix part and its own part.
 template <typename T, int HD>
 __global__ void __launch_bounds__(256) group_merge_parts_kernel(const __grid_constant__ TGKvGroupParams p) {
+    __shared__ uint32_t tok0[TGKV_MAX_ITEMS + 1];
+    __shared__ Starts starts[2];
+    const int lp = p.prefix_line, lo = p.own_line;
+    copy_table(tok0, p.tok0, p.n_seq + 1, threadIdx.x, 256);
+    starts[lp].copy(p, lp);
+    if (lo != lp) starts[lo].copy(p, lo);
+    __syncthreads();
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const uint32_t row = blockIdx.x * 8 + (threadIdx.x >> 5), total = p.tok0[p.n_seq] * p.n_heads;
+    const uint32_t row = blockIdx.x * 8 + (threadIdx.x >> 5), total = tok0[p.n_seq] * p.n_heads;
     const int lane = threadIdx.x & 31;
     if (row >= total) return;
     const uint32_t G = p.n_heads / p.n_kv_heads;
-    const int lp = p.prefix_line, lo = p.own_line;
-    const TGKvGroupShape sp = shape_of(p, lp, p.old_len, p.tok0), so = shape_of(p, lo, p.old_len, p.tok0);
+    const TGKvGroupShape sp = shape_of(p, lp, nullptr, tok0), so = shape_of(p, lo, nullptr, tok0);
     const uint32_t t = row / p.n_heads, h = row % p.n_heads, kvh = h / G, sub = h % G;
-    const uint32_t i = seq_of(p, t), own = t - p.tok0[i];
+    const uint32_t i = seq_of(tok0, p.n_seq, t), own = t - tok0[i];
     Acc<HD> acc;
     acc.add(p, row, lane);
-    add_continued<HD>(p, lp, acc, TGKvGroupPos{0, kvh, t / sp.item_tokens, 0}, item_row(sp, t % sp.item_tokens, G, sub),
-                      lane);
+    add_continued<HD>(p, lp, starts[lp], acc, TGKvGroupPos{0, kvh, t / sp.item_tokens, 0},
+                      item_row(sp, t % sp.item_tokens, G, sub), lane);
     acc.add(p, (uint64_t)total + row, lane);
-    add_continued<HD>(p, lo, acc, TGKvGroupPos{i + 1, kvh, own / so.item_tokens, 0},
+    add_continued<HD>(p, lo, starts[lo], acc, TGKvGroupPos{i + 1, kvh, own / so.item_tokens, 0},
                       item_row(so, own % so.item_tokens, G, sub), lane);
     acc.template store<T>(p, row, lane);
 }
@@ -724,25 +775,30 @@ __global__ void __launch_bounds__(256) group_merge_parts_kernel(const __grid_con
 // query rows 16 y .. +15 of the item that CTA b leaves unfinished and began itself.
 template <typename T, int HD>
 __global__ void __launch_bounds__(256) group_merge_split_kernel(const __grid_constant__ TGKvGroupParams p) {
+    __shared__ Starts st;
+    const int line = p.own_line;
+    st.copy(p, line);
+    __syncthreads();
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const uint32_t b = blockIdx.x;
-    const int line = p.own_line;
-    const TGKvGroupPos s = start_of(p, line, b), e = start_of(p, line, b + 1);
+    const TGKvGroupPos s = st.at(b), e = st.at(b + 1);
     // the item that the next CTA continues, begun in this one
     if (e.seq > p.n_seq || e.tile == 0 || (tgkv_group_same_item(s, e) && s.tile > 0)) return;
     TGKvGroupPos it = e;
     it.tile = 0;
     const uint32_t G = p.n_heads / p.n_kv_heads;
-    const TGKvGroupShape sh = shape_of(p, line, p.old_len, p.tok0);
+    const uint32_t* tok0 = as_memory(p.tok0);
+    const TGKvGroupShape sh = shape_of(p, line, nullptr, tok0);
     const uint32_t t0 = it.at * sh.item_tokens, ntok = min(sh.item_tokens, tgkv_group_tokens(&sh, it.seq) - t0);
+    const uint32_t first = tok0[it.seq - 1] + t0;
     const int lane = threadIdx.x & 31;
     for (uint32_t x = blockIdx.y * 16 + (threadIdx.x >> 5); x < blockIdx.y * 16 + 16 && x < ntok * G; x += 8) {
         const uint32_t t = x / G, sub = x % G, r = item_row(sh, t, G, sub);
         Acc<HD> acc;
         acc.add(p, (uint64_t)p.line[line].cta_rows + slot_rows(line) * (2 * b + 1) + r, lane);
-        add_continued<HD>(p, line, acc, it, r, lane);
-        acc.template store<T>(p, (uint64_t)(p.tok0[it.seq - 1] + t0 + t) * p.n_heads + it.kvh * G + sub, lane);
+        add_continued<HD>(p, line, st, acc, it, r, lane);
+        acc.template store<T>(p, (uint64_t)(first + t) * p.n_heads + it.kvh * G + sub, lane);
     }
 }
 
@@ -750,21 +806,16 @@ template <typename T, int HD>
 int launch(const TGKvGroupParams* p, cudaStream_t st) {
     const uint32_t total = p->tok0[p->n_seq];
     static bool done[64];
-    cudaError_t e = allow_smem(group_kernel<T, HD>, Cfg<HD>::SMEM, done);
+    constexpr uint32_t smem = Cfg<HD>::SMEM > light::Cfg<T, HD>::SMEM ? Cfg<HD>::SMEM : light::Cfg<T, HD>::SMEM;
+    cudaError_t e = allow_smem(group_kernel<T, HD>, smem, done);
     if (e != cudaSuccess) return (int)e;
     if (p->k_new) {
         const uint64_t n = (uint64_t)total * (p->n_kv_heads * HD / 8);
         e = launch_pdl(group_append_kernel<T>, dim3((unsigned)((n + 255) / 256), 2), 256, 0, st, p);
         if (e != cudaSuccess) return (int)e;
     }
-    if (p->line[0].n_cta) {
-        e = launch_pdl(group_kernel<T, HD>, dim3(p->line[0].n_cta), kThreads, Cfg<HD>::SMEM, st, p);
-        if (e != cudaSuccess) return (int)e;
-    }
-    if (p->line[1].n_cta) {
-        const int r = tgkv_launch_group_light(p, sizeof(T) == 2, (void*)st);
-        if (r) return r;
-    }
+    e = launch_pdl(group_kernel<T, HD>, dim3(p->line[0].n_cta + p->line[1].n_cta), kThreads, smem, st, p);
+    if (e != cudaSuccess) return (int)e;
     const TGKvGroupLine* own = &p->line[p->own_line];
     if (p->share)
         e = launch_pdl(group_merge_parts_kernel<T, HD>, dim3((total * p->n_heads + 7) / 8), 256, 0, st, p);

@@ -1,5 +1,5 @@
-// tgkv_group.cuh -- device code shared by the kernels of tgkv_group.cu and
-// tgkv_group_light.cu: the pieces of a CTA's stretch (tgkv_group_plan.h), TMEM
+// tgkv_group.cuh -- device code shared by tgkv_group.cu and
+// tgkv_group_light.cuh: the pieces of a CTA's stretch (tgkv_group_plan.h), TMEM
 // access and the launch helper.
 #pragma once
 #include <cuda.h>
@@ -18,13 +18,26 @@ namespace group {
 constexpr int kRows = TGKV_GROUP_ROWS, kPos = TGKV_GROUP_TILE;
 constexpr uint32_t kBlock = 16384;              // 128 rows x 64 bf16: one swizzled box
 constexpr int kErrTimeout = 7;
+constexpr int kThreads = 384;
 
 __device__ __forceinline__ float lo_f(uint32_t x) { return __uint_as_float(x << 16); }
 __device__ __forceinline__ float hi_f(uint32_t x) { return __uint_as_float(x & 0xffff0000u); }
 
+// A table in the parameter block as ordinary memory.  Read as parameters, entries
+// would come through the constant cache one after another, each first touch a miss
+// that costs as much as a trip to L2 (25 us for a merge over 148 stretches); so the
+// threads of a block copy the tables they search into shared memory side by side.
+__device__ __forceinline__ const uint32_t* as_memory(const uint32_t* table) {
+    asm volatile("" : "+l"(table));
+    return table;
+}
+__device__ __forceinline__ void copy_table(uint32_t* dst, const uint32_t* table, uint32_t n, int tid, int threads) {
+    const uint32_t* src = as_memory(table);
+    for (uint32_t i = tid; i < n; i += threads) dst[i] = src[i];
+}
 __device__ __forceinline__ TGKvGroupPos start_of(const TGKvGroupParams& p, int line, uint32_t b) {
-    const uint32_t* s = p.line[line].start + 4 * b;
-    return TGKvGroupPos{s[0], s[1], s[2], s[3]};
+    const uint4 s = *reinterpret_cast<const uint4*>(as_memory(p.line[line].start) + 4 * b);
+    return TGKvGroupPos{s.x, s.y, s.z, s.w};
 }
 __device__ __forceinline__ TGKvGroupShape shape_of(const TGKvGroupParams& p, int line, const uint32_t* old_len,
                                                    const uint32_t* tok0) {
@@ -80,11 +93,11 @@ struct ItemRows {
 
 // The sequence of packed token t: the last one whose first token is at or
 // before t among those with tokens.
-__device__ __forceinline__ uint32_t seq_of(const TGKvGroupParams& p, uint32_t t) {
-    uint32_t lo = 0, hi = p.n_seq;
+__device__ __forceinline__ uint32_t seq_of(const uint32_t* tok0, uint32_t n_seq, uint32_t t) {
+    uint32_t lo = 0, hi = n_seq;
     while (hi - lo > 1) {
         const uint32_t mid = (lo + hi) >> 1;
-        if (p.tok0[mid] <= t) lo = mid;
+        if (tok0[mid] <= t) lo = mid;
         else hi = mid;
     }
     return lo;

@@ -1,6 +1,6 @@
-// tgkv_group_light.cu -- group attention (tgkv_group.cu) of items with few query
+// tgkv_group_light.cuh -- group attention (tgkv_group.cu) of items with few query
 // rows: a decode step's tokens over their own caches, up to 16 rows of one KV
-// head (10 with fp32 activations).
+// head (10 with fp32 activations).  The part of a CTA on line 1.
 //
 // The products go the other way round, S^T = K Q^T and O^T += V^T P^T, with the
 // rows as 16 or 32 columns: K and V tiles are the 128-row operands straight from
@@ -14,13 +14,13 @@
 // a tile; at the end head dim r), 8 TMA, 9 and 10 the streams' MMAs.
 // TMEM columns: S^T of stream h [64 h, +32), O^T [128 + 64 h, +32).
 // Every mbarrier wait is bounded, as in tgkv_group.cu.
+#pragma once
 #include "tgkv_group.cuh"
 
 namespace tgkv {
 namespace group {
 namespace light {
 
-constexpr int kThreads = 384;
 constexpr int kTmaWarp = 8, kMmaWarp = 9;
 constexpr uint32_t TM_S = 0, TM_O = 128, TM_COLS = 256;
 
@@ -82,12 +82,11 @@ __device__ __forceinline__ void tmem_st_cols(uint32_t addr, const uint32_t (&w)[
 __device__ __forceinline__ void tmem_st_cols(uint32_t addr, const uint32_t (&w)[16]) { tmem_st16(addr, w); }
 
 template <typename T, int HD>
-__global__ void __launch_bounds__(kThreads, 1) group_light_kernel(const __grid_constant__ TGKvGroupParams p) {
+__device__ __forceinline__ void run(const TGKvGroupParams& p, uint32_t cta_index, unsigned char* smem_raw) {
     using C = Cfg<T, HD>;
     constexpr int TERMS = C::TERMS, ROWS = C::ROWS, N = C::N;
     // fp32 sums: at most 16 tiles per accumulator (see tgkv_group.cu)
     constexpr uint32_t kMost = TERMS == 3 ? 32 : 0;
-    extern __shared__ unsigned char smem_raw[];
     unsigned char* base =
         reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     const uint32_t sbase = smem_addr(base);
@@ -97,10 +96,8 @@ __global__ void __launch_bounds__(kThreads, 1) group_light_kernel(const __grid_c
     uint32_t* old_len = tok0 + p.n_seq + 1;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
-    for (uint32_t i = tid; i <= p.n_seq; i += kThreads) {
-        tok0[i] = p.tok0[i];
-        if (i < p.n_seq) old_len[i] = p.old_len[i];
-    }
+    copy_table(tok0, p.tok0, p.n_seq + 1, tid, kThreads);
+    copy_table(old_len, p.old_len, p.n_seq, tid, kThreads);
     if (tid == 0) {
         for (int i = 0; i < C::kStages; ++i) {
             mbar_init(&bar[C::B_KFULL + i], 1);
@@ -131,7 +128,7 @@ __global__ void __launch_bounds__(kThreads, 1) group_light_kernel(const __grid_c
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
-    Pieces pc(sh, start_of(p, 1, blockIdx.x), start_of(p, 1, blockIdx.x + 1), kMost);
+    Pieces pc(sh, start_of(p, 1, cta_index), start_of(p, 1, cta_index + 1), kMost);
     if (warp == kTmaWarp) {
         if (lane == 0) {
             uint32_t n = 0, nv = 0;              // K and V tiles issued
@@ -249,56 +246,64 @@ __global__ void __launch_bounds__(kThreads, 1) group_light_kernel(const __grid_c
         const uint32_t total_rows = tok0[p.n_seq] * p.n_heads;
         uint32_t g0 = 0, it = 0, n = 0;          // K/V tiles of earlier pieces; pieces; this stream's steps
         bool ok = true;
-        // q of a piece, as TERMS bf16 rows each: two dims a thread, the streams take every other row
+        // q of a piece, as TERMS bf16 rows each: two dims a thread, the streams take every other
+        // row.  Loaded while the piece before is worked on, stored once that one's last S^T is made.
         constexpr int kMine = (ROWS + 1) / 2;
-        auto put_q = [&](const Pieces& a, uint32_t piece) {
+        float2 qv[kMine];
+        uint32_t q_rows = 0;
+        auto load_q = [&](const Pieces& a) {
+            if (!a.more()) return;
             const ItemRows ir(sh, a);
-            const uint32_t R = ir.tokens * G;
+            q_rows = ir.tokens * G;
             const uint64_t row0 = (uint64_t)((a.at.seq ? tok0[a.at.seq - 1] : 0) + a.at.at * sh.item_tokens) * p.n_heads +
                                   a.at.kvh * G;
-            float2 v[kMine];
-            if (r < HD / 2) {
+            if (r >= HD / 2) return;
 #pragma unroll
-                for (int i = 0; i < kMine; ++i) {
-                    const uint32_t x = 2 * i + h;
-                    if (x >= R) continue;
-                    const uint64_t e = (row0 + x / G * p.n_heads + x % G) * HD + 2 * r;
-                    if constexpr (TERMS == 3) v[i] = *reinterpret_cast<const float2*>(reinterpret_cast<const float*>(p.q) + e);
-                    else v[i].x = __uint_as_float(*reinterpret_cast<const uint32_t*>(reinterpret_cast<const uint16_t*>(p.q) + e));
-                }
+            for (int i = 0; i < kMine; ++i) {
+                const uint32_t x = 2 * i + h;
+                if (x >= q_rows) break;
+                const uint64_t e = (row0 + x / G * p.n_heads + x % G) * HD + 2 * r;
+                if constexpr (TERMS == 3) qv[i] = *reinterpret_cast<const float2*>(reinterpret_cast<const float*>(p.q) + e);
+                else qv[i].x = __uint_as_float(*reinterpret_cast<const uint32_t*>(reinterpret_cast<const uint16_t*>(p.q) + e));
             }
+        };
+        auto store_q = [&](uint32_t piece) {
             if (ok && piece > 0) ok = __all_sync(0xffffffffu, mbar_wait(&bar[C::B_QEMPTY], (piece - 1) & 1u));
             if (r < HD / 2) {
 #pragma unroll
                 for (int i = 0; i < kMine; ++i) {
                     const uint32_t x = 2 * i + h;
-                    if (x >= R) continue;
+                    if (x >= q_rows) break;
 #pragma unroll
                     for (int t = 0; t < TERMS; ++t) {
-                        const uint32_t w = TERMS == 3 ? cvt_bf16x2(v[i].x, v[i].y) : __float_as_uint(v[i].x);
+                        const uint32_t w = TERMS == 3 ? cvt_bf16x2(qv[i].x, qv[i].y) : __float_as_uint(qv[i].x);
                         const uint32_t c = t * ROWS + x;
                         *reinterpret_cast<uint32_t*>(base + C::OFF_Q + (r >> 5) * C::kSmall + c * 128 +
                                                      ((((uint32_t)r & 31u) >> 2) ^ (c & 7u)) * 16 + (r & 3) * 4) = w;
-                        v[i].x -= lo_f(w);
-                        v[i].y -= hi_f(w);
+                        qv[i].x -= lo_f(w);
+                        qv[i].y -= hi_f(w);
                     }
                 }
             }
             fence_proxy_async_smem();
             mbar_arrive(&bar[C::B_QFULL]);
         };
-        if (pc.more()) put_q(pc, 0);
+        load_q(pc);
+        if (pc.more()) store_q(0);
         while (pc.more()) {
             const ItemRows pr(sh, pc);
             const uint32_t seq = pc.at.seq, R = pr.tokens * G, t0 = pc.at.at * sh.item_tokens;
             const uint32_t own_min = seq ? old_len[seq - 1] + t0 + 1 : 0;                // rows that token 0 sees
             const uint64_t row0 = (uint64_t)((seq ? tok0[seq - 1] : 0) + t0) * p.n_heads + pc.at.kvh * G;
             const uint32_t steps = pc.j1 - pc.j0;
+            const Pieces cur = pc;
+            pc.next(sh, kMost);
+            load_q(pc);
             float m[ROWS], l[ROWS];              // of the scaled scores, log2 domain; l: this thread's positions
 #pragma unroll
             for (int x = 0; x < ROWS; ++x) { m[x] = -INFINITY; l[x] = 0.f; }
             for (uint32_t k = (uint32_t)h; k < steps; k += 2, ++n) {
-                const uint32_t j = pc.j0 + k, pos = pr.pos(j), rows = pr.rows(j) - pos;
+                const uint32_t j = cur.j0 + k, pos = pr.pos(j), rows = pr.rows(j) - pos;
                 const bool own = pr.own(j);
                 const int first = (int)((own ? own_min : p.prefix_len) - pos);           // of the tile, that token 0 sees
                 if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&bar[C::B_SFULL + h], n & 1u));
@@ -324,39 +329,39 @@ __global__ void __launch_bounds__(kThreads, 1) group_light_kernel(const __grid_c
                 }
                 int lim = first, sub = 0;        // positions that row x's token sees
 #pragma unroll
-                for (int x = 0; x < ROWS; ++x)
-                    if ((uint32_t)x < R) {
-                        float s = __uint_as_float(v[x]);
-                        if constexpr (TERMS == 3) s = (s + __uint_as_float(v[ROWS + x])) + __uint_as_float(v[2 * ROWS + x]);
-                        sc[x] = r < lim ? s * scale : -INFINITY;
-                        grow |= !(sc[x] <= m[x] + 8.f) && sc[x] != -INFINITY;
-                        if (own && ++sub == (int)G) { sub = 0; ++lim; }
-                    }
+                for (int x = 0; x < ROWS; ++x) {
+                    if ((uint32_t)x >= R) break;
+                    float s = __uint_as_float(v[x]);
+                    if constexpr (TERMS == 3) s = (s + __uint_as_float(v[ROWS + x])) + __uint_as_float(v[2 * ROWS + x]);
+                    sc[x] = r < lim ? s * scale : -INFINITY;
+                    grow |= !(sc[x] <= m[x] + 8.f) && sc[x] != -INFINITY;
+                    if (own && ++sub == (int)G) { sub = 0; ++lim; }
+                }
                 // the running maxima move only when one is exceeded by more than 2^8 (or NaN)
                 if (stream_any(h, grow)) {
 #pragma unroll
-                    for (int x = 0; x < ROWS; ++x)
-                        if ((uint32_t)x < R) {
-                            float a = sc[x];
+                    for (int x = 0; x < ROWS; ++x) {
+                        if ((uint32_t)x >= R) break;
+                        float a = sc[x];
 #pragma unroll
-                            for (int o = 16; o >= 1; o >>= 1) a = max3(a, __shfl_xor_sync(0xffffffffu, a, o), a);
-                            if (lane == 0) red[quarter * 16 + x] = a;
-                        }
+                        for (int o = 16; o >= 1; o >>= 1) a = max3(a, __shfl_xor_sync(0xffffffffu, a, o), a);
+                        if (lane == 0) red[quarter * 16 + x] = a;
+                    }
                     stream_sync(h);
                     uint32_t ov[N];
                     const bool scale_o = k > 1;  // O^T holds the stream's earlier tiles, all complete before this S^T
                     if (ok && scale_o) tmem_ld_cols(to + (uint32_t)h * 64u, ov);
 #pragma unroll
-                    for (int x = 0; x < ROWS; ++x)
-                        if ((uint32_t)x < R) {
-                            const float a = max3(max3(red[x], red[16 + x], red[32 + x]), red[48 + x], m[x]);
-                            const float alpha = m[x] == -INFINITY ? 0.f : ex2_approx(m[x] - a);
-                            m[x] = a;
-                            l[x] *= alpha;
+                    for (int x = 0; x < ROWS; ++x) {
+                        if ((uint32_t)x >= R) break;
+                        const float a = max3(max3(red[x], red[16 + x], red[32 + x]), red[48 + x], m[x]);
+                        const float alpha = m[x] == -INFINITY ? 0.f : ex2_approx(m[x] - a);
+                        m[x] = a;
+                        l[x] *= alpha;
 #pragma unroll
-                            for (int t = 0; t < TERMS; ++t)
-                                ov[t * ROWS + x] = __float_as_uint(__uint_as_float(ov[t * ROWS + x]) * alpha);
-                        }
+                        for (int t = 0; t < TERMS; ++t)
+                            ov[t * ROWS + x] = __float_as_uint(__uint_as_float(ov[t * ROWS + x]) * alpha);
+                    }
                     if (ok && scale_o) {
                         tmem_st_cols(to + (uint32_t)h * 64u, ov);
                         tmem_wait_st();
@@ -367,57 +372,56 @@ __global__ void __launch_bounds__(kThreads, 1) group_light_kernel(const __grid_c
                     const uint32_t pb = sbase + C::OFF_P + ((uint32_t)h * 2 + ((uint32_t)r >> 6)) * C::kSmall;
                     const uint32_t c = ((uint32_t)r & 63u) >> 3, e = ((uint32_t)r & 7u) * 2u;
 #pragma unroll
-                    for (int x = 0; x < ROWS; ++x)
-                        if ((uint32_t)x < R) {
-                            float w = m[x] == -INFINITY ? 0.f : ex2_approx(sc[x] - m[x]);
-                            l[x] += w;
+                    for (int x = 0; x < ROWS; ++x) {
+                        if ((uint32_t)x >= R) break;
+                        float w = m[x] == -INFINITY ? 0.f : ex2_approx(sc[x] - m[x]);
+                        l[x] += w;
 #pragma unroll
-                            for (int t = 0; t < TERMS; ++t) {
-                                const uint32_t b = cvt_bf16x2(w, 0.f) & 0xffffu, q = t * ROWS + x;
-                                asm volatile("st.shared.u16 [%0], %1;" ::"r"(pb + q * 128u + ((c ^ (q & 7u)) << 4) + e),
-                                             "h"((uint16_t)b) : "memory");
-                                w -= lo_f(b);
-                            }
+                        for (int t = 0; t < TERMS; ++t) {
+                            const uint32_t b = cvt_bf16x2(w, 0.f) & 0xffffu, q = t * ROWS + x;
+                            asm volatile("st.shared.u16 [%0], %1;" ::"r"(pb + q * 128u + ((c ^ (q & 7u)) << 4) + e),
+                                         "h"((uint16_t)b) : "memory");
+                            w -= lo_f(b);
                         }
+                    }
                 }
                 fence_proxy_async_smem();
                 tc_fence_before();
                 mbar_arrive(&bar[C::B_PFULL + h]);
             }
             g0 += steps;
-            const Pieces cur = pc;
-            pc.next(sh, kMost);
             ++it;
-            if (pc.more()) put_q(pc, it);        // the next piece's first scores are made meanwhile
+            if (pc.more()) store_q(it);          // the next piece's first scores are made meanwhile
 
             // ---- the rows' sums, over the stream's threads, then both streams
             if (ok && (uint32_t)h < steps) ok = __all_sync(0xffffffffu, mbar_wait(&bar[C::B_PVDONE + h], (n - 1) & 1u));
 #pragma unroll
-            for (int x = 0; x < ROWS; ++x)
-                if ((uint32_t)x < R) {
-                    float a = l[x];
+            for (int x = 0; x < ROWS; ++x) {
+                if ((uint32_t)x >= R) break;
+                float a = l[x];
 #pragma unroll
-                    for (int o = 16; o >= 1; o >>= 1) a += __shfl_xor_sync(0xffffffffu, a, o);
-                    if (lane == 0) {
-                        red[quarter * 16 + x] = a;
-                        if (quarter == 0) maxima[h * 16 + x] = m[x];
-                    }
+                for (int o = 16; o >= 1; o >>= 1) a += __shfl_xor_sync(0xffffffffu, a, o);
+                if (lane == 0) {
+                    red[quarter * 16 + x] = a;
+                    if (quarter == 0) maxima[h * 16 + x] = m[x];
                 }
+            }
             tc_fence_before();
             streams_sync();
             tc_fence_after();
             const bool whole = cur.first == 0 && cur.j1 == cur.nt && !p.share;
             const bool again = TERMS == 3 && cur.j0 > cur.first;                         // adds to the item's earlier piece here
             const uint64_t cta = (uint64_t)p.line[1].cta_rows +
-                                 TGKV_GROUP_LIGHT_ROWS * (2u * blockIdx.x + (cur.first > 0 ? 0u : 1u));
+                                 TGKV_GROUP_LIGHT_ROWS * (2u * cta_index + (cur.first > 0 ? 0u : 1u));
             uint32_t oa[N], ob[N];
             if (ok) {
                 tmem_ld_cols(to, oa);
                 tmem_ld_cols(to + 64, ob);
             }
 #pragma unroll
-            for (int x = 0; x < ROWS; ++x)
-                if ((uint32_t)x < R && ok && r < HD && (x & 1) == h) {
+            for (int x = 0; x < ROWS; ++x) {
+                if ((uint32_t)x >= R) break;
+                if (ok && r < HD && (x & 1) == h) {
                     const float ma = maxima[x], mb = maxima[16 + x];
                     float M = max3(ma, mb, ma);
                     const float wa = ma == -INFINITY ? 0.f : ex2_approx(ma - M), wb = mb == -INFINITY ? 0.f : ex2_approx(mb - M);
@@ -446,6 +450,7 @@ __global__ void __launch_bounds__(kThreads, 1) group_light_kernel(const __grid_c
                     joint[x] = M;                // the same from every thread of the row
                     joint[16 + x] = L;
                 }
+            }
             tc_fence_before();
             streams_sync();                      // O^T, the sums and the slots' (m, l) have been read
             if (!whole && ok && (uint32_t)r < R && (r & 1) == h) {
@@ -464,23 +469,6 @@ __global__ void __launch_bounds__(kThreads, 1) group_light_kernel(const __grid_c
     }
 }
 
-template <typename T, int HD>
-int launch(const TGKvGroupParams* p, cudaStream_t st) {
-    using C = Cfg<T, HD>;
-    static bool done[64];
-    cudaError_t e = allow_smem(group_light_kernel<T, HD>, C::SMEM, done);
-    if (e != cudaSuccess) return (int)e;
-    return (int)launch_pdl(group_light_kernel<T, HD>, dim3(p->line[1].n_cta), kThreads, C::SMEM, st, p);
-}
-
 }  // namespace light
 }  // namespace group
 }  // namespace tgkv
-
-extern "C" int tgkv_launch_group_light(const TGKvGroupParams* p, int act, void* stream) {
-    using namespace tgkv::group::light;
-    cudaStream_t st = (cudaStream_t)stream;
-    if (p->head_dim == 128) return act ? launch<uint16_t, 128>(p, st) : launch<float, 128>(p, st);
-    if (p->head_dim == 64) return act ? launch<uint16_t, 64>(p, st) : launch<float, 64>(p, st);
-    return (int)cudaErrorInvalidValue;
-}

@@ -20,7 +20,7 @@
  * an item and only its last piece can leave one unfinished, so partial results
  * need two slots of an item's rows per CTA (and, split, one row per query row
  * and part).
- * Line 0 holds the items of tgkv_group.cu, line 1 those of tgkv_group_light.cu:
+ * Line 0 holds the items of tgkv_group.cu, line 1 those of tgkv_group_light.cuh:
  * the sequences' own items when none of them has more than the light rows (most
  * decode steps), and with them the prefix's when all tokens together are that
  * few.

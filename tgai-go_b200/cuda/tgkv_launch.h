@@ -208,7 +208,8 @@ typedef struct {
                                   * cta_rows + 2 S b on, S for the item it continues, then S for
                                   * the one it leaves unfinished; S = 256 on line 0,
                                   * TGKV_GROUP_LIGHT_ROWS on line 1 */
-    uint32_t start[(TGKV_GROUP_MAX_CTAS + 1) * 4];  /* TGKvGroupPos of each CTA, and the end */
+    uint32_t start[(TGKV_GROUP_MAX_CTAS + 1) * 4];  /* TGKvGroupPos of each CTA, and the end
+                                                     * (16-byte aligned in TGKvGroupParams) */
 } TGKvGroupLine;
 #define TGKV_GROUP_LIGHT_ROWS 16 /* query rows of a light item at most */
 
@@ -241,8 +242,7 @@ typedef struct {
 } TGKvGroupParams;
 int tgkv_launch_fork(const TGKvForkParams* p, void* stream);
 int tgkv_launch_compact(const TGKvCompactParams* p, uint32_t cluster, void* stream);
-/* act: 0 fp32, 1 bf16 activations; the second: line 1 alone */
-int tgkv_launch_group_light(const TGKvGroupParams* p, int act, void* stream);
+/* act: 0 fp32, 1 bf16 activations */
 int tgkv_launch_group(const TGKvGroupParams* p, int act, void* stream);
 
 /* Launchers (tgkv_kernels.cu, tgkv_prefill.cu, tgkv_prefill_f32.cu).  Return 0
