@@ -1179,12 +1179,12 @@ static int plan_group(const TGCudaGroupCall* c, uint32_t sms, TGKvGroupParams* p
     else if (all_light) plan_line(&light, 0, c->n_seq, sms, &p->line[1]);
     else {
         /* both lines at once, each on the SMs its work takes: a tile of line 0 about
-         * 1.2 us (2.3 us for two row tiles), one of line 1 1 us and an item 2 us more */
+         * 2 us (2.4 us for two row tiles), one of line 1 1.2 us and an item 2 us more */
         uint64_t w0 = 0, w1 = 0;
         const uint64_t pre = tgkv_group_prefix_tiles(&heavy, 0), items = tgkv_group_items(&heavy, 0);
-        w0 = pre * items * (total > tpt && c->act == 1 ? 23 : 12);
+        w0 = pre * items * (total > tpt && c->act == 1 ? 24 : 20);
         for (uint32_t i = 1; i <= c->n_seq; i++)
-            if (c->n_new[i - 1]) w1 += 20 + 10ull * tgkv_group_item_tiles(&light, i, 0);
+            if (c->n_new[i - 1]) w1 += 20 + 12ull * tgkv_group_item_tiles(&light, i, 0);
         if (sms == 0 || sms > TGKV_GROUP_MAX_CTAS) sms = TGKV_GROUP_MAX_CTAS;
         uint32_t n0 = (uint32_t)((sms * w0 + (w0 + w1) / 2) / (w0 + w1));
         if (n0 < 1) n0 = 1;

@@ -636,27 +636,36 @@ __global__ void __launch_bounds__(kThreads, 1) group_kernel(const __grid_constan
 
 // ------------------------------------------------------------------ merge
 // A row's result from its partials (o, m, l): sum 2^(m - M) o / sum 2^(m - M) l.
-// One warp per query row, HD / 32 dims per lane.  Lane i keeps partial i's (m, l)
-// and, up to 32 at a time, all partials' rows are in flight at once: the kernel's
-// time is a few memory latencies.
+// One warp per query row, HD / 32 dims per lane.  Lane i keeps partial i's place and
+// (m, l), and up to 32 partials' rows are in flight at once.  What it takes is a few
+// memory latencies, so the places are worked out, and the parameters read, before
+// the wait for the partials.
 template <int HD>
 struct Acc {
     static constexpr int D = HD / 32;
+    const float *part_o, *part_ml;
     float o[D], m, l;
-    uint32_t n;                                  // partials noted
+    uint32_t n, all;                             // partials noted; in all
     uint64_t slot;                               // lane i: partial i's row
-    __device__ Acc() : m(-INFINITY), l(0.f), n(0), slot(0) {
+    bool ready;                                  // the partials may be read
+    __device__ Acc(const TGKvGroupParams& p)
+        : part_o(p.part_o), part_ml(p.part_ml), m(-INFINITY), l(0.f), n(0), all(0), slot(0), ready(false) {
+        asm volatile("" : "+l"(part_o), "+l"(part_ml));
 #pragma unroll
         for (int d = 0; d < D; ++d) o[d] = 0.f;
     }
-    // Notes a partial row.
-    __device__ void add(const TGKvGroupParams& p, uint64_t s, int lane) {
+    // Notes a partial row (before the partials may be read, the first 32).
+    __device__ void add(uint64_t s, int lane) {
+        ++all;
+        if (n == 32) {
+            if (!ready) return;
+            flush(lane);
+        }
         if (lane == (int)n) slot = s;
-        if (++n == 32) flush(p, lane);
+        ++n;
     }
-    __device__ void flush(const TGKvGroupParams& p, int lane) {
-        const float2 ml = lane < (int)n ? *reinterpret_cast<const float2*>(p.part_ml + slot * 2)
-                                        : make_float2(-INFINITY, 0.f);
+    __device__ void flush(int lane) {
+        const float2 ml = lane < (int)n ? *reinterpret_cast<const float2*>(part_ml + slot * 2) : make_float2(-INFINITY, 0.f);
         float M = ml.x;
 #pragma unroll
         for (int w = 16; w >= 1; w >>= 1) M = max3(M, __shfl_xor_sync(0xffffffffu, M, w), m);
@@ -668,11 +677,11 @@ struct Acc {
         l = l * a + L;
 #pragma unroll
         for (int d = 0; d < D; ++d) o[d] *= a;
-#pragma unroll 8
+#pragma unroll 4
         for (uint32_t i = 0; i < n; ++i) {
             const uint64_t s = __shfl_sync(0xffffffffu, slot, i);
             const float wi = __shfl_sync(0xffffffffu, w, i);
-            const float* src = p.part_o + s * HD + lane * D;
+            const float* src = part_o + s * HD + lane * D;
             if constexpr (D == 4) {
                 const float4 v = *reinterpret_cast<const float4*>(src);
                 o[0] += wi == 0.f ? 0.f : wi * v.x;
@@ -688,11 +697,22 @@ struct Acc {
         m = M;
         n = 0;
     }
+    // The sums over the partials that `note` notes; `wait` waits for them.
+    template <typename Note>
+    __device__ void run(Note note, int lane) {
+        note();
+        asm volatile("griddepcontrol.wait;" ::: "memory");
+        ready = true;
+        if (all > 32) {
+            n = 0;
+            note();
+        }
+        if (n) flush(lane);
+    }
     template <typename T>
-    __device__ void store(const TGKvGroupParams& p, uint64_t row, int lane) {
-        if (n) flush(p, lane);
+    __device__ void store(T* out, uint64_t row, int lane) const {
         const float inv = 1.f / l;
-        T* dst = reinterpret_cast<T*>(p.out) + row * HD + lane * D;
+        T* dst = out + row * HD + lane * D;
         if constexpr (sizeof(T) == 4) {
 #pragma unroll
             for (int d = 0; d < D; d += 2) *reinterpret_cast<float2*>(dst + d) = make_float2(o[d] * inv, o[d + 1] * inv);
@@ -733,7 +753,7 @@ __device__ __forceinline__ void add_continued(const TGKvGroupParams& p, int line
         if (!tgkv_group_same_item(s, it)) break;
         const TGKvGroupPos e = st.at(b + 1);
         if (tgkv_group_same_item(s, e) && s.tile == e.tile) continue;            // an empty stretch
-        acc.add(p, (uint64_t)p.line[line].cta_rows + 2u * slot_rows(line) * b + r, lane);
+        acc.add((uint64_t)p.line[line].cta_rows + 2u * slot_rows(line) * b + r, lane);
     }
 }
 
@@ -753,7 +773,6 @@ __global__ void __launch_bounds__(256) group_merge_parts_kernel(const __grid_con
     if (lo != lp) starts[lo].copy(p, lo);
     __syncthreads();
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    asm volatile("griddepcontrol.wait;" ::: "memory");
     const uint32_t row = blockIdx.x * 8 + (threadIdx.x >> 5), total = tok0[p.n_seq] * p.n_heads;
     const int lane = threadIdx.x & 31;
     if (row >= total) return;
@@ -761,14 +780,18 @@ __global__ void __launch_bounds__(256) group_merge_parts_kernel(const __grid_con
     const TGKvGroupShape sp = shape_of(p, lp, nullptr, tok0), so = shape_of(p, lo, nullptr, tok0);
     const uint32_t t = row / p.n_heads, h = row % p.n_heads, kvh = h / G, sub = h % G;
     const uint32_t i = seq_of(tok0, p.n_seq, t), own = t - tok0[i];
-    Acc<HD> acc;
-    acc.add(p, row, lane);
-    add_continued<HD>(p, lp, starts[lp], acc, TGKvGroupPos{0, kvh, t / sp.item_tokens, 0},
-                      item_row(sp, t % sp.item_tokens, G, sub), lane);
-    acc.add(p, (uint64_t)total + row, lane);
-    add_continued<HD>(p, lo, starts[lo], acc, TGKvGroupPos{i + 1, kvh, own / so.item_tokens, 0},
-                      item_row(so, own % so.item_tokens, G, sub), lane);
-    acc.template store<T>(p, row, lane);
+    T* out = reinterpret_cast<T*>(p.out);
+    asm volatile("" : "+l"(out));
+    Acc<HD> acc(p);
+    acc.run([&] {
+        acc.add(row, lane);
+        add_continued<HD>(p, lp, starts[lp], acc, TGKvGroupPos{0, kvh, t / sp.item_tokens, 0},
+                          item_row(sp, t % sp.item_tokens, G, sub), lane);
+        acc.add((uint64_t)total + row, lane);
+        add_continued<HD>(p, lo, starts[lo], acc, TGKvGroupPos{i + 1, kvh, own / so.item_tokens, 0},
+                          item_row(so, own % so.item_tokens, G, sub), lane);
+    }, lane);
+    acc.template store<T>(out, row, lane);
 }
 
 // joined: the rows of items that several CTAs worked on.  Block (b, y) merges
@@ -780,7 +803,6 @@ __global__ void __launch_bounds__(256) group_merge_split_kernel(const __grid_con
     st.copy(p, line);
     __syncthreads();
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    asm volatile("griddepcontrol.wait;" ::: "memory");
     const uint32_t b = blockIdx.x;
     const TGKvGroupPos s = st.at(b), e = st.at(b + 1);
     // the item that the next CTA continues, begun in this one
@@ -795,10 +817,12 @@ __global__ void __launch_bounds__(256) group_merge_split_kernel(const __grid_con
     const int lane = threadIdx.x & 31;
     for (uint32_t x = blockIdx.y * 16 + (threadIdx.x >> 5); x < blockIdx.y * 16 + 16 && x < ntok * G; x += 8) {
         const uint32_t t = x / G, sub = x % G, r = item_row(sh, t, G, sub);
-        Acc<HD> acc;
-        acc.add(p, (uint64_t)p.line[line].cta_rows + slot_rows(line) * (2 * b + 1) + r, lane);
-        add_continued<HD>(p, line, st, acc, it, r, lane);
-        acc.template store<T>(p, (uint64_t)(first + t) * p.n_heads + it.kvh * G + sub, lane);
+        Acc<HD> acc(p);
+        acc.run([&] {
+            acc.add((uint64_t)p.line[line].cta_rows + slot_rows(line) * (2 * b + 1) + r, lane);
+            add_continued<HD>(p, line, st, acc, it, r, lane);
+        }, lane);
+        acc.template store<T>(reinterpret_cast<T*>(p.out), (uint64_t)(first + t) * p.n_heads + it.kvh * G + sub, lane);
     }
 }
 

@@ -413,10 +413,19 @@ __device__ __forceinline__ void run(const TGKvGroupParams& p, uint32_t cta_index
             const bool again = TERMS == 3 && cur.j0 > cur.first;                         // adds to the item's earlier piece here
             const uint64_t cta = (uint64_t)p.line[1].cta_rows +
                                  TGKV_GROUP_LIGHT_ROWS * (2u * cta_index + (cur.first > 0 ? 0u : 1u));
-            uint32_t oa[N], ob[N];
-            if (ok) {
-                tmem_ld_cols(to, oa);
-                tmem_ld_cols(to + 64, ob);
+            uint32_t v[N];
+            float oa[ROWS], ob[ROWS];            // the streams' sums, over the terms
+            if (ok) tmem_ld_cols(to, v);
+#pragma unroll
+            for (int x = 0; x < ROWS; ++x) {
+                oa[x] = __uint_as_float(v[x]);
+                if constexpr (TERMS == 3) oa[x] = (oa[x] + __uint_as_float(v[ROWS + x])) + __uint_as_float(v[2 * ROWS + x]);
+            }
+            if (ok) tmem_ld_cols(to + 64, v);
+#pragma unroll
+            for (int x = 0; x < ROWS; ++x) {
+                ob[x] = __uint_as_float(v[x]);
+                if constexpr (TERMS == 3) ob[x] = (ob[x] + __uint_as_float(v[ROWS + x])) + __uint_as_float(v[2 * ROWS + x]);
             }
 #pragma unroll
             for (int x = 0; x < ROWS; ++x) {
@@ -427,13 +436,8 @@ __device__ __forceinline__ void run(const TGKvGroupParams& p, uint32_t cta_index
                     const float wa = ma == -INFINITY ? 0.f : ex2_approx(ma - M), wb = mb == -INFINITY ? 0.f : ex2_approx(mb - M);
                     const float* ra = red_all + x;
                     float L = wa * ((ra[0] + ra[16]) + (ra[32] + ra[48])) + wb * ((ra[64] + ra[80]) + (ra[96] + ra[112]));
-                    float a = __uint_as_float(oa[x]), b = __uint_as_float(ob[x]);
-                    if constexpr (TERMS == 3) {
-                        a = (a + __uint_as_float(oa[ROWS + x])) + __uint_as_float(oa[2 * ROWS + x]);
-                        b = (b + __uint_as_float(ob[ROWS + x])) + __uint_as_float(ob[2 * ROWS + x]);
-                    }
                     // (a stream that had no tile left O^T as it was)
-                    float o = (wa == 0.f ? 0.f : a * wa) + (wb == 0.f ? 0.f : b * wb);
+                    float o = (wa == 0.f ? 0.f : oa[x] * wa) + (wb == 0.f ? 0.f : ob[x] * wb);
                     const uint64_t row = row0 + x / (int)G * p.n_heads + x % (int)G;
                     const uint64_t slot = cur.first > 0 || !p.share ? cta + x : (seq ? total_rows : 0u) + row;
                     if (again) {
