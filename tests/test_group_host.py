@@ -167,6 +167,7 @@ def test_plan_covers_the_lines(lib, old, new, prefix, nh, nkv, share, sms, act):
         assert cuts[0] == 0 and all(a <= b for a, b in zip(cuts, cuts[1:]))
         n_cta = len(st) - 1
         assert n_cta <= min(len(tiles), sms or 160)
+        cost = 4 if st is starts[1] else 1 if act else 5         # of an item beside its tiles
         items = len({t[:3] for t in tiles})
-        most = max(b - a + len({t[:3] for t in tiles[a:b]}) for a, b in zip(cuts, cuts[1:]))
-        assert most <= (len(tiles) + items) / n_cta + 3
+        most = max(b - a + cost * len({t[:3] for t in tiles[a:b]}) for a, b in zip(cuts, cuts[1:]))
+        assert most <= (len(tiles) + cost * items) / n_cta + 2 * cost + 1

@@ -960,15 +960,16 @@ int tg_cuda_kv_fork_rows(const TGCudaRowCache* src, uint32_t n_src, const TGCuda
     return 1;
 }
 
-/* Column slices and CTAs per cluster of a compaction: a cluster serialises its
- * slice's waves, so the slices are what runs in parallel.  Rows are cut (down
- * to 256 bytes, two DRAM bursts of a row) until there are two CTAs of a
- * cluster of 8 per SM; clusters shrink when a slice's rows fit fewer CTAs. */
+/* Column slices and CTAs per cluster of a compaction.  A slice is at most 4 KB
+ * of a row (256 threads of 16 bytes) and, while a row's slices stay at 256
+ * bytes (four DRAM bursts), there are enough of them that the clusters make
+ * several rounds of the SMs (two CTAs each): what the last round leaves idle
+ * counts little.  Clusters of 8 shrink when a slice's rows fit fewer CTAs. */
 static void compact_shape(uint32_t n, uint64_t row_bytes, uint32_t n_move, uint32_t sms,
                           uint32_t* n_slices, uint32_t* cluster) {
-    uint32_t s = 1;
-    while ((uint64_t)n * 2 * s * 8 < 2ull * sms && row_bytes % (2 * s * 256) == 0) s *= 2;
-    const uint64_t bytes = (uint64_t)n_move * (row_bytes / s);
+    uint32_t s = (uint32_t)((row_bytes + 4095) / 4096);
+    while ((uint64_t)n * 2 * s * 8 < 16ull * sms && row_bytes >= 512ull * s) s *= 2;
+    const uint64_t bytes = (uint64_t)n_move * ((row_bytes + s - 1) / s);
     uint32_t c = 8;
     while (c > 1 && bytes <= (uint64_t)(c / 2) * 256 * 8 * 16) c /= 2;
     *n_slices = s;
@@ -1082,7 +1083,7 @@ static void plan_line(const TGKvGroupShape* sh, uint32_t first, uint32_t last, u
         uint64_t tiles = 0;
         for (uint32_t at = 0; at < n; at++) tiles += tgkv_group_item_tiles(sh, s, at);
         units += tiles * sh->n_kv_heads;
-        cost += (tiles + (uint64_t)n * TGKV_GROUP_ITEM_COST) * sh->n_kv_heads;
+        cost += (tiles + (uint64_t)n * sh->item_cost) * sh->n_kv_heads;
     }
     if (units == 0) return;
     uint32_t n_cta = sms && sms < TGKV_GROUP_MAX_CTAS ? sms : TGKV_GROUP_MAX_CTAS;
@@ -1095,17 +1096,17 @@ static void plan_line(const TGKvGroupShape* sh, uint32_t first, uint32_t last, u
         const uint32_t n = tgkv_group_items(sh, s);
         uint64_t head = 0;                          /* cost of one KV head's items of s */
         for (uint32_t at = 0; at < n; at++)
-            head += tgkv_group_item_tiles(sh, s, at) + TGKV_GROUP_ITEM_COST;
+            head += tgkv_group_item_tiles(sh, s, at) + sh->item_cost;
         for (uint32_t kvh = 0; kvh < sh->n_kv_heads; kvh++) {
             if (b >= n_cta || (uint64_t)b * cost / n_cta >= done + head) { done += head; continue; }
             for (uint32_t at = 0; at < n; at++) {
-                const uint64_t end = done + tgkv_group_item_tiles(sh, s, at) + TGKV_GROUP_ITEM_COST;
+                const uint64_t end = done + tgkv_group_item_tiles(sh, s, at) + sh->item_cost;
                 for (; b < n_cta && (uint64_t)b * cost / n_cta < end; b++) {
                     const uint64_t off = (uint64_t)b * cost / n_cta - done;
                     start[b].seq = s;
                     start[b].kvh = kvh;
                     start[b].at = at;
-                    start[b].tile = off > TGKV_GROUP_ITEM_COST ? (uint32_t)(off - TGKV_GROUP_ITEM_COST) : 0;
+                    start[b].tile = off > sh->item_cost ? (uint32_t)(off - sh->item_cost) : 0;
                     if (start[b].tile) ln->n_split++;
                 }
                 done = end;
@@ -1158,8 +1159,12 @@ static int plan_group(const TGCudaGroupCall* c, uint32_t sms, TGKvGroupParams* p
      * activations.) */
     const uint32_t light_tokens = (c->act == 1 ? TGKV_GROUP_LIGHT_ROWS : 10u) / g;
     const int own_light = longest <= light_tokens;
+    /* An item's start and end take as long as this many of its tiles (measured at
+     * 1, 2, 3 and 5: 31 prompts of up to 1000 tokens 200, 202, 207, 214 us with bf16
+     * activations, 531, 478, 450, 442 us with fp32 ones; decode over 64 caches of
+     * 1000-4000 positions 114, 114, 113, 112 us and 131, 125, 123, 120 us). */
     TGKvGroupShape heavy = {p->n_seq, p->n_kv_heads, p->prefix_len, 0, tpt, c->act == 1 ? 2 * tpt : tpt,
-                            p->old_len, p->tok0};
+                            c->act == 1 ? 1 : 5, p->old_len, p->tok0};
     /* Split when items over all sequences' tokens need at most 3/4 of the prefix
      * passes that the sequences' own items make. */
     uint64_t own_items = seqs;
@@ -1172,6 +1177,7 @@ static int plan_group(const TGCudaGroupCall* c, uint32_t sms, TGKvGroupParams* p
         p->share = heavy.share = 1;
     TGKvGroupShape light = heavy;
     light.item_tokens = light_tokens;
+    light.item_cost = 4;
     const int all_light = own_light && (!p->share || total <= light_tokens);
     p->own_line = own_light;
     p->prefix_line = all_light;

@@ -42,7 +42,7 @@ __device__ __forceinline__ TGKvGroupPos start_of(const TGKvGroupParams& p, int l
 __device__ __forceinline__ TGKvGroupShape shape_of(const TGKvGroupParams& p, int line, const uint32_t* old_len,
                                                    const uint32_t* tok0) {
     return TGKvGroupShape{p.n_seq, p.n_kv_heads, p.prefix_len, p.share, kRows / (p.n_heads / p.n_kv_heads),
-                          p.line[line].item_tokens, old_len, tok0};
+                          p.line[line].item_tokens, 0, old_len, tok0};
 }
 
 // The pieces of a CTA's stretch, one after another.  With `most` > 0 an item's

@@ -15,7 +15,7 @@
  *           cache.
  * Items in order (sequence, KV head, place in the sequence) form a line of
  * tiles, which is cut into n_cta contiguous stretches of about the same cost
- * (tiles plus TGKV_GROUP_ITEM_COST per item).  A CTA's stretch is a run of
+ * (tiles plus item_cost per item).  A CTA's stretch is a run of
  * pieces: parts of an item's tiles.  Only a stretch's first piece can continue
  * an item and only its last piece can leave one unfinished, so partial results
  * need two slots of an item's rows per CTA (and, split, one row per query row
@@ -39,13 +39,13 @@
 
 #define TGKV_GROUP_ROWS 128
 #define TGKV_GROUP_TILE 128
-#define TGKV_GROUP_ITEM_COST 1
 
 /* What the cut depends on. */
 typedef struct {
     uint32_t n_seq, n_kv_heads, prefix_len, share;
     uint32_t tpt;                /* tokens of a row tile: 128 / G */
     uint32_t item_tokens;        /* tokens of an item */
+    uint32_t item_cost;          /* of an item beside its tiles, in tiles */
     const uint32_t* old_len;     /* [n_seq] */
     const uint32_t* tok0;        /* [n_seq + 1] */
 } TGKvGroupShape;

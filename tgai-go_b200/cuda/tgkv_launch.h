@@ -189,7 +189,7 @@ typedef struct {
 
 /* In-place compaction of n_caches caches: destination row first[r] + j takes
  * row start[r] + j; the first `skip` rows stay where they are.  A cluster per
- * (cache, half, column slice); row_bytes / 16 is a multiple of n_slices. */
+ * (cache, half, column slice of at most 4 KB). */
 typedef struct {
     uint64_t row_bytes;
     uint32_t n_caches, n_slices, n_ranges, n_keep, skip, pad;

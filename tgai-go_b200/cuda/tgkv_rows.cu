@@ -41,68 +41,77 @@ __global__ void __launch_bounds__(kThreads) fork_kernel(const __grid_constant__ 
 // Destination row d takes source row s(d) >= d, s strictly increasing.  In
 // place, a row must have been read before the row that lands on it is
 // written.  One cluster owns a column slice of one half (K or V) of one cache
-// and walks the destination rows in waves of W rows: its CTAs read the
-// wave's sources into registers, meet at a cluster barrier, then write.  The
-// reads of wave w + 1 need no order against the writes of waves <= w: their
-// sources lie at or behind wave w + 1's own destinations.  So one barrier per
-// wave (every CTA's reads of wave w before any CTA's writes of wave w), with
-// the next wave's reads in flight across it, and no flags or scratch in
-// memory.  Bound: HBM, 2 * moved bytes.
-constexpr int kMoveVec = 8;
+// and walks the destination rows in waves: its CTAs read the wave's sources into
+// registers, meet at a cluster barrier, then write.  The reads of wave w + 1
+// need no order against the writes of waves <= w: their sources lie at or behind
+// wave w + 1's own destinations.  So one barrier per wave (every CTA's reads of
+// wave w before any CTA's writes of wave w), with the next wave's reads in
+// flight across it, and no flags or scratch in memory.  Bound: HBM, 2 * moved
+// bytes.  A thread keeps its column and steps through rows, so that there is no
+// division and its place among the ranges only moves on.
+constexpr int kMoveRows = 8;                      // rows in flight per thread
 
-__device__ __forceinline__ uint64_t source_row(const TGKvCompactParams& p, uint32_t d) {
-    uint32_t lo = 0, hi = p.n_ranges;             // the last range starting at or before d
-    while (hi - lo > 1) {
-        const uint32_t mid = (lo + hi) >> 1;
-        if (p.first[mid] <= d) lo = mid;
-        else hi = mid;
+__global__ void __launch_bounds__(kThreads, 2) compact_kernel(const __grid_constant__ TGKvCompactParams p) {
+    __shared__ uint32_t start[TGKV_MAX_ITEMS], first[TGKV_MAX_ITEMS + 1];
+    {
+        // side by side through ordinary loads, not one by one through the constant cache
+        const uint32_t *s = p.start, *f = p.first;
+        asm volatile("" : "+l"(s), "+l"(f));
+        for (uint32_t i = threadIdx.x; i < p.n_ranges; i += kThreads) {
+            start[i] = s[i];
+            first[i] = f[i];
+        }
+        if (threadIdx.x == 0) first[p.n_ranges] = p.n_keep;
     }
-    return (uint64_t)p.start[lo] + (d - p.first[lo]);
-}
-
-__global__ void __launch_bounds__(kThreads) compact_kernel(const __grid_constant__ TGKvCompactParams p) {
+    __syncthreads();
     uint32_t cl;
     asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(cl));
     const uint32_t rank = cluster_ctarank();
     const uint32_t unit = blockIdx.x / cl;        // (cache, half, slice)
     const uint32_t slice = unit % p.n_slices, half = (unit / p.n_slices) & 1u;
     const uint32_t ci = unit / p.n_slices / 2;
-    const uint64_t rv = p.row_bytes / 16;         // vectors of a row
-    const uint32_t sv = (uint32_t)(rv / p.n_slices);
-    uint4* mem = reinterpret_cast<uint4*>(p.caches[ci].base + half * p.caches[ci].max_seq * p.row_bytes) +
-                 (uint64_t)slice * sv;
-    // vector v of the slice's destination vectors: row v / sv, column v % sv
-    const uint64_t total = (uint64_t)(p.n_keep - p.skip) * sv;
-    const uint64_t per = (uint64_t)cl * kThreads * kMoveVec;
-    const uint64_t mine = (uint64_t)rank * kThreads * kMoveVec + threadIdx.x;
-    uint4 a[kMoveVec];
-    auto load = [&](uint64_t w) {
+    const uint32_t rv = (uint32_t)(p.row_bytes / 16);                     // vectors of a row
+    const uint32_t width = (rv + p.n_slices - 1) / p.n_slices;            // of a slice, at most kThreads
+    const uint32_t per = kThreads / width;                                // rows side by side
+    const uint32_t col = slice * width + threadIdx.x % width, lane_row = threadIdx.x / width;
+    const bool mine = lane_row < per && col < rv;
+    uint4* mem = reinterpret_cast<uint4*>(p.caches[ci].base + half * p.caches[ci].max_seq * p.row_bytes) + col;
+    // wave w of this CTA: rows d0 + w * step + u * per, u < kMoveRows
+    const uint32_t rows_cta = per * kMoveRows;
+    const uint64_t step = (uint64_t)cl * rows_cta;
+    const uint64_t d0 = p.skip + (uint64_t)rank * rows_cta + lane_row;
+    const uint32_t waves = (uint32_t)((p.n_keep - p.skip + step - 1) / step);
+    uint4 a[kMoveRows];
+    uint32_t ri = 0;                              // the range of the last row read
+    auto load = [&](uint64_t d) {
+        // the range of row d: behind the last one's, most often far behind
+        uint32_t hi = p.n_ranges;
+        while (hi - ri > 1) {
+            const uint32_t mid = (ri + hi) >> 1;
+            if (first[mid] <= d) ri = mid;
+            else hi = mid;
+        }
 #pragma unroll
-        for (int u = 0; u < kMoveVec; ++u) {
-            const uint64_t v = w * per + mine + (uint64_t)u * kThreads;
-            if (v < total) {
-                const uint32_t d = p.skip + (uint32_t)(v / sv);
-                a[u] = mem[source_row(p, d) * rv + v % sv];
+        for (int u = 0; u < kMoveRows; ++u, d += per)
+            if (mine && d < p.n_keep) {
+                while (first[ri + 1] <= d) ++ri;
+                a[u] = __ldcs(mem + ((uint64_t)start[ri] + (d - first[ri])) * rv);
             }
-        }
     };
-    auto store = [&](uint64_t w, const uint4 (&x)[kMoveVec]) {
+    load(d0);
+    for (uint32_t w = 0; w < waves; ++w) {
+        uint4 b[kMoveRows];
 #pragma unroll
-        for (int u = 0; u < kMoveVec; ++u) {
-            const uint64_t v = w * per + mine + (uint64_t)u * kThreads;
-            if (v < total) mem[(uint64_t)(p.skip + (uint32_t)(v / sv)) * rv + v % sv] = x[u];
-        }
-    };
-    const uint64_t waves = (total + per - 1) / per;
-    load(0);
-    for (uint64_t w = 0; w < waves; ++w) {
-        uint4 b[kMoveVec];
-#pragma unroll
-        for (int u = 0; u < kMoveVec; ++u) b[u] = a[u];
+        for (int u = 0; u < kMoveRows; ++u) b[u] = a[u];
+        __syncwarp();                             // the .aligned cluster barrier wants whole warps
         cluster_arrive();
-        if (w + 1 < waves) load(w + 1);
+        const uint64_t d = d0 + w * step;
+        if (w + 1 < waves) load(d + step);
+        __syncwarp();
         cluster_wait();
-        store(w, b);
+#pragma unroll
+        for (int u = 0; u < kMoveRows; ++u)
+            if (mine && d + (uint64_t)u * per < p.n_keep) mem[(d + (uint64_t)u * per) * rv] = b[u];
     }
 }
 
