@@ -154,6 +154,12 @@ DECODE = [  # old lengths, prefix (None: no cache), heads, kv heads, head_dim
     (list(range(0, 140, 2)), 640, 16, 2, 128),
     ([2000], 3001, 128, 1, 64),
     ([17] * 40, 4000, 6, 3, 64),
+    ([33] * 64, 1030, 32, 8, 128),                           # a long enough prefix for many: shared
+    ([5, 0, 300, 9], 20000, 32, 8, 128),                     # shared by four
+    ([9000, 20], None, 8, 2, 64),                            # several CTAs per sequence
+    ([70000], None, 2, 1, 64),                               # more than 32 CTAs for one row
+    ([255, 256, 383], 130, 32, 2, 128),                      # 16 query heads per KV head
+    ([90, 4], 200, 36, 2, 128),                              # 18
 ]
 
 
@@ -184,6 +190,10 @@ PROMPT = [  # old lengths, new tokens, prefix, heads, kv heads, head_dim
     ([0, 20], [70, 33], 65, 7, 1, 64),
     ([1500], [600], 900, 4, 1, 64),
     ([0, 0], [3, 2], 50, 128, 1, 128),
+    ([10] * 12, [2, 9, 1, 4, 31, 8, 1, 1, 3, 5, 6, 7], 9000, 16, 2, 128),
+    ([7] * 20, [6] * 20, 3000, 16, 4, 128),
+    ([126, 300, 5], [2, 1, 2], 77, 8, 2, 64),                # few tokens, over a tile's end
+    ([125, 0], [5, 3], None, 2, 2, 128),
 ]
 
 

@@ -1072,25 +1072,51 @@ uint64_t tg_cuda_kv_group_scratch_bytes(uint32_t n_seq, uint32_t n_heads, uint32
     return group_rows(n_seq, n_heads) * (head_dim + 2) * 4;
 }
 
+/* A merge launch, in tiles: about 5 us. */
+enum { kMergeTiles = 6 };
+
 /* The stretches of a line: the items of sequences [first, last] (0: the shared
  * prefix) on up to `sms` CTAs. */
 static void plan_line(const TGKvGroupShape* sh, uint32_t first, uint32_t last, uint32_t sms, TGKvGroupLine* ln) {
     ln->n_cta = ln->n_split = 0;
     ln->item_tokens = sh->item_tokens;
-    uint64_t cost = 0, units = 0;
+    uint64_t cost = 0, units = 0, n_items = 0;
+    uint32_t longest = 0;
     for (uint32_t s = tgkv_group_skip(sh, first); s <= last; s = tgkv_group_skip(sh, s + 1)) {
         const uint32_t n = tgkv_group_items(sh, s);
         uint64_t tiles = 0;
-        for (uint32_t at = 0; at < n; at++) tiles += tgkv_group_item_tiles(sh, s, at);
+        for (uint32_t at = 0; at < n; at++) {
+            const uint32_t one = tgkv_group_item_tiles(sh, s, at);
+            tiles += one;
+            if (one > longest) longest = one;
+        }
+        n_items += n;
         units += tiles * sh->n_kv_heads;
         cost += (tiles + (uint64_t)n * sh->item_cost) * sh->n_kv_heads;
     }
     if (units == 0) return;
-    uint32_t n_cta = sms && sms < TGKV_GROUP_MAX_CTAS ? sms : TGKV_GROUP_MAX_CTAS;
-    if (units < n_cta) n_cta = (uint32_t)units;
-    ln->n_cta = n_cta;
+    const uint32_t most = sms && sms < TGKV_GROUP_MAX_CTAS ? sms : TGKV_GROUP_MAX_CTAS;
     TGKvGroupPos* start = (TGKvGroupPos*)ln->start;
     uint32_t b = 0, s = tgkv_group_skip(sh, first);
+    if (n_items * sh->n_kv_heads <= most && longest <= units / most + kMergeTiles) {
+        /* a CTA per item: the longest item takes no longer than shorter stretches and
+         * the merge that they would need */
+        for (; s <= last; s = tgkv_group_skip(sh, s + 1))
+            for (uint32_t kvh = 0; kvh < sh->n_kv_heads; kvh++)
+                for (uint32_t at = 0; at < tgkv_group_items(sh, s); at++) {
+                    start[b].seq = s;
+                    start[b].kvh = kvh;
+                    start[b].at = at;
+                    start[b++].tile = 0;
+                }
+        ln->n_cta = b;
+        start[b].seq = s;
+        start[b].kvh = start[b].at = start[b].tile = 0;
+        return;
+    }
+    uint32_t n_cta = most;
+    if (units < 2ull * n_cta) n_cta = (uint32_t)((units + 1) / 2);       /* a tile for each stream */
+    ln->n_cta = n_cta;
     uint64_t done = 0;                              /* cost before the current item */
     for (; s <= last; s = tgkv_group_skip(sh, s + 1)) {
         const uint32_t n = tgkv_group_items(sh, s);
@@ -1166,13 +1192,17 @@ static int plan_group(const TGCudaGroupCall* c, uint32_t sms, TGKvGroupParams* p
     TGKvGroupShape heavy = {p->n_seq, p->n_kv_heads, p->prefix_len, 0, tpt, c->act == 1 ? 2 * tpt : tpt,
                             c->act == 1 ? 1 : 5, p->old_len, p->tok0};
     /* Split when items over all sequences' tokens need at most 3/4 of the prefix
-     * passes that the sequences' own items make. */
+     * passes that the sequences' own items make, and that saves every SM more tiles
+     * than the merge takes. */
     uint64_t own_items = seqs;
     if (!own_light) {
         own_items = 0;
         for (uint32_t i = 1; i <= c->n_seq; i++) own_items += tgkv_group_items(&heavy, i);
     }
-    if (c->prefix_len && 4 * ((total + heavy.item_tokens - 1) / heavy.item_tokens) <= 3 * own_items &&
+    const uint64_t shared_items = (total + heavy.item_tokens - 1) / heavy.item_tokens;
+    const uint64_t pre_tiles = (c->prefix_len + TGKV_GROUP_TILE - 1ull) / TGKV_GROUP_TILE;
+    if (c->prefix_len && 4 * shared_items <= 3 * own_items &&
+        (own_items - shared_items) * pre_tiles * c->n_kv_heads > (uint64_t)kMergeTiles * (sms ? sms : TGKV_GROUP_MAX_CTAS) &&
         2 * total * c->n_heads <= group_share_rows(c->n_seq, c->n_heads))
         p->share = heavy.share = 1;
     TGKvGroupShape light = heavy;
@@ -1180,6 +1210,7 @@ static int plan_group(const TGCudaGroupCall* c, uint32_t sms, TGKvGroupParams* p
     light.item_cost = 4;
     const int all_light = own_light && (!p->share || total <= light_tokens);
     p->own_line = own_light;
+    p->append = own_light && c->k_new;             /* by the CTAs that load the rows' tiles */
     p->prefix_line = all_light;
     if (!own_light) plan_line(&heavy, 0, c->n_seq, sms, &p->line[0]);
     else if (all_light) plan_line(&light, 0, c->n_seq, sms, &p->line[1]);

@@ -95,14 +95,7 @@ __global__ void __launch_bounds__(256) group_append_kernel(const __grid_constant
     const TGKvRowCache c = p.table[i];
     uint16_t* dst = reinterpret_cast<uint16_t*>(c.base) +
                     ((uint64_t)blockIdx.y * c.max_seq + as_memory(p.old_len)[i] + (t - tok0[i])) * kv_dim + e;
-    uint4 w;
-    if constexpr (sizeof(T) == 4) {
-        const float4 a = *reinterpret_cast<const float4*>(src), b = *reinterpret_cast<const float4*>(src + 4);
-        w = make_uint4(pack_bf16x2(a.x, a.y), pack_bf16x2(a.z, a.w), pack_bf16x2(b.x, b.y), pack_bf16x2(b.z, b.w));
-    } else {
-        w = *reinterpret_cast<const uint4*>(src);
-    }
-    *reinterpret_cast<uint4*>(dst) = w;
+    *reinterpret_cast<uint4*>(dst) = row_part(src);
     // read by the attention's TMA loads
     asm volatile("fence.proxy.async.global;" ::: "memory");
 }
@@ -833,7 +826,7 @@ int launch(const TGKvGroupParams* p, cudaStream_t st) {
     constexpr uint32_t smem = Cfg<HD>::SMEM > light::Cfg<T, HD>::SMEM ? Cfg<HD>::SMEM : light::Cfg<T, HD>::SMEM;
     cudaError_t e = allow_smem(group_kernel<T, HD>, smem, done);
     if (e != cudaSuccess) return (int)e;
-    if (p->k_new) {
+    if (p->k_new && !p->append) {
         const uint64_t n = (uint64_t)total * (p->n_kv_heads * HD / 8);
         e = launch_pdl(group_append_kernel<T>, dim3((unsigned)((n + 255) / 256), 2), 256, 0, st, p);
         if (e != cudaSuccess) return (int)e;

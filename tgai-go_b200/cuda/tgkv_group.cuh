@@ -126,6 +126,13 @@ __device__ __forceinline__ void tmem_wait_ld16(uint32_t (&r)[16]) {
                    "+r"(r[15])::"memory");
 }
 
+// 8 elements of a new row as the cache stores them.
+__device__ __forceinline__ uint4 row_part(const float* src) {
+    const float4 a = *reinterpret_cast<const float4*>(src), b = *reinterpret_cast<const float4*>(src + 4);
+    return make_uint4(pack_bf16x2(a.x, a.y), pack_bf16x2(a.z, a.w), pack_bf16x2(b.x, b.y), pack_bf16x2(b.z, b.w));
+}
+__device__ __forceinline__ uint4 row_part(const uint16_t* src) { return *reinterpret_cast<const uint4*>(src); }
+
 // Programmatic dependent launch (TGKV_PDL=0 turns it off): each kernel waits
 // (griddepcontrol.wait) before its first access to global memory.
 template <typename K>

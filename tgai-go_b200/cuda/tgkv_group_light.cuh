@@ -130,31 +130,58 @@ __device__ __forceinline__ void run(const TGKvGroupParams& p, uint32_t cta_index
 
     Pieces pc(sh, start_of(p, 1, cta_index), start_of(p, 1, cta_index + 1), kMost);
     if (warp == kTmaWarp) {
-        if (lane == 0) {
-            uint32_t n = 0, nv = 0;              // K and V tiles issued
-            bool ok = true;
-            for (; ok && pc.more(); pc.next(sh, kMost)) {
-                const uint32_t seq = pc.at.seq, npre = tgkv_group_prefix_tiles(&sh, seq);
-                const int x = (int)(pc.at.kvh * HD);
-                for (uint32_t j = pc.j0; j < pc.j1; ++j) {
-                    const bool own = j >= npre;
-                    const uint64_t map = p.tmaps + 128ull * (own ? seq - 1 : p.n_seq);
-                    const int y = (int)((own ? j - npre : j) * kPos);
-                    const uint32_t s = n % C::kStages, ph = (n / C::kStages - 1) & 1u;
-                    if (n >= C::kStages && !(ok = mbar_wait(&bar[C::B_KEMPTY + s], ph))) break;
-                    mbar_arrive_expect_tx(&bar[C::B_KFULL + s], C::kTile);
-                    for (int b = 0; b < HD / 64; ++b)
-                        tma_load_3d(base + C::OFF_K + s * C::kTile + b * kBlock, map, x + 64 * b, y, 0,
-                                    &bar[C::B_KFULL + s]);
-                    ++n;
-                    if (nv >= C::kStages && !(ok = mbar_wait(&bar[C::B_VEMPTY + s], ph))) break;
-                    mbar_arrive_expect_tx(&bar[C::B_VFULL + s], C::kTile);
-                    for (int b = 0; b < HD / 64; ++b)
-                        tma_load_3d(base + C::OFF_V + s * C::kTile + b * kBlock, map, x + 64 * b, y, 1,
-                                    &bar[C::B_VFULL + s]);
-                    ++nv;
+        uint32_t n = 0, nv = 0;                  // K and V tiles issued
+        bool ok = true;
+        for (; ok && pc.more(); pc.next(sh, kMost)) {
+            const uint32_t seq = pc.at.seq, npre = tgkv_group_prefix_tiles(&sh, seq);
+            const int x = (int)(pc.at.kvh * HD);
+            for (uint32_t j = pc.j0; ok && j < pc.j1; ++j) {
+                const bool own = j >= npre;
+                const uint64_t map = p.tmaps + 128ull * (own ? seq - 1 : p.n_seq);
+                const uint32_t y = (own ? j - npre : j) * kPos;
+                if (p.append && own) {
+                    // the new rows of this KV head and tile: stored here, where alone they are
+                    // loaded, 8 elements a lane
+                    const uint32_t first = old_len[seq - 1], r0 = max(y, first),
+                                   r1 = min(y + kPos, first + tgkv_group_tokens(&sh, seq));
+                    if (r0 < r1) {
+                        const uint64_t kv_dim = (uint64_t)p.n_kv_heads * HD;
+                        const TGKvRowCache c = p.table[seq - 1];
+                        for (uint32_t i = lane; i < (r1 - r0) * (HD / 4); i += 32) {
+                            const uint32_t v = i % (HD / 4), half = v / (HD / 8), e = v % (HD / 8) * 8 + pc.at.kvh * HD;
+                            const uint32_t row = r0 + i / (HD / 4);
+                            *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(c.base) +
+                                                      (half * c.max_seq + row) * kv_dim + e) =
+                                row_part(reinterpret_cast<const T*>(half ? p.v_new : p.k_new) +
+                                         (uint64_t)(tok0[seq - 1] + (row - first)) * kv_dim + e);
+                        }
+                        asm volatile("fence.proxy.async.global;" ::: "memory");
+                        __syncwarp();
+                    }
                 }
+                const uint32_t s = n % C::kStages, ph = (n / C::kStages - 1) & 1u;
+                if (lane == 0) {
+                    if (n >= C::kStages) ok = mbar_wait(&bar[C::B_KEMPTY + s], ph);
+                    if (ok) {
+                        mbar_arrive_expect_tx(&bar[C::B_KFULL + s], C::kTile);
+                        for (int b = 0; b < HD / 64; ++b)
+                            tma_load_3d(base + C::OFF_K + s * C::kTile + b * kBlock, map, x + 64 * b, (int)y, 0,
+                                        &bar[C::B_KFULL + s]);
+                        ++n;
+                        if (nv >= C::kStages) ok = mbar_wait(&bar[C::B_VEMPTY + s], ph);
+                    }
+                    if (ok) {
+                        mbar_arrive_expect_tx(&bar[C::B_VFULL + s], C::kTile);
+                        for (int b = 0; b < HD / 64; ++b)
+                            tma_load_3d(base + C::OFF_V + s * C::kTile + b * kBlock, map, x + 64 * b, (int)y, 1,
+                                        &bar[C::B_VFULL + s]);
+                        ++nv;
+                    }
+                }
+                ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
             }
+        }
+        if (lane == 0) {
             // every copy has landed before the CTA may end (at once in a normal run)
             for (uint32_t i = n > C::kStages ? n - C::kStages : 0; i < n; ++i)
                 ok = mbar_wait(&bar[C::B_KFULL + i % C::kStages], (i / C::kStages) & 1u) && ok;

@@ -235,7 +235,7 @@ typedef struct {
     float    qscale;             /* softmax scale * log2(e) */
     uint32_t share;
     uint32_t prefix_line, own_line;   /* whose items the shared prefix's and the sequences' are */
-    uint32_t pad;
+    uint32_t append;             /* the new rows are stored by line 1, not by a launch before */
     TGKvGroupLine line[2];
     uint32_t old_len[TGKV_MAX_ITEMS];       /* own rows before the call's tokens */
     uint32_t tok0[TGKV_MAX_ITEMS + 1];      /* first packed token of each sequence; the total */
