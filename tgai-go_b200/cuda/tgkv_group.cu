@@ -100,41 +100,32 @@ __global__ void __launch_bounds__(256) group_append_kernel(const __grid_constant
     asm volatile("fence.proxy.async.global;" ::: "memory");
 }
 
-template <bool MASK>
-__device__ __forceinline__ float max32(const uint32_t (&v)[32], int lim) {
+__device__ __forceinline__ float max32(const uint32_t (&v)[32]) {
     float a[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         a[i] = -INFINITY;
 #pragma unroll
-        for (int k = 0; k < 8; k += 2) {
-            const float x = __uint_as_float(v[8 * i + k]), y = __uint_as_float(v[8 * i + k + 1]);
-            a[i] = max3(a[i], (!MASK || 8 * i + k < lim) ? x : -INFINITY, (!MASK || 8 * i + k + 1 < lim) ? y : -INFINITY);
-        }
+        for (int k = 0; k < 8; k += 2) a[i] = max3(a[i], __uint_as_float(v[8 * i + k]), __uint_as_float(v[8 * i + k + 1]));
     }
     return max3(max3(a[0], a[1], a[2]), a[3], a[3]);
 }
 
 // P = 2^(s * scale - msc) of 32 positions as bf16 words (two positions each) into
 // the TMEM columns from `col` on: hi there and, with two terms, the rounding
-// residuals lo 32 columns behind; the fp32 values add up in l.  Positions at or
-// behind lim get 0.  (A part of the exponentials as a polynomial on the FMA units
-// measured no faster: 490 us with none to a quarter of them, 513 us with three
-// eighths, 4 prompts of 2000 tokens behind 2048; the streams' chain of products
-// bounds the kernel, not the exponential unit.)
-template <int TERMS, bool MASK>
-__device__ __forceinline__ void exp32(const uint32_t (&v)[32], float scale, float msc, int lim, float2& l,
-                                      uint32_t col) {
+// residuals lo 32 columns behind; the fp32 values add up in l.  A position the row
+// does not see has s = -inf and gets 0.  (A part of the exponentials as a polynomial
+// on the FMA units measured no faster: 490 us with none to a quarter of them, 513 us
+// with three eighths, 4 prompts of 2000 tokens behind 2048; the streams' chain of
+// products bounds the kernel, not the exponential unit.)
+template <int TERMS>
+__device__ __forceinline__ void exp32(const uint32_t (&v)[32], float scale, float msc, float2& l, uint32_t col) {
     const float2 sc = make_float2(scale, scale), nm = make_float2(-msc, -msc);
     uint32_t ph[16], pl[16];
 #pragma unroll
     for (int c = 0; c < 16; ++c) {
         const float2 d = __ffma2_rn(make_float2(__uint_as_float(v[2 * c]), __uint_as_float(v[2 * c + 1])), sc, nm);
-        float2 pp = make_float2(ex2_approx(d.x), ex2_approx(d.y));
-        if (MASK) {
-            pp.x = 2 * c < lim ? pp.x : 0.f;
-            pp.y = 2 * c + 1 < lim ? pp.y : 0.f;
-        }
+        const float2 pp = make_float2(ex2_approx(d.x), ex2_approx(d.y));
         l = __fadd2_rn(l, pp);
         ph[c] = cvt_bf16x2(pp.x, pp.y);
         if (TERMS == 2) {
@@ -429,8 +420,14 @@ __device__ __forceinline__ void run(const TGKvGroupParams& p, uint32_t cta_index
                         tmem_ld32(tsb, va);
                         tmem_ld32(tsb + 32, vb);
                         tmem_wait_ld(va, vb);
-                        const float tm = mask ? max3(-INFINITY, max32<true>(va, lm), max32<true>(vb, lm - 32))
-                                              : max3(-INFINITY, max32<false>(va, 0), max32<false>(vb, 0));
+                        if (mask) {
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) {
+                                if (i >= lm) va[i] = 0xff800000u;                // -inf
+                                if (i >= lm - 32) vb[i] = 0xff800000u;
+                            }
+                        }
+                        const float tm = max3(-INFINITY, max32(va), max32(vb));
                         // the running maximum moves only when exceeded by more than 2^8 (or NaN)
                         const bool grow = !((tm - m) * scale <= 8.f);
                         if (__any_sync(0xffffffffu, grow)) {
@@ -457,13 +454,8 @@ __device__ __forceinline__ void run(const TGKvGroupParams& p, uint32_t cta_index
                             }
                         }
                         const float msc = m == -INFINITY ? 0.f : m * scale;
-                        if (mask) {
-                            exp32<TERMS, true>(va, scale, msc, lm, l2, tsb);
-                            exp32<TERMS, true>(vb, scale, msc, lm - 32, l2, tsb + 16);
-                        } else {
-                            exp32<TERMS, false>(va, scale, msc, 0, l2, tsb);
-                            exp32<TERMS, false>(vb, scale, msc, 0, l2, tsb + 16);
-                        }
+                        exp32<TERMS>(va, scale, msc, l2, tsb);
+                        exp32<TERMS>(vb, scale, msc, l2, tsb + 16);
                         tmem_wait_st();
                     }
                     tc_fence_before();

@@ -81,6 +81,20 @@ __device__ __forceinline__ void tmem_ld_cols(uint32_t taddr, uint32_t (&v)[16]) 
 __device__ __forceinline__ void tmem_st_cols(uint32_t addr, const uint32_t (&w)[32]) { tmem_st32(addr, w); }
 __device__ __forceinline__ void tmem_st_cols(uint32_t addr, const uint32_t (&w)[16]) { tmem_st16(addr, w); }
 
+// One column of this thread's TMEM lane.
+__device__ __forceinline__ float tmem_ld1(uint32_t taddr) {
+    uint32_t v;
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];" : "=r"(v) : "r"(taddr));
+    asm volatile("tcgen05.wait::ld.sync.aligned;" : "+r"(v)::"memory");
+    return __uint_as_float(v);
+}
+// A row's sums over its terms.
+template <int TERMS, int ROWS>
+__device__ __forceinline__ float tmem_ld_row(uint32_t taddr) {
+    if constexpr (TERMS == 1) return tmem_ld1(taddr);
+    return (tmem_ld1(taddr) + tmem_ld1(taddr + ROWS)) + tmem_ld1(taddr + 2 * ROWS);
+}
+
 template <typename T, int HD>
 __device__ __forceinline__ void run(const TGKvGroupParams& p, uint32_t cta_index, unsigned char* smem_raw) {
     using C = Cfg<T, HD>;
@@ -273,6 +287,10 @@ __device__ __forceinline__ void run(const TGKvGroupParams& p, uint32_t cta_index
         const uint32_t total_rows = tok0[p.n_seq] * p.n_heads;
         uint32_t g0 = 0, it = 0, n = 0;          // K/V tiles of earlier pieces; pieces; this stream's steps
         bool ok = true;
+        // row x of an item, from its first row: its token's, one of G heads
+        auto row_of = [&](uint64_t row0, uint32_t x, uint32_t tokens) -> uint64_t {
+            return tokens == 1 ? row0 + x : row0 + (uint64_t)(x / G) * p.n_heads + x % G;
+        };
         // q of a piece, as TERMS bf16 rows each: two dims a thread, the streams take every other
         // row.  Loaded while the piece before is worked on, stored once that one's last S^T is made.
         constexpr int kMine = (ROWS + 1) / 2;
@@ -289,7 +307,7 @@ __device__ __forceinline__ void run(const TGKvGroupParams& p, uint32_t cta_index
             for (int i = 0; i < kMine; ++i) {
                 const uint32_t x = 2 * i + h;
                 if (x >= q_rows) break;
-                const uint64_t e = (row0 + x / G * p.n_heads + x % G) * HD + 2 * r;
+                const uint64_t e = row_of(row0, x, ir.tokens) * HD + 2 * r;
                 if constexpr (TERMS == 3) qv[i] = *reinterpret_cast<const float2*>(reinterpret_cast<const float*>(p.q) + e);
                 else qv[i].x = __uint_as_float(*reinterpret_cast<const uint32_t*>(reinterpret_cast<const uint16_t*>(p.q) + e));
             }
@@ -440,52 +458,41 @@ __device__ __forceinline__ void run(const TGKvGroupParams& p, uint32_t cta_index
             const bool again = TERMS == 3 && cur.j0 > cur.first;                         // adds to the item's earlier piece here
             const uint64_t cta = (uint64_t)p.line[1].cta_rows +
                                  TGKV_GROUP_LIGHT_ROWS * (2u * cta_index + (cur.first > 0 ? 0u : 1u));
-            uint32_t v[N];
-            float oa[ROWS], ob[ROWS];            // the streams' sums, over the terms
-            if (ok) tmem_ld_cols(to, v);
-#pragma unroll
-            for (int x = 0; x < ROWS; ++x) {
-                oa[x] = __uint_as_float(v[x]);
-                if constexpr (TERMS == 3) oa[x] = (oa[x] + __uint_as_float(v[ROWS + x])) + __uint_as_float(v[2 * ROWS + x]);
-            }
-            if (ok) tmem_ld_cols(to + 64, v);
-#pragma unroll
-            for (int x = 0; x < ROWS; ++x) {
-                ob[x] = __uint_as_float(v[x]);
-                if constexpr (TERMS == 3) ob[x] = (ob[x] + __uint_as_float(v[ROWS + x])) + __uint_as_float(v[2 * ROWS + x]);
-            }
-#pragma unroll
-            for (int x = 0; x < ROWS; ++x) {
-                if ((uint32_t)x >= R) break;
-                if (ok && r < HD && (x & 1) == h) {
-                    const float ma = maxima[x], mb = maxima[16 + x];
-                    float M = max3(ma, mb, ma);
-                    const float wa = ma == -INFINITY ? 0.f : ex2_approx(ma - M), wb = mb == -INFINITY ? 0.f : ex2_approx(mb - M);
-                    const float* ra = red_all + x;
-                    float L = wa * ((ra[0] + ra[16]) + (ra[32] + ra[48])) + wb * ((ra[64] + ra[80]) + (ra[96] + ra[112]));
-                    // (a stream that had no tile left O^T as it was)
-                    float o = (wa == 0.f ? 0.f : oa[x] * wa) + (wb == 0.f ? 0.f : ob[x] * wb);
-                    const uint64_t row = row0 + x / (int)G * p.n_heads + x % (int)G;
-                    const uint64_t slot = cur.first > 0 || !p.share ? cta + x : (seq ? total_rows : 0u) + row;
-                    if (again) {
-                        const float2 old = *reinterpret_cast<const float2*>(p.part_ml + slot * 2);
-                        const float M2 = max3(M, old.x, M);
-                        const float wn = M == -INFINITY ? 0.f : ex2_approx(M - M2), wo = old.x == -INFINITY ? 0.f : ex2_approx(old.x - M2);
-                        o = o * wn + (wo == 0.f ? 0.f : p.part_o[slot * HD + r] * wo);
-                        L = L * wn + old.y * wo;
-                        M = M2;
-                    }
+            // A loop, not unrolled: code that runs once an item costs its fetch.  The streams take
+            // every other row.
+#pragma unroll 1
+            for (uint32_t x = (uint32_t)h; ok && x < R; x += 2) {
+                const float a = tmem_ld_row<TERMS, ROWS>(to + x), b = tmem_ld_row<TERMS, ROWS>(to + 64 + x);
+                const float ma = maxima[x], mb = maxima[16 + x];
+                float M = max3(ma, mb, ma);
+                const float wa = ma == -INFINITY ? 0.f : ex2_approx(ma - M), wb = mb == -INFINITY ? 0.f : ex2_approx(mb - M);
+                const float* ra = red_all + x;
+                float L = wa * ((ra[0] + ra[16]) + (ra[32] + ra[48])) + wb * ((ra[64] + ra[80]) + (ra[96] + ra[112]));
+                // (a stream that had no tile left O^T as it was)
+                float o = (wa == 0.f ? 0.f : a * wa) + (wb == 0.f ? 0.f : b * wb);
+                const uint64_t row = row_of(row0, x, pr.tokens);
+                const uint64_t slot = cur.first > 0 || !p.share ? cta + x : (seq ? total_rows : 0u) + row;
+                if (again) {
+                    const float2 old = *reinterpret_cast<const float2*>(p.part_ml + slot * 2);
+                    const float M2 = max3(M, old.x, M);
+                    const float wn = M == -INFINITY ? 0.f : ex2_approx(M - M2), wo = old.x == -INFINITY ? 0.f : ex2_approx(old.x - M2);
+                    if (r < HD) o = o * wn + (wo == 0.f ? 0.f : p.part_o[slot * HD + r] * wo);
+                    L = L * wn + old.y * wo;
+                    M = M2;
+                }
+                if (r < HD) {
                     if (!whole) p.part_o[slot * HD + r] = o;
                     else if constexpr (TERMS == 3) reinterpret_cast<float*>(p.out)[row * HD + r] = o / L;
                     else reinterpret_cast<uint16_t*>(p.out)[row * HD + r] = (uint16_t)(cvt_bf16x2(o / L, 0.f) & 0xffffu);
-                    joint[x] = M;                // the same from every thread of the row
-                    joint[16 + x] = L;
                 }
+                joint[x] = M;                    // the same from every thread
+                joint[16 + x] = L;
+                __syncwarp();
             }
             tc_fence_before();
             streams_sync();                      // O^T, the sums and the slots' (m, l) have been read
             if (!whole && ok && (uint32_t)r < R && (r & 1) == h) {
-                const uint64_t row = row0 + r / (int)G * p.n_heads + r % (int)G;
+                const uint64_t row = row_of(row0, (uint32_t)r, pr.tokens);
                 const uint64_t slot = cur.first > 0 || !p.share ? cta + r : (seq ? total_rows : 0u) + row;
                 *reinterpret_cast<float2*>(p.part_ml + slot * 2) = make_float2(joint[r], joint[16 + r]);
             }
