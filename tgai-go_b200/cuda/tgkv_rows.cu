@@ -28,8 +28,12 @@ __global__ void __launch_bounds__(kThreads) fork_kernel(const __grid_constant__ 
 #pragma unroll
     for (int u = 0; u < kForkVec; ++u)
         if (v0 + u * kThreads < p.n_vec) r[u] = __ldcs(src + v0 + u * kThreads);
+    // the destinations as ordinary memory: through the constant cache each would be a miss of its own
+    const TGKvRowCache* to = p.dst + i * p.fan;
+    asm volatile("" : "+l"(to));
+#pragma unroll 4
     for (uint32_t j = 0; j < p.fan; ++j) {
-        const TGKvRowCache c = p.dst[i * p.fan + j];
+        const TGKvRowCache c = to[j];
         uint4* dst = reinterpret_cast<uint4*>(c.base + half * c.max_seq * p.row_bytes);
 #pragma unroll
         for (int u = 0; u < kForkVec; ++u)
