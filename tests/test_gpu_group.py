@@ -344,3 +344,187 @@ def test_compact(cuda, n, rows, nkv, hd, dtype, kind):
         assert np.array_equal(raw[:, :len(index)], b.view(bits)[:, index])
         assert np.array_equal(raw[:, len(index):], b.view(bits)[:, len(index):])   # the rest as it was
         lib.tg_kv_destroy(c)
+
+
+# ------------------------------------------------------- used together, and refused
+def test_a_thousand_sequences(cuda, devbuf):
+    n = 1024
+    s = Setup(cuda, [i % 7 for i in range(n)], [2] * n, 300, 2, 1, 64, BF16, seed=31)
+    call(s, devbuf, [1] * n, decode=True)
+    call(s, devbuf, [(i % 3 == 0) * 1 for i in range(n)])
+    s.close()
+
+
+def test_on_a_stream_and_replayed_from_a_graph(cuda, devbuf):
+    """A step on its own stream, then captured once and replayed over new inputs in the same buffers."""
+    import torch
+    lib, n = cuda, 6
+    s = Setup(lib, [50 * i for i in range(n)], [40] * n, 700, 16, 4, 128, BF16, seed=41)
+    stream = torch.cuda.Stream()
+    handle = C.c_void_p(stream.cuda_stream)
+    call(s, devbuf, [1] * n, decode=True, stream=handle)
+    call(s, devbuf, [3, 0, 31, 1, 2, 5], stream=handle)
+    old = [r.shape[1] for r in s.rows]
+    (qb, _), (kb, _), (vb, _) = s.new(n)
+    qd, kd, vd, od = devbuf(qb), devbuf(kb), devbuf(vb), devbuf(nbytes=qb.nbytes)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        tgkv.check(lib.tg_kv_group_decode(s.g, qd.ptr, kd.ptr, vd.ptr, od.ptr, handle), lib)
+    before = s.rows
+    for _ in range(3):                           # each replay stores the row at the captured length
+        (qb, q), (kb, k), (vb, v) = s.new(n)
+        for d, b in ((qd, qb), (kd, kb), (vd, vb)):
+            assert lib.tg_cuda_kv_h2d(d.ptr, b.ctypes.data, b.nbytes, None)
+        graph.replay()
+        torch.cuda.synchronize()
+        s.rows = [r[:, :o] for r, o in zip(before, old)]
+        s.grow([1] * n, k, v)
+        want, tol = s.expect(q, [1] * n)
+        assert (np.abs(s.read(od, n) - want) <= tol).all()
+        s.check_caches()
+    del graph
+    s.close()
+
+
+def test_two_groups_over_one_prefix(cuda, devbuf):
+    """Groups with their own caches and scratch, on two streams at once."""
+    import torch
+    lib = cuda
+    a = Setup(lib, [100, 40, 7], [9] * 3, 2000, 8, 2, 128, F32, seed=51)
+    b = Setup(lib, [300, 2], [9] * 2, None, 8, 2, 128, F32, seed=52)
+    lib.tg_kv_group_destroy(b.g)
+    b.g = lib.tg_kv_group_create(a.prefix, b.arr, 2, 8, F32)
+    tgkv.check(b.g, lib)
+    b.P, b.prefix_rows = a.P, a.prefix_rows
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    outs = []
+    for s, st in zip((a, b), streams):
+        n = len(s.old)
+        (qb, q), (kb, k), (vb, v) = s.new(n)
+        bufs = devbuf(qb), devbuf(kb), devbuf(vb), devbuf(nbytes=qb.nbytes)
+        s.grow([1] * n, k, v)
+        outs.append((s, q, n, bufs))
+    for _ in range(4):
+        for (s, q, n, bufs), st in zip(outs, streams):
+            ptrs = [x.ptr for x in bufs]
+            lens = (C.c_uint32 * n)(*s.old)
+            tgkv.check(lib.tg_kv_group_truncate(s.g, lens), lib)
+            tgkv.check(lib.tg_kv_group_decode(s.g, *ptrs, C.c_void_p(st.cuda_stream)), lib)
+    torch.cuda.synchronize()
+    for s, q, n, bufs in outs:
+        want, tol = s.expect(q, [1] * n)
+        assert (np.abs(s.read(bufs[3], n) - want) <= tol).all()
+        s.check_caches()
+    b.close()
+    a.close()
+
+
+def test_a_serving_loop(cuda, devbuf):
+    """A system prompt through tg_kv_append_attention, chats behind it, a fork, an eviction, and on."""
+    lib, nh, nkv, hd, P = cuda, 16, 4, 128, 150
+    s = Setup(lib, [0, 0, 0], [400] * 3, 0, nh, nkv, hd, F32, seed=61)
+    lib.tg_kv_group_destroy(s.g)                             # a prefix cache with room, filled through the API
+    lib.tg_kv_destroy(s.prefix)
+    s.prefix = lib.tg_kv_create_ex(P + 50, nkv, hd, BF16)
+    s.g = lib.tg_kv_group_create(s.prefix, s.arr, 3, nh, F32)
+    tgkv.check(s.g, lib)
+    (qb, q), (kb, k), (vb, v) = s.new(P)
+    bufs = [devbuf(x) for x in (kb, vb, qb)] + [devbuf(nbytes=qb.nbytes)]
+    tgkv.check(lib.tg_kv_append_attention(s.prefix, *[x.ptr for x in bufs], nh, P, None), lib)
+    s.P, s.prefix_rows = P, np.stack([bf16(k)[1], bf16(v)[1]])
+    call(s, devbuf, [90, 0, 33])
+    call(s, devbuf, [1, 1, 1], decode=True)
+    # chat 1 becomes a branch of chat 0 (its own rows), then both go on
+    tgkv.check(lib.tg_kv_fork((C.c_void_p * 1)(s.caches[0]), 1, (C.c_void_p * 1)(s.caches[1]), 1, 60, None), lib)
+    s.rows[1] = s.rows[0][:, :60]
+    s.check_caches()
+    call(s, devbuf, [2, 40, 1])
+    # chat 0 keeps its first 4 and last 50 positions
+    n0 = s.rows[0].shape[1]
+    tgkv.check(lib.tg_kv_compact((C.c_void_p * 1)(s.caches[0]), 1, (C.c_uint32 * 2)(0, n0 - 50), (C.c_uint32 * 2)(4, 50),
+                                 2, None), lib)
+    s.rows[0] = np.concatenate([s.rows[0][:, :4], s.rows[0][:, n0 - 50:]], 1)
+    s.check_caches()
+    call(s, devbuf, [1, 1, 1], decode=True)
+    # the prefix grows: all sequences see it from the next call on
+    extra = s.rng.standard_normal((2, 20, s.kvd)).astype(np.float32)
+    tgkv.check(lib.tg_kv_append(s.prefix, extra[0].ctypes.data, extra[1].ctypes.data, 20), lib)
+    s.prefix_rows = np.concatenate([s.prefix_rows, bf16(extra)[1]], 1)
+    call(s, devbuf, [5, 1, 0])
+    s.close()
+
+
+@pytest.mark.parametrize("act", [F32, BF16])
+def test_a_nan_query_stays_in_its_row(cuda, devbuf, act):
+    s = Setup(cuda, [200, 10, 40], [8, 8, 8], 300, 8, 2, 128, act, seed=71)
+    n_new = [40, 1, 3]
+    s.cap = [c + 40 for c in s.cap]
+    normal = s.new
+
+    def new(total):
+        (qb, q), k, v = normal(total)
+        qb, q = qb.copy().reshape(total, 8, 128), q.copy().reshape(total, 8, 128)
+        qb[5, 3] = 0x7fc0 if act == BF16 else np.nan
+        q[5, 3] = np.nan
+        return [(qb.reshape(total, -1), q.reshape(total, -1)), k, v]
+    s.new = new
+    (qb, q), _, _ = s.new(44)
+    qd, od = devbuf(qb), devbuf(nbytes=qb.nbytes)
+    tgkv.check(cuda.tg_kv_group_prompt(s.g, (C.c_uint32 * 3)(*n_new), qd.ptr, None, None, od.ptr, None), cuda)
+    assert cuda.tg_cuda_kv_sync(None)
+    got, (want, tol) = s.read(od, 44), s.expect(q, n_new)
+    assert np.isnan(got[5, 3]).all()
+    rest = ~np.isnan(want)
+    assert rest.sum() == want.size - 128 and (np.abs(got - want)[rest] <= tol[rest]).all()
+    s.close()
+
+
+def test_refusals_change_nothing(cuda, devbuf):
+    lib = cuda
+    mk = lambda cap=64, nkv=2, hd=64, dt=BF16: lib.tg_kv_create_ex(cap, nkv, hd, dt)  # noqa: E731
+    a, b, p = mk(), mk(), mk()
+    f32, other, wide, hd32 = mk(dt=F32), mk(nkv=4), mk(hd=128), mk(hd=32)
+    arr = lambda *c: (C.c_void_p * len(c))(*c)  # noqa: E731
+    u = lambda *x: (C.c_uint32 * len(x))(*x)  # noqa: E731
+    err = lambda: lib.tg_kv_last_error()  # noqa: E731
+    for caches, pre, nh, act, why in [
+            (arr(a, a), None, 4, F32, b"twice"), (arr(a, b), a, 4, F32, b"twice"), (arr(a, other), None, 4, F32, b"differs"),
+            (arr(a, wide), None, 4, F32, b"differs"), (arr(a, f32), None, 4, F32, b"differs"), (arr(a), f32, 4, F32, b"differs"),
+            (arr(f32), None, 4, F32, b"no attention kernel"), (arr(hd32), None, 4, F32, b"no attention kernel"),
+            (arr(a), None, 3, F32, b"multiple"), (arr(a), None, 0, F32, b"multiple"), (arr(a), None, 258, F32, b"128 times"),
+            (arr(a), None, 4, 7, b"invalid dtype")]:
+        assert not lib.tg_kv_group_create(pre, caches, len(caches), nh, act)
+        assert why in err(), (why, err())
+    for c in (a, b, p):
+        lib.tg_kv_advance(c, 60)
+    g = lib.tg_kv_group_create(p, arr(a, b), 2, 4, F32)
+    d = devbuf(nbytes=1 << 20)
+    args = (d.ptr, d.ptr, d.ptr, d.ptr, None)
+    assert lib.tg_kv_group_prompt(g, u(4, 5), *args) == 0 and b"capacity exceeded at cache 1" in err()
+    assert lib.tg_kv_group_prompt(g, u(1, 61), d.ptr, None, None, d.ptr, None) == 0 and b"61 queries" in err()
+    assert lib.tg_kv_group_decode(g, d.ptr, d.ptr, None, d.ptr, None) == 0 and b"together" in err()
+    assert lib.tg_kv_group_decode(g, d.ptr + 4, d.ptr, d.ptr, d.ptr, None) == 0 and b"16-byte" in err()
+    assert lib.tg_kv_group_truncate(g, u(10, 61)) == 0 and b"beyond" in err()
+    lib.tg_kv_set_attn_mscale(b, 1.5)
+    assert lib.tg_kv_group_decode(g, *args) == 0 and b"mscale" in err()
+    for c in (a, b, p):
+        lib.tg_kv_set_attn_mscale(c, -1.0)
+    assert lib.tg_kv_group_decode(g, *args) == 0 and b"positive" in err()
+    assert lib.tg_kv_group_prompt(g, u(0, 0), d.ptr, None, None, d.ptr, None) == 0
+    for c in (a, b, p):
+        lib.tg_kv_set_attn_mscale(c, 1.0)
+    assert lib.tg_kv_group_prompt(g, u(0, 0), *args) == 1                   # nothing to do
+    assert lib.tg_kv_fork(arr(a), 1, arr(a), 1, 3, None) == 0 and b"source" in err()
+    assert lib.tg_kv_fork(arr(a), 1, arr(b, b), 2, 3, None) == 0 and b"twice" in err()
+    assert lib.tg_kv_fork(arr(a), 1, arr(b), 1, 61, None) == 0 and b"61 rows" in err()
+    assert lib.tg_kv_fork(arr(a), 1, arr(other), 1, 3, None) == 0 and b"differs" in err()
+    tiny = mk(cap=2)
+    assert lib.tg_kv_fork(arr(a), 1, arr(tiny), 1, 3, None) == 0 and b"capacity" in err()
+    assert lib.tg_kv_compact(arr(a, a), 2, u(0), u(1), 1, None) == 0 and b"twice" in err()
+    assert lib.tg_kv_compact(arr(a, tiny), 2, u(0), u(1), 1, None) == 0 and b"rows" in err()
+    assert lib.tg_kv_compact(arr(a), 1, u(59), u(2), 1, None) == 0 and b"beyond length 60" in err()
+    assert lib.tg_kv_compact(arr(a), 1, u(5, 6), u(2, 2), 2, None) == 0 and b"out of order" in err()
+    assert [lib.tg_kv_len(c) for c in (a, b, p, tiny)] == [60, 60, 60, 0]
+    lib.tg_kv_group_destroy(g)
+    for c in (a, b, p, f32, other, wide, hd32, tiny):
+        lib.tg_kv_destroy(c)
