@@ -230,6 +230,7 @@ typedef struct {
     float       scale;              /* softmax scale, > 0 */
     void*       scratch;            /* device, >= tg_cuda_kv_group_scratch_bytes() */
 } TGCudaGroupCall;
+/* 0 without a device. */
 uint64_t tg_cuda_kv_group_scratch_bytes(uint32_t n_seq, uint32_t n_heads, uint32_t head_dim);
 /* How a call's work is dealt to CTAs on a device of `sms` SMs (no launch, no
  * device needed): share 1 if the prefix is attended for all sequences' tokens

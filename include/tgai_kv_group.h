@@ -15,8 +15,11 @@
  * legacy default stream).  Lengths live on the host and travel with each
  * launch, so a call captured into a CUDA graph replays with the lengths it was
  * captured with.  No call allocates device memory after create.  A group's
- * scratch is shared by its calls: order calls and graph replays that use one
- * group (or one of its caches) on one stream or with events.
+ * scratch (about 59 MB at head_dim 128, half of it at 64) is shared by its
+ * calls: order calls and graph replays that use one group (or one of its caches,
+ * the prefix's rows included while they change) on one stream or with events.
+ * Calls of different groups may overlap.  Device waits are bounded; one that runs
+ * out leaves the call's output undefined and shows in tg_cuda_kv_device_error().
  */
 #ifndef TGAI_KV_GROUP_H
 #define TGAI_KV_GROUP_H
@@ -47,7 +50,8 @@ void       tg_kv_group_destroy(TGKvGroup* g);
  * cache's len grows by one.  With k_new and v_new NULL nothing is appended and
  * row i is the query of cache i's last position (len_i >= 1).  All pointers
  * are 16-byte aligned device addresses.  Scores are scaled by
- * mscale / sqrt(head_dim); all caches of the group have the same mscale > 0. */
+ * mscale / sqrt(head_dim); all caches of the group have the same mscale > 0.
+ * Rows behind a cache's length may hold anything. */
 int tg_kv_group_decode(TGKvGroup* g, const void* q, const void* k_new, const void* v_new,
                        void* out, void* stream);
 
@@ -58,7 +62,15 @@ int tg_kv_group_decode(TGKvGroup* g, const void* q, const void* k_new, const voi
  * sees the prefix and its own cache's positions up to its own.  Each cache's
  * len grows by n_new[i].  n_new is a host array.  With k_new and v_new NULL
  * nothing is appended and the queries are those of each cache's last n_new[i]
- * positions.  Otherwise as tg_kv_group_decode. */
+ * positions.  Otherwise as tg_kv_group_decode.
+ *
+ * Precision: scores, maxima and sums are fp32.  bf16 activations: q is exact, a
+ * weight is rounded once to bf16 before it meets V, as the output is.  fp32
+ * ones: q and the weights enter as two bf16 terms (16 mantissa bits; within
+ * 5e-5 of a head's output scale), or as three (24 bits) where no sequence has
+ * more than 10 query rows per KV head (most decode steps' own rows).  A V row of
+ * the call's own tokens that is not finite reaches the queries up to 127
+ * positions before it as NaN (0 x Inf), as in tg_kv_append_attention. */
 int tg_kv_group_prompt(TGKvGroup* g, const uint32_t* n_new, const void* q, const void* k_new,
                        const void* v_new, void* out, void* stream);
 

@@ -1065,10 +1065,11 @@ static uint64_t group_share_rows(uint32_t n_seq, uint32_t n_heads) {
     return 2 * (rows > 16384 ? rows : 16384);
 }
 static uint64_t group_rows(uint32_t n_seq, uint32_t n_heads) {
-    return group_share_rows(n_seq, n_heads) +
-           (2ull * 256 + 2 * TGKV_GROUP_LIGHT_ROWS) * TGKV_GROUP_MAX_CTAS;
+    const uint64_t ctas = g_sm_count > 0 && g_sm_count < TGKV_GROUP_MAX_CTAS ? g_sm_count : TGKV_GROUP_MAX_CTAS;
+    return group_share_rows(n_seq, n_heads) + (2ull * 256 + 2 * TGKV_GROUP_LIGHT_ROWS) * ctas;
 }
 uint64_t tg_cuda_kv_group_scratch_bytes(uint32_t n_seq, uint32_t n_heads, uint32_t head_dim) {
+    if (!g_ready && !tg_cuda_kv_init()) return 0;
     return group_rows(n_seq, n_heads) * (head_dim + 2) * 4;
 }
 
