@@ -51,7 +51,8 @@ void       tg_kv_group_destroy(TGKvGroup* g);
  * row i is the query of cache i's last position (len_i >= 1).  All pointers
  * are 16-byte aligned device addresses.  Scores are scaled by
  * mscale / sqrt(head_dim); all caches of the group have the same mscale > 0.
- * Rows behind a cache's length may hold anything. */
+ * Rows behind a cache's length may hold anything.  out overlaps none of the
+ * call's other arrays. */
 int tg_kv_group_decode(TGKvGroup* g, const void* q, const void* k_new, const void* v_new,
                        void* out, void* stream);
 
@@ -68,9 +69,9 @@ int tg_kv_group_decode(TGKvGroup* g, const void* q, const void* k_new, const voi
  * weight is rounded once to bf16 before it meets V, as the output is.  fp32
  * ones: q and the weights enter as two bf16 terms (16 mantissa bits; within
  * 5e-5 of a head's output scale), or as three (24 bits) where no sequence has
- * more than 10 query rows per KV head (most decode steps' own rows).  A V row of
- * the call's own tokens that is not finite reaches the queries up to 127
- * positions before it as NaN (0 x Inf), as in tg_kv_append_attention. */
+ * more than 10 query rows per KV head (most decode steps' own rows).  Values of
+ * K and V that are not finite reach the queries that see them and no others (with
+ * fp32 activations an infinity of V as NaN where lo parts of weights meet it). */
 int tg_kv_group_prompt(TGKvGroup* g, const uint32_t* n_new, const void* q, const void* k_new,
                        const void* v_new, void* out, void* stream);
 

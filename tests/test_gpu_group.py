@@ -479,6 +479,63 @@ def test_a_nan_query_stays_in_its_row(cuda, devbuf, act):
     s.close()
 
 
+NON_FINITE = [  # old lengths, new tokens, prefix, heads, kv heads, head_dim
+    ([0, 100], [300, 40], 70, 8, 2, 128),                    # pairs of row tiles, sequences joined with the prefix
+    ([60], [700], None, 2, 2, 64),                           # 256 tokens an item
+    ([5, 5, 5, 5, 5, 5], [70] * 6, 9000, 16, 4, 128),        # the prefix shared
+    ([5000], [200], 300, 6, 2, 128),                         # an item over several CTAs, or in pieces
+    ([3, 126, 255, 0], [2, 2, 1, 2], 40, 8, 2, 128),         # few rows
+    ([125, 9000], [3, 3], None, 6, 2, 64),
+]
+
+
+@pytest.mark.parametrize("act", [F32, BF16])
+@pytest.mark.parametrize("case", range(len(NON_FINITE)))
+def test_non_finite_values_reach_only_who_sees_them(cuda, devbuf, case, act):
+    """NaN and infinities among a call's own V: queries before them are as if they
+    were not there, those that see them have something non-finite in their dims and
+    in no others: exactly the sum with bf16 activations."""
+    old, new, P, nh, nkv, hd = NON_FINITE[case]
+    s = Setup(cuda, old, [n + 3 for n in new], P, nh, nkv, hd, act, seed=90 + case)
+    total = sum(new)
+    (qb, q), (kb, k), (vb, v) = s.new(total)
+    bad = np.zeros_like(v)
+    at = 0
+    for i, t in enumerate(new):
+        bad[at + t - 1, (3 * i + 1) % s.kvd] = np.nan
+        bad[at + t // 2, [5, 9, s.kvd - 1]] = np.inf, -np.inf, np.inf
+        bad[at + (3 * t) // 4, [9, 7]] = np.inf, -np.inf      # dim 9 gets both infinities
+        if t > 64:
+            bad[at + 33, s.kvd // 2:] = np.inf                # half a row
+        at += t
+    raw = np.where(bad != 0, bad, v).astype(np.float32)
+    clean = np.where(bad != 0, 0, v)
+    s.grow(new, k, clean)
+    qd, kd, vd = devbuf(qb), devbuf(kb), devbuf(bf16(raw)[0] if act == BF16 else raw)
+    od = devbuf(nbytes=qb.nbytes)
+    for again in (False, True):                               # with the rows appended, then as they lie there
+        tgkv.check(cuda.tg_kv_group_prompt(s.g, (C.c_uint32 * len(new))(*new), qd.ptr, None if again else kd.ptr,
+                                           None if again else vd.ptr, od.ptr, None), cuda)
+        assert cuda.tg_cuda_kv_sync(None)
+        got, (want, tol) = s.read(od, total), s.expect(q, new)
+        at = 0
+        for t in new:
+            with np.errstate(invalid="ignore"):
+                add = np.cumsum(bad[at:at + t], 0).reshape(t, nkv, hd).repeat(nh // nkv, 1)
+                want[at:at + t] += add
+            at += t
+        fin = np.isfinite(want)
+        assert (np.abs(got[fin] - want[fin]) <= tol[fin]).all()
+        if act == BF16:
+            assert np.array_equal(got[~fin], want[~fin], equal_nan=True)
+        else:
+            # a weight enters as hi + lo parts, and lo is often 0 or below it: 0 x Inf and Inf - Inf
+            # are NaN, so an infinity that a whole item sees may come out as NaN
+            assert not np.isfinite(got[~fin]).any()
+        assert cuda.tg_cuda_kv_device_error() == 0
+    s.close()
+
+
 def test_refusals_change_nothing(cuda, devbuf):
     lib = cuda
     mk = lambda cap=64, nkv=2, hd=64, dt=BF16: lib.tg_kv_create_ex(cap, nkv, hd, dt)  # noqa: E731

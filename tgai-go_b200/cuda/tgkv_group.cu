@@ -23,10 +23,11 @@
 // A tile with at most 64 rows is one half.
 // Bound, long prompts: a stream's chain scores - softmax - product, about 2150
 // cycles per 128 rows x 128 positions of 128 dims against 1024 of the tensor core
-// alone.  4 prompts of 2000 tokens behind 2048 (32/8 heads of 128): 490 us, 816
-// TFLOP/s with bf16 activations, 726 us with fp32 ones.  Measured slower in the
-// first case: both halves' scores at once (584 us), the streams' softmax in strict
-// turns (563 us), one thread watching both streams' barriers (728 us).
+// alone.  4 prompts of 2000 tokens behind 2048 (32/8 heads of 128): 501 us, 797
+// TFLOP/s with bf16 activations, 733 us with fp32 ones.  Measured slower in the
+// first case (at 490 us): both halves' scores at once (584 us), the streams' softmax in strict
+// turns (563 us), one thread watching both streams' barriers (728 us), sixteen
+// softmax warps, two threads a row (649 us).
 // Warps (384 threads): 0-3 and 4-7 the streams' softmax, 8 TMA (K/V tiles in
 // 64-dim boxes, 128-byte swizzle, into two rings that run ahead over the whole
 // stretch; Q of bf16 calls), 9 and 10 the streams' MMAs (one lane each).
@@ -179,6 +180,7 @@ __device__ __forceinline__ void run(const TGKvGroupParams& p, uint32_t cta_index
     const uint32_t sbase = smem_addr(base);
     uint64_t* bar = reinterpret_cast<uint64_t*>(base + C::OFF_BAR);
     uint32_t* tslot = reinterpret_cast<uint32_t*>(base + C::OFF_SLOT);
+    volatile uint32_t* flag = tslot + 1;         // some value of V was not finite (clear_unseen)
     uint32_t* tok0 = reinterpret_cast<uint32_t*>(base + C::OFF_TAB);
     uint32_t* old_len = tok0 + p.n_seq + 1;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -186,6 +188,7 @@ __device__ __forceinline__ void run(const TGKvGroupParams& p, uint32_t cta_index
     copy_table(tok0, p.tok0, p.n_seq + 1, tid, kThreads);
     copy_table(old_len, p.old_len, p.n_seq, tid, kThreads);
     if (tid == 0) {
+        *flag = 0;
         for (int i = 0; i < C::kStages; ++i) {
             mbar_init(&bar[C::B_KFULL + i], 1);
             mbar_init(&bar[C::B_KEMPTY + i], 2);
@@ -378,7 +381,8 @@ __device__ __forceinline__ void run(const TGKvGroupParams& p, uint32_t cta_index
             const uint32_t ntok = min(sh.tpt, left - tb);
             const bool valid = rtok < ntok;
             const bool busy = (uint32_t)(quarter * 32) < ntok * G;            // the warp has rows
-            const uint32_t own_min = seq ? old_len[seq - 1] + t0 + tb + 1 : 0;   // rows the stream's first token sees
+            const uint32_t own_first = seq ? old_len[seq - 1] + t0 + 1 : 0;      // rows the item's first token sees
+            const uint32_t own_min = seq ? own_first + tb : 0;                   // the stream's first token
             const uint32_t own_mine = own_min + min(rtok, ntok - 1);             // rows this thread's token sees
             const uint64_t row = (uint64_t)((seq ? tok0[seq - 1] : 0) + t0 + tb + rtok) * p.n_heads + pc.at.kvh * G + sub;
             const uint32_t tiles = pc.j1 - pc.j0, steps = wide ? 2 * tiles : tiles;
@@ -399,25 +403,22 @@ __device__ __forceinline__ void run(const TGKvGroupParams& p, uint32_t cta_index
                 const int lim = (int)((pr.own(j) ? own_mine : p.prefix_len) - pr.pos(j));      // that this thread's sees
                 const bool mask = (int)all < kPos;
                 const uint32_t halves = rows > kSub ? 2 : 1;
+                // of the tile, that every query of the item sees
+                const uint32_t lo = pr.own(j) ? (uint32_t)max((int)(own_first - pr.pos(j)), 0) : rows;
 #pragma unroll 1
                 for (uint32_t b = 0; b < 2; ++b) {
                     const uint32_t tsb = ts + b * 64u;
                     const int lm = lim - (int)(b * kSub);
                     if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&bar[C::B_SFULL + 2 * h + b], n & 1u));
-                    if (ok && b == 0 && rows < kPos) {
-                        // V rows that no query of the item sees may hold anything; P is 0 there, but
-                        // 0 * Inf is NaN, so they are cleared before this stream's PV reads them (in
-                        // wide pieces by both streams: either may be first).  Only after this S is
-                        // there has the stage's last tile been used, so that the parity means this
-                        // tile.
+                    if (ok && b == 0 && lo < kPos) {
+                        // V rows that no query of the item sees may hold anything, and those that only
+                        // some see are cleared of what is not finite, before this stream's PV reads
+                        // them (in wide pieces by both streams: either may be first).  Only after
+                        // this S is there has the stage's last tile been used, so that the parity
+                        // means this tile.
                         const uint32_t g = g0 + t, s = g % C::kStages;
                         ok = __all_sync(0xffffffffu, mbar_wait(&bar[C::B_VFULL + s], (g / C::kStages) & 1u));
-                        if (ok)
-                            for (uint32_t y = rows + ((uint32_t)r >> 3); y < kPos; y += 16)
-#pragma unroll
-                                for (int c = 0; c < HD / 64; ++c)
-                                    *reinterpret_cast<uint4*>(base + C::OFF_V + s * C::kTile + c * kBlock + y * 128 +
-                                                              (r & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
+                        if (ok) clear_unseen<HD>(base + C::OFF_V + s * C::kTile, lo, rows, r, flag);
                         __syncwarp();
                         fence_proxy_async_smem();
                     }
@@ -599,6 +600,20 @@ __device__ __forceinline__ void run(const TGKvGroupParams& p, uint32_t cta_index
                     }
                 }
                 if (valid && !whole && (wide || h == 0)) *slot_ml = make_float2(msc, l);
+                if (__any_sync(0xffffffffu, *flag != 0) && valid && seq) {
+                    // what the piece's V rows hold that is not finite, of those this row sees
+                    const uint32_t f0 = pr.own(pc.j0) ? pr.pos(pc.j0) : 0u, f1 = pr.own(pc.j1) ? pr.pos(pc.j1) : 0u;
+#pragma unroll 1
+                    for (int d = c0 * 16; d < c1 * 16; ++d) {
+                        const float x = cache_non_finite(p.table + (seq - 1), p.n_kv_heads * HD, pc.at.kvh * HD + d,
+                                                         max(own_first, f0), min(own_mine, f1));
+                        if (x == 0.f) continue;
+                        if (!whole) p.part_o[slot * HD + d] += x;
+                        else if constexpr (TERMS == 2) reinterpret_cast<float*>(p.out)[row * HD + d] += x;
+                        else reinterpret_cast<uint16_t*>(p.out)[row * HD + d] =
+                            (uint16_t)(cvt_bf16x2(lo_f(reinterpret_cast<uint16_t*>(p.out)[row * HD + d]) + x, 0.f) & 0xffffu);
+                    }
+                }
             }
             if (!wide) {
                 // the other stream has read this one's O and (m, l), and both the slot's rows are written

@@ -110,6 +110,7 @@ __device__ __forceinline__ void run(const TGKvGroupParams& p, uint32_t cta_index
     const uint32_t sbase = smem_addr(base);
     uint64_t* bar = reinterpret_cast<uint64_t*>(base + C::OFF_BAR);
     uint32_t* tslot = reinterpret_cast<uint32_t*>(base + C::OFF_SLOT);
+    volatile uint32_t* flag = tslot + 1;         // some value of V was not finite (clear_unseen)
     uint32_t* tok0 = reinterpret_cast<uint32_t*>(base + C::OFF_TAB);
     uint32_t* old_len = tok0 + p.n_seq + 1;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -117,6 +118,7 @@ __device__ __forceinline__ void run(const TGKvGroupParams& p, uint32_t cta_index
     copy_table(tok0, p.tok0, p.n_seq + 1, tid, kThreads);
     copy_table(old_len, p.old_len, p.n_seq, tid, kThreads);
     if (tid == 0) {
+        *flag = 0;
         for (int i = 0; i < C::kStages; ++i) {
             mbar_init(&bar[C::B_KFULL + i], 1);
             mbar_init(&bar[C::B_KEMPTY + i], 2);
@@ -356,17 +358,13 @@ __device__ __forceinline__ void run(const TGKvGroupParams& p, uint32_t cta_index
                 const bool own = pr.own(j);
                 const int first = (int)((own ? own_min : p.prefix_len) - pos);           // of the tile, that token 0 sees
                 if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&bar[C::B_SFULL + h], n & 1u));
-                if (ok && rows < kPos) {
-                    // V rows that no query sees may hold anything; P is 0 there, but 0 * Inf is NaN,
-                    // so they are cleared before PV reads them
+                const uint32_t lo = (uint32_t)max(first, 0);
+                if (ok && lo < kPos) {
+                    // V rows that no query sees may hold anything, and those that only some see are
+                    // cleared of what is not finite, before PV reads them
                     const uint32_t g = g0 + k, s = g % C::kStages;
                     ok = __all_sync(0xffffffffu, mbar_wait(&bar[C::B_VFULL + s], (g / C::kStages) & 1u));
-                    if (ok)
-                        for (uint32_t y = rows + ((uint32_t)r >> 3); y < kPos; y += 16)
-#pragma unroll
-                            for (int c = 0; c < HD / 64; ++c)
-                                *reinterpret_cast<uint4*>(base + C::OFF_V + s * C::kTile + c * kBlock + y * 128 +
-                                                          (r & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
+                    if (ok) clear_unseen<HD>(base + C::OFF_V + s * C::kTile, lo, rows, r, flag);
                     __syncwarp();
                 }
                 uint32_t v[N];
@@ -474,6 +472,13 @@ __device__ __forceinline__ void run(const TGKvGroupParams& p, uint32_t cta_index
                 float L = wa * ((ra[0] + ra[16]) + (ra[32] + ra[48])) + wb * ((ra[64] + ra[80]) + (ra[96] + ra[112]));
                 // (a stream that had no tile left O^T as it was)
                 float o = (wa == 0.f ? 0.f : a * wa) + (wb == 0.f ? 0.f : b * wb);
+                if (*flag && seq && r < HD) {
+                    // what the piece's V rows hold that is not finite, of those the row sees
+                    const uint32_t f0 = pr.own(cur.j0) ? pr.pos(cur.j0) : 0u, f1 = pr.own(cur.j1) ? pr.pos(cur.j1) : 0u;
+                    const float y = cache_non_finite(p.table + (seq - 1), p.n_kv_heads * HD, cur.at.kvh * HD + r,
+                                                     max(own_min, f0), min(own_min + x / G, f1));
+                    if (y != 0.f) o += y;
+                }
                 const uint64_t row = row_of(row0, x, pr.tokens);
                 const uint64_t slot = cur.first > 0 || !p.share ? cta + x : (seq ? total_rows : 0u) + row;
                 if (again) {
