@@ -18,7 +18,8 @@
  * scratch (about 59 MB at head_dim 128, half of it at 64) is shared by its
  * calls: order calls and graph replays that use one group (or one of its caches,
  * the prefix's rows included while they change) on one stream or with events.
- * Calls of different groups may overlap.  Device waits are bounded; one that runs
+ * Calls of different groups may overlap.  A group's caches, and those of a fork or
+ * compaction, lie on the current device.  Device waits are bounded; one that runs
  * out leaves the call's output undefined and shows in tg_cuda_kv_device_error().
  */
 #ifndef TGAI_KV_GROUP_H

@@ -582,6 +582,17 @@ def test_refusals_change_nothing(cuda, devbuf):
     assert lib.tg_kv_compact(arr(a), 1, u(59), u(2), 1, None) == 0 and b"beyond length 60" in err()
     assert lib.tg_kv_compact(arr(a), 1, u(5, 6), u(2, 2), 2, None) == 0 and b"out of order" in err()
     assert [lib.tg_kv_len(c) for c in (a, b, p, tiny)] == [60, 60, 60, 0]
+    # a cache of another device (by what its record says; nothing runs): the record's seventh word
+    device = C.c_int32.from_address(b + 24)
+    assert device.value == lib.tg_cuda_kv_device()
+    device.value += 1
+    assert not lib.tg_kv_group_create(None, arr(a, b), 2, 4, F32) and b"cache 1 lies on device" in err()
+    assert not lib.tg_kv_group_create(b, arr(a), 1, 4, F32) and b"prefix: cache 0 lies on device" in err()
+    assert lib.tg_kv_fork(arr(a), 1, arr(b), 1, 3, None) == 0 and b"copies: cache 0 lies on device" in err()
+    assert lib.tg_kv_fork(arr(b), 1, arr(a), 1, 3, None) == 0 and b"lies on device" in err()
+    assert lib.tg_kv_compact(arr(a, b), 2, u(0), u(1), 1, None) == 0 and b"cache 1 lies on device" in err()
+    device.value -= 1
+    assert [lib.tg_kv_len(c) for c in (a, b, p, tiny)] == [60, 60, 60, 0]
     lib.tg_kv_group_destroy(g)
     for c in (a, b, p, f32, other, wide, hd32, tiny):
         lib.tg_kv_destroy(c)

@@ -82,6 +82,7 @@ TGKvCache* tg_kv_create_ex(uint32_t max_seq, uint32_t n_kv_heads, uint32_t head_
         free(c);
         return NULL;
     }
+    c->device = tg_cuda_kv_device();
     c->host = (float*)(b->map ? b->map(c->dev) : NULL);
     if (tg_cuda_kv_attn_supported(dtype, head_dim)) {
         c->tmap = tg_cuda_kv_tmap_create(dtype, (uint64_t)(uintptr_t)c->dev, max_seq, n_kv_heads,

@@ -55,6 +55,18 @@ static int same_geometry(const TGKvCache* a, const TGKvCache* b) {
     return a->n_kv_heads == b->n_kv_heads && a->head_dim == b->head_dim && a->dtype == b->dtype;
 }
 
+/* The cuda backend, and caches that lie on the current device. */
+static int on_device(const char* what, TGKvCache* const* v, uint32_t n) {
+    if (!on_cuda(what)) return 0;
+    const int dev = tg_cuda_kv_device();
+    for (uint32_t i = 0; i < n; i++)
+        if (v[i]->device != dev) {
+            set_err("%s: cache %u lies on device %d, called on device %d", what, i, v[i]->device, dev);
+            return 0;
+        }
+    return 1;
+}
+
 /* ---- groups --------------------------------------------------------------- */
 struct TGKvGroup {
     uint32_t n, n_heads;
@@ -101,7 +113,8 @@ TGKvGroup* tg_kv_group_create(TGKvCache* prefix, TGKvCache* const* caches, uint3
         set_err("group: a cache appears twice");
         return NULL;
     }
-    if (!on_cuda("group")) return NULL;
+    if (!on_device("group", caches, n)) return NULL;
+    if (prefix && !on_device("group: prefix", &prefix, 1)) return NULL;
     TGKvGroup* g = (TGKvGroup*)calloc(1, sizeof(TGKvGroup));
     TGCudaRowCache* table = (TGCudaRowCache*)calloc((size_t)n + 1, sizeof(TGCudaRowCache));
     if (g) {
@@ -259,7 +272,7 @@ int tg_kv_fork(TGKvCache* const* src, uint32_t n_src, TGKvCache* const* dst, uin
         }
     for (uint32_t i = 0; i < n_dst; i++)
         if (n_rows > dst[i]->max_seq) { set_err("fork: capacity exceeded at copy %u", i); return 0; }
-    if (!on_cuda("fork")) return 0;
+    if (!on_device("fork", src, n_src) || !on_device("fork: copies", dst, n_dst)) return 0;
     TGCudaRowCache s[TGKV_GROUP_MAX], d[TGKV_GROUP_MAX];
     for (uint32_t i = 0; i < n_src; i++) s[i] = row_cache(src[i]);
     for (uint32_t i = 0; i < n_dst; i++) d[i] = row_cache(dst[i]);
@@ -296,7 +309,7 @@ int tg_kv_compact(TGKvCache* const* caches, uint32_t n, const uint32_t* start,
         end = (uint64_t)start[r] + count[r];
         keep += count[r];
     }
-    if (!on_cuda("compact")) return 0;
+    if (!on_device("compact", caches, n)) return 0;
     TGCudaRowCache t[TGKV_GROUP_MAX];
     for (uint32_t i = 0; i < n; i++) t[i] = row_cache(caches[i]);
     if (!tg_cuda_kv_compact_rows(t, n, (uint64_t)caches[0]->kv_dim * caches[0]->esize, start, count,

@@ -12,6 +12,7 @@ struct TGKvCache {
     uint32_t max_seq, n_kv_heads, head_dim, kv_dim;
     int      dtype;
     uint32_t esize;
+    int      device;              /* that was current at create: dev lies there */
     size_t   bytes;               /* 2 * max_seq * kv_dim * esize */
     void*    dev;                 /* device address of the buffer */
     float*   host;                /* always NULL (not mappable) */
