@@ -23,14 +23,15 @@
 // A tile with at most 64 rows is one half.
 // Bound, long prompts: a stream's chain scores - softmax - product, about 2150
 // cycles per 128 rows x 128 positions of 128 dims against 1024 of the tensor core
-// alone.  4 prompts of 2000 tokens behind 2048 (32/8 heads of 128): 501 us, 797
-// TFLOP/s with bf16 activations, 733 us with fp32 ones.  Measured slower in the
-// first case (at 490 us): both halves' scores at once (584 us), the streams' softmax in strict
+// alone.  4 prompts of 2000 tokens behind 2048 (32/8 heads of 128): 490 us, 815
+// TFLOP/s with bf16 activations, 711 us with fp32 ones.  Measured slower in the
+// first case: both halves' scores at once (584 us), the streams' softmax in strict
 // turns (563 us), one thread watching both streams' barriers (728 us), sixteen
 // softmax warps, two threads a row (649 us).
 // Warps (384 threads): 0-3 and 4-7 the streams' softmax, 8 TMA (K/V tiles in
 // 64-dim boxes, 128-byte swizzle, into two rings that run ahead over the whole
-// stretch; Q of bf16 calls), 9 and 10 the streams' MMAs (one lane each).
+// stretch; Q of bf16 calls), 9 and 10 the streams' MMAs (one lane each), 11 clears
+// unseen rows of V tiles.
 // TERMS is the number of bf16 terms of q and P: 1 with bf16 activations (q is
 // exact, P is rounded once, 2^-8 of a weight, as the output itself is), 2 with
 // fp32 ones (hi + lo, 16 mantissa bits; a third term of P has no room in the
@@ -75,12 +76,13 @@ struct Cfg {
     static constexpr int B_PVDONE = B_PFULL + 4;     // its PV is complete
     static constexpr int B_QFULL = B_PVDONE + 4;      // a piece's Q is in shared memory
     static constexpr int B_QEMPTY = B_QFULL + 1;     // every S of a piece is complete
-    static constexpr uint32_t OFF_ML = OFF_BAR + 32 * 8;               // [2 streams][128] (m, l)
+    static constexpr uint32_t OFF_ML = OFF_BAR + 40 * 8;               // [2 streams][128] (m, l)
     static constexpr uint32_t OFF_SLOT = OFF_ML + 2 * kRows * 8;
     static constexpr uint32_t OFF_TAB = OFF_SLOT + 16;                 // tok0, old_len
     static constexpr uint32_t OFF_STG = (OFF_TAB + (2 * TGKV_MAX_ITEMS + 1) * 4 + 127) / 128 * 128;
     static constexpr uint32_t SMEM = OFF_STG + 8 * 2048 + 1024;        // 2 KB per softmax warp; slack: alignment
-    static_assert(B_QEMPTY < 32 && SMEM <= 232448, "shared memory per CTA");
+    static constexpr int B_VREADY = B_QEMPTY + 1;    // a V tile's unseen rows are cleared
+    static_assert(B_VREADY + kStages <= 40 && SMEM <= 232448, "shared memory per CTA");
 };
 
 // The two warps (streams 0 and 1) of a TMEM lane quarter.
@@ -194,6 +196,7 @@ __device__ __forceinline__ void run(const TGKvGroupParams& p, uint32_t cta_index
             mbar_init(&bar[C::B_KEMPTY + i], 2);
             mbar_init(&bar[C::B_VFULL + i], 1);
             mbar_init(&bar[C::B_VEMPTY + i], 2);
+            mbar_init(&bar[C::B_VREADY + i], 1);
         }
         for (int i = 0; i < 4; ++i) {
             mbar_init(&bar[C::B_SFULL + i], 1);
@@ -333,7 +336,8 @@ __device__ __forceinline__ void run(const TGKvGroupParams& p, uint32_t cta_index
                     const uint64_t vd = umma_desc_sw128(sbase + C::OFF_V + s * C::kTile, kBlock, 1024);
                     for (uint32_t b = 0; ok && b < 2; ++b) {
                         ok = mbar_wait(&bar[C::B_PFULL + 2 * h + b], n & 1u) &&
-                             (b || mbar_wait(&bar[C::B_VFULL + s], (g / C::kStages) & 1u));
+                             (b || (mbar_wait(&bar[C::B_VFULL + s], (g / C::kStages) & 1u) &&
+                                    mbar_wait(&bar[C::B_VREADY + s], (g / C::kStages) & 1u)));
                         if (!ok) break;
                         tc_fence_after();
                         if (b < halves)
@@ -358,6 +362,28 @@ __device__ __forceinline__ void run(const TGKvGroupParams& p, uint32_t cta_index
                 pass(C::B_VFULL, C::B_VEMPTY, vs, g0);
             }
             if (!ok) atomicExch(p.err, kErrTimeout);
+        } else if (warp == kMmaWarp + 2) {
+            // V rows that no query of the item sees may hold anything; P is 0 there, but 0 * Inf is
+            // NaN, so they are cleared, and those that only some see are cleared of what is not
+            // finite, before a PV reads the tile (a stage's next tile comes after that PV)
+            uint32_t g = 0;
+            bool ok = true;
+            for (; ok && pc.more(); pc.next(sh, kMost)) {
+                const PieceRows pr(sh, pc, TERMS);
+                const uint32_t first = pc.at.seq ? old_len[pc.at.seq - 1] + pc.at.at * sh.item_tokens + 1 : 0;   // token 0 sees
+                for (uint32_t j = pc.j0; ok && j < pc.j1; ++j, ++g) {
+                    const uint32_t rows = pr.rows(j) - pr.pos(j), s = g % C::kStages;
+                    const uint32_t lo = pr.own(j) ? (uint32_t)max((int)(first - pr.pos(j)), 0) : rows;
+                    ok = __all_sync(0xffffffffu, mbar_wait(&bar[C::B_VFULL + s], (g / C::kStages) & 1u));
+                    if (ok && lo < kPos) {
+                        clear_unseen<HD, 32>(base + C::OFF_V + s * C::kTile, lo, rows, rows > kSub ? kPos : kSub, lane, flag);
+                        fence_proxy_async_smem();
+                        __syncwarp();
+                    }
+                    if (ok && lane == 0) mbar_arrive(&bar[C::B_VREADY + s]);
+                }
+            }
+            if (!ok && lane == 0) atomicExch(p.err, kErrTimeout);
         }
         __syncwarp();
     } else {
@@ -368,7 +394,7 @@ __device__ __forceinline__ void run(const TGKvGroupParams& p, uint32_t cta_index
         const float scale = p.qscale;
         const uint32_t rtok = (uint32_t)r / G, sub = (uint32_t)r % G;
         const uint32_t total_rows = tok0[p.n_seq] * p.n_heads;
-        uint32_t g0 = 0, it = 0, n = 0;          // K/V tiles of earlier pieces; pieces; this stream's steps
+        uint32_t it = 0, n = 0;                  // pieces; this stream's steps
         bool ok = true;
         // Both warps of a pair meet at named barriers, so neither leaves early:
         // after a failed wait a warp only keeps the barriers' counts.
@@ -403,25 +429,11 @@ __device__ __forceinline__ void run(const TGKvGroupParams& p, uint32_t cta_index
                 const int lim = (int)((pr.own(j) ? own_mine : p.prefix_len) - pr.pos(j));      // that this thread's sees
                 const bool mask = (int)all < kPos;
                 const uint32_t halves = rows > kSub ? 2 : 1;
-                // of the tile, that every query of the item sees
-                const uint32_t lo = pr.own(j) ? (uint32_t)max((int)(own_first - pr.pos(j)), 0) : rows;
 #pragma unroll 1
                 for (uint32_t b = 0; b < 2; ++b) {
                     const uint32_t tsb = ts + b * 64u;
                     const int lm = lim - (int)(b * kSub);
                     if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&bar[C::B_SFULL + 2 * h + b], n & 1u));
-                    if (ok && b == 0 && lo < kPos) {
-                        // V rows that no query of the item sees may hold anything, and those that only
-                        // some see are cleared of what is not finite, before this stream's PV reads
-                        // them (in wide pieces by both streams: either may be first).  Only after
-                        // this S is there has the stage's last tile been used, so that the parity
-                        // means this tile.
-                        const uint32_t g = g0 + t, s = g % C::kStages;
-                        ok = __all_sync(0xffffffffu, mbar_wait(&bar[C::B_VFULL + s], (g / C::kStages) & 1u));
-                        if (ok) clear_unseen<HD>(base + C::OFF_V + s * C::kTile, lo, rows, r, flag);
-                        __syncwarp();
-                        fence_proxy_async_smem();
-                    }
                     if (ok && busy && b < halves) {
                         tc_fence_after();
                         uint32_t va[32], vb[32];
@@ -471,7 +483,6 @@ __device__ __forceinline__ void run(const TGKvGroupParams& p, uint32_t cta_index
                 }
                 ++n;
             }
-            g0 += tiles;
 
             // ---- the piece's rows: out, or a partial
             const bool mine = (uint32_t)h < steps;                               // this stream had a tile

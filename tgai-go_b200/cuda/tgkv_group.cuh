@@ -130,7 +130,8 @@ __device__ __forceinline__ void tmem_wait_ld16(uint32_t (&r)[16]) {
 // other, though 0 x Inf is NaN: among the rows that only some queries of an item see,
 // such values are cleared in the tile, and their sum is added to the results of
 // those that do see them (cache_non_finite, off the usual path).  Looking for them
-// takes 2 % of the time of prompts of 2000 tokens, 3 % of ragged ones of up to 1000.
+// took 2 % of the time of prompts of 2000 tokens, 8 % of ragged ones of up to 1000,
+// while it was the softmax threads' work; a warp of its own ahead of them leaves 0 and 3 %.
 __device__ __forceinline__ uint32_t non_finite_bits(uint4 v) {                 // 0x80008000: some
     constexpr uint32_t e = 0x7f807f80u, one = 0x00800080u;
     return ((v.x & e) + one) | ((v.y & e) + one) | ((v.z & e) + one) | ((v.w & e) + one);
@@ -140,27 +141,22 @@ __device__ __forceinline__ uint32_t clear_non_finite(uint32_t w) {
     if ((w & 0x7f800000u) == 0x7f800000u) w &= 0xffffu;
     return w;
 }
-// Rows [lo, 128) of a V tile in shared memory, HD / 64 boxes, by 128 threads: those
-// behind `rows` are cleared whole, the others of what is not finite; *flag becomes 1
-// (before the first is cleared) if there was any.
-template <int HD>
-__device__ __forceinline__ void clear_unseen(unsigned char* tile, uint32_t lo, uint32_t rows, int r, volatile uint32_t* flag) {
+// Rows [lo, rows) of a V tile in shared memory, HD / 64 boxes, by THREADS threads: what
+// is not finite is cleared, and *flag becomes 1 if there was any.  (A call: the code of a
+// decode step, which has no such rows, stays short.)
+template <int HD, int THREADS>
+__device__ __noinline__ void clear_non_finite(unsigned char* tile, uint32_t lo, uint32_t rows, int r, volatile uint32_t* flag) {
     uint4* at = reinterpret_cast<uint4*>(tile) + (r & 7);
-    const uint32_t y0 = lo + ((uint32_t)r >> 3);
+    const uint32_t y0 = lo + ((uint32_t)r >> 3), y1 = min(rows, (uint32_t)kPos);
     uint32_t bits = 0;
-#pragma unroll 2
-    for (uint32_t y = y0; y < kPos; y += 16)
+#pragma unroll 4
+    for (uint32_t y = y0; y < y1; y += THREADS / 8)
 #pragma unroll
-        for (int c = 0; c < HD / 64; ++c) {
-            uint4* x = at + c * (kBlock / 16) + y * 8;
-            if (y >= rows) *x = make_uint4(0u, 0u, 0u, 0u);
-            else bits |= non_finite_bits(*x);
-        }
+        for (int c = 0; c < HD / 64; ++c) bits |= non_finite_bits(at[c * (kBlock / 16) + y * 8]);
     if (bits & 0x80008000u) {
         *flag = 1;
-        __threadfence_block();
 #pragma unroll 1
-        for (uint32_t y = y0; y < kPos && y < rows; y += 16)
+        for (uint32_t y = y0; y < y1; y += THREADS / 8)
 #pragma unroll 1
             for (int c = 0; c < HD / 64; ++c) {
                 uint4* x = at + c * (kBlock / 16) + y * 8;
@@ -168,7 +164,16 @@ __device__ __forceinline__ void clear_unseen(unsigned char* tile, uint32_t lo, u
                 *x = make_uint4(clear_non_finite(v.x), clear_non_finite(v.y), clear_non_finite(v.z), clear_non_finite(v.w));
             }
     }
-    __threadfence_block();                       // another stream's threads may have cleared what was read here
+}
+// Rows [rows, end) of the tile cleared whole, rows [lo, rows) of what is not finite.
+template <int HD, int THREADS>
+__device__ __forceinline__ void clear_unseen(unsigned char* tile, uint32_t lo, uint32_t rows, uint32_t end, int r,
+                                             volatile uint32_t* flag) {
+    for (uint32_t y = rows + ((uint32_t)r >> 3); y < end; y += THREADS / 8)
+#pragma unroll
+        for (int c = 0; c < HD / 64; ++c)
+            *reinterpret_cast<uint4*>(tile + c * kBlock + y * 128 + (r & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
+    if (lo < rows) clear_non_finite<HD, THREADS>(tile, lo, rows, r, flag);
 }
 // The sum of the values of V's column `col` that are not finite, rows [a, e) of a cache.
 __device__ __noinline__ float cache_non_finite(const TGKvRowCache* cache, uint32_t kv_dim, uint32_t col, uint32_t a, uint32_t e) {

@@ -364,7 +364,7 @@ __device__ __forceinline__ void run(const TGKvGroupParams& p, uint32_t cta_index
                     // cleared of what is not finite, before PV reads them
                     const uint32_t g = g0 + k, s = g % C::kStages;
                     ok = __all_sync(0xffffffffu, mbar_wait(&bar[C::B_VFULL + s], (g / C::kStages) & 1u));
-                    if (ok) clear_unseen<HD>(base + C::OFF_V + s * C::kTile, lo, rows, r, flag);
+                    if (ok) clear_unseen<HD, 128>(base + C::OFF_V + s * C::kTile, lo, rows, kPos, r, flag);
                     __syncwarp();
                 }
                 uint32_t v[N];
