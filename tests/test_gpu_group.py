@@ -536,6 +536,54 @@ def test_non_finite_values_reach_only_who_sees_them(cuda, devbuf, case, act):
     s.close()
 
 
+@pytest.mark.parametrize("as_prefix", [False, True])
+def test_offsets_past_32_bits(cuda, devbuf, as_prefix):
+    """Halves of 4.5 GB.  K is zero, so every weight is 1 and a result is the sum of the
+    few V rows that are not zero over the length: one rounding of the output, and the
+    division's."""
+    lib, nkv, hd, n = cuda, 8, 128, 2_200_000
+    kvd, cap, rng = nkv * hd, 2_200_001, np.random.default_rng(123)
+    mk = lambda cap: lib.tg_kv_create_ex(cap, nkv, hd, BF16)  # noqa: E731
+    big, copy, small = mk(cap), mk(cap), mk(8)
+    tgkv.check(big and copy and small, lib)
+    at = [0, 1, n // 2, n - 2, n - 1]
+    bits, v = bf16(rng.standard_normal((len(at), kvd)) * 2.0 ** 20)
+    row = lambda c, r, half=1: lib.tg_kv_device_handle(c) + (half * cap + r) * kvd * 2  # noqa: E731
+    for r, b in zip(at, bits):
+        assert lib.tg_cuda_kv_h2d(row(big, r), b.ctypes.data, b.nbytes, None)
+    lib.tg_kv_advance(big, n)
+    caches = (C.c_void_p * 1)(small if as_prefix else big)
+    g = lib.tg_kv_group_create(big if as_prefix else None, caches, 1, 16, BF16)
+    tgkv.check(g, lib)
+    new_bits, new = bf16(rng.standard_normal((1, kvd)) * 2.0 ** 20)
+    q, k = devbuf(bf16(rng.standard_normal((1, 16 * hd)))[0]), devbuf(np.zeros((1, kvd), np.uint16))
+    vd, od = devbuf(new_bits), devbuf(nbytes=16 * hd * 2)
+    tgkv.check(lib.tg_kv_group_decode(g, q.ptr, k.ptr, vd.ptr, od.ptr, None), lib)
+    assert lib.tg_cuda_kv_sync(None)
+    import oracle as O
+    got = O.bf16_to_f32(od.get(np.uint16, (nkv, 2, hd))).astype(np.float64)
+    want = ((v.sum(0) + new[0]) / (n + 1)).reshape(nkv, 1, hd)
+    mag = ((np.abs(v).sum(0) + np.abs(new[0])) / (n + 1)).reshape(nkv, 1, hd)
+    assert (np.abs(got - want) <= 2.0 ** -8 * np.abs(want) + 2.0 ** -20 * mag).all()
+    assert lib.tg_cuda_kv_device_error() == 0
+    if not as_prefix:
+        def read(c, r):
+            out = np.empty(kvd, np.uint16)
+            assert lib.tg_cuda_kv_d2h(out.ctypes.data, row(c, r), out.nbytes, None) and lib.tg_cuda_kv_sync(None)
+            return out
+        assert np.array_equal(read(big, n), new_bits[0])
+        tgkv.check(lib.tg_kv_fork((C.c_void_p * 1)(big), 1, (C.c_void_p * 1)(copy), 1, n + 1, None), lib)
+        every = list(zip(at + [n], np.concatenate([bits, new_bits])))
+        assert all(np.array_equal(read(copy, r), b) for r, b in every)
+        start, count = (C.c_uint32 * 3)(1, n // 2, n - 2), (C.c_uint32 * 3)(1, 1, 3)
+        tgkv.check(lib.tg_kv_compact((C.c_void_p * 1)(copy), 1, start, count, 3, None), lib)
+        assert lib.tg_kv_len(copy) == 5
+        assert all(np.array_equal(read(copy, i), b) for i, (_, b) in enumerate(every[1:]))
+    lib.tg_kv_group_destroy(g)
+    for c in (big, copy, small):
+        lib.tg_kv_destroy(c)
+
+
 def test_refusals_change_nothing(cuda, devbuf):
     lib = cuda
     mk = lambda cap=64, nkv=2, hd=64, dt=BF16: lib.tg_kv_create_ex(cap, nkv, hd, dt)  # noqa: E731
