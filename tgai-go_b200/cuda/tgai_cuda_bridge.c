@@ -1187,7 +1187,7 @@ static int plan_group(const TGCudaGroupCall* c, uint32_t sms, TGKvGroupParams* p
     const uint32_t light_tokens = (c->act == 1 ? TGKV_GROUP_LIGHT_ROWS : 10u) / g;
     const int own_light = longest <= light_tokens;
     /* An item's start and end take as long as this many of its tiles (measured at
-     * 1, 2, 3 and 5: 31 prompts of up to 1000 tokens 200, 202, 207, 214 us with bf16
+     * 1, 2, 3 and 5: 32 prompts of up to 1000 tokens 200, 202, 207, 214 us with bf16
      * activations, 531, 478, 450, 442 us with fp32 ones; decode over 64 caches of
      * 1000-4000 positions 114, 114, 113, 112 us and 131, 125, 123, 120 us). */
     TGKvGroupShape heavy = {p->n_seq, p->n_kv_heads, p->prefix_len, 0, tpt, c->act == 1 ? 2 * tpt : tpt,
