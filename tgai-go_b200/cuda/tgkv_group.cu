@@ -541,7 +541,9 @@ __device__ __forceinline__ void run(const TGKvGroupParams& p, uint32_t cta_index
                     dst[i] = __shfl_sync(0xffffffffu, mine_row, (lane >> 2) + 8 * i);
                     kp[i] = TERMS == 2 ? __shfl_sync(0xffffffffu, keep, (lane >> 2) + 8 * i) : 0.f;
                 }
-                const uint64_t cta_slot = (uint64_t)p.line[0].cta_rows + 512u * cta_index + 256u;   // a whole item's earlier sums
+                // the earlier sums are where the earlier pieces put them: a whole item's in this
+                // CTA's slots, consecutive rows for consecutive lanes
+                const uint64_t first_slot = slot - (uint32_t)lane;
                 auto flush = [&](const uint4 (&w)[4], unsigned char* out, uint32_t row_bytes, uint32_t off, bool add) {
 #pragma unroll
                     for (int q = 0; q < 4; ++q)
@@ -555,7 +557,7 @@ __device__ __forceinline__ void run(const TGKvGroupParams& p, uint32_t cta_index
                         if (TERMS == 2 && add) {
                             const float4 o = *reinterpret_cast<const float4*>(
                                 reinterpret_cast<const unsigned char*>(p.part_o) +
-                                (whole ? cta_slot + x : dst[i]) * row_bytes + off + part * 16);
+                                (whole ? first_slot + x : dst[i]) * row_bytes + off + part * 16);
                             y = make_uint4(__float_as_uint(fmaf(o.x, kp[i], __uint_as_float(y.x))),
                                            __float_as_uint(fmaf(o.y, kp[i], __uint_as_float(y.y))),
                                            __float_as_uint(fmaf(o.z, kp[i], __uint_as_float(y.z))),
