@@ -569,18 +569,18 @@ __device__ __forceinline__ void run(const TGKvGroupParams& p, uint32_t cta_index
                 };
                 // 16 columns of the row's sums (columns 16 c ..), joined and scaled
                 const uint32_t oa = wide ? to : lanes + TM_O;
+                // (a weight that is 0 takes part too: 0 x Inf is NaN, and the row sees it)
                 auto take = [&](int c, float (&o)[16]) {
-                    uint32_t x[16], y[16];
+                    uint32_t x[16];
                     tmem_ld16(oa + c * 16, x);
-                    if (!wide && steps > 1) {
-                        tmem_ld16(oa + 128 + c * 16, y);
-                        tmem_wait_ld16(y);
-                    }
                     tmem_wait_ld16(x);
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        o[i] = w0 == 0.f ? 0.f : __uint_as_float(x[i]) * w0;
-                        if (w1 != 0.f) o[i] = fmaf(__uint_as_float(y[i]), w1, o[i]);
+                    for (int i = 0; i < 16; ++i) o[i] = __uint_as_float(x[i]) * w0;
+                    if (!wide && steps > 1) {                                    // the other stream had a tile
+                        tmem_ld16(oa + 128 + c * 16, x);
+                        tmem_wait_ld16(x);
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) o[i] = fmaf(__uint_as_float(x[i]), w1, o[i]);
                     }
                 };
                 const int c0 = wide ? 0 : h * (HD / 32), c1 = wide ? HD / 16 : c0 + HD / 32;
@@ -689,7 +689,8 @@ struct Acc {
         float M = ml.x;
 #pragma unroll
         for (int w = 16; w >= 1; w >>= 1) M = max3(M, __shfl_xor_sync(0xffffffffu, M, w), m);
-        // (a part of which the row saw nothing has m = -inf and counts nothing)
+        // (a part of which the row saw nothing has m = -inf and sums of 0; one whose weight
+        // underflows takes part all the same, since 0 x Inf is NaN)
         const float w = ml.x == -INFINITY ? 0.f : ex2_approx(ml.x - M), a = m == -INFINITY ? 0.f : ex2_approx(m - M);
         float L = w * ml.y;
 #pragma unroll
@@ -704,14 +705,14 @@ struct Acc {
             const float* src = part_o + s * HD + lane * D;
             if constexpr (D == 4) {
                 const float4 v = *reinterpret_cast<const float4*>(src);
-                o[0] += wi == 0.f ? 0.f : wi * v.x;
-                o[1] += wi == 0.f ? 0.f : wi * v.y;
-                o[2] += wi == 0.f ? 0.f : wi * v.z;
-                o[3] += wi == 0.f ? 0.f : wi * v.w;
+                o[0] += wi * v.x;
+                o[1] += wi * v.y;
+                o[2] += wi * v.z;
+                o[3] += wi * v.w;
             } else {
                 const float2 v = *reinterpret_cast<const float2*>(src);
-                o[0] += wi == 0.f ? 0.f : wi * v.x;
-                o[1] += wi == 0.f ? 0.f : wi * v.y;
+                o[0] += wi * v.x;
+                o[1] += wi * v.y;
             }
         }
         m = M;

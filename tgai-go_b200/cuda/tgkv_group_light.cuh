@@ -470,8 +470,10 @@ __device__ __forceinline__ void run(const TGKvGroupParams& p, uint32_t cta_index
                 const float wa = ma == -INFINITY ? 0.f : ex2_approx(ma - M), wb = mb == -INFINITY ? 0.f : ex2_approx(mb - M);
                 const float* ra = red_all + x;
                 float L = wa * ((ra[0] + ra[16]) + (ra[32] + ra[48])) + wb * ((ra[64] + ra[80]) + (ra[96] + ra[112]));
-                // (a stream that had no tile left O^T as it was)
-                float o = (wa == 0.f ? 0.f : a * wa) + (wb == 0.f ? 0.f : b * wb);
+                // (a stream that had no tile left O^T as it was; a weight that is 0 takes part, since
+                // 0 x Inf is NaN)
+                float o = a * wa;
+                if (steps > 1) o += b * wb;
                 if (*flag && seq && r < HD) {
                     // what the piece's V rows hold that is not finite, of those the row sees
                     const uint32_t f0 = pr.own(cur.j0) ? pr.pos(cur.j0) : 0u, f1 = pr.own(cur.j1) ? pr.pos(cur.j1) : 0u;
@@ -485,7 +487,7 @@ __device__ __forceinline__ void run(const TGKvGroupParams& p, uint32_t cta_index
                     const float2 old = *reinterpret_cast<const float2*>(p.part_ml + slot * 2);
                     const float M2 = max3(M, old.x, M);
                     const float wn = M == -INFINITY ? 0.f : ex2_approx(M - M2), wo = old.x == -INFINITY ? 0.f : ex2_approx(old.x - M2);
-                    if (r < HD) o = o * wn + (wo == 0.f ? 0.f : p.part_o[slot * HD + r] * wo);
+                    if (r < HD) o = o * wn + p.part_o[slot * HD + r] * wo;
                     L = L * wn + old.y * wo;
                     M = M2;
                 }
