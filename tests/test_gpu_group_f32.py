@@ -1,4 +1,4 @@
-"""fp32 activations over long histories.
+"""fp32 activations: long histories, and what a head's row may be off by.
 
 A full row tile that sees more than 32 K/V tiles of 128 positions is worked in
 pieces of 32 tiles whose sums meet in the group's scratch.  The cases hold such
@@ -12,10 +12,12 @@ import pytest
 
 import tgkv
 from conftest import rel_head_err
+from group_model import bf16, reference
 from test_gpu_group import F32, Setup
 from test_group_host import plan
 
 C = tgkv.C
+FULL, FEW = 5e-5, 2e-6
 
 LONG = [  # old lengths, new tokens, prefix, heads, kv heads, head_dim; tiles that an item in one CTA passes
     ([4200], [1152], None, 16, 4, 128, 32),
@@ -72,5 +74,50 @@ def test_long_items(cuda, devbuf, case):
     got, want, tol = attend(s, devbuf, new)
     bad = ~(np.abs(got - want) <= tol)
     assert not bad.any(), (bad.mean(), np.argwhere(bad)[:5], got[bad][:5], want[bad][:5])
-    assert rel_head_err(got, want) < 5e-5
+    assert rel_head_err(got, want) < FULL
+    s.close()
+
+
+@pytest.mark.parametrize("terms,bound,holds", [(1, FULL, False), (2, FULL, True), (2, FEW, False), (3, FEW, True)])
+def test_bounds_tell_the_terms(terms, bound, holds):
+    """q and the weights as that many bf16 terms, all else in 64 bits."""
+    def rounded(x):
+        out, rest = np.zeros_like(x), x
+        for _ in range(terms):
+            t = bf16(rest)[1]
+            out, rest = out + t, rest - t
+        return out
+    rng = np.random.default_rng(terms)
+    got, want = [], []
+    for _ in range(24):                                      # heads
+        q, k, v = (rng.standard_normal((n, 128)).astype(np.float32).astype(np.float64) for n in (8, 400, 400))
+        want.append(reference(q, [(k, v)], 128 ** -0.5, False)[0])
+        w = rounded(np.exp(np.where(np.arange(400) <= 392 + np.arange(8)[:, None], rounded(q) @ k.T * 128 ** -0.5, -np.inf)))
+        got.append(w @ v / w.sum(1, keepdims=True))
+    assert (rel_head_err(np.array(got), np.array(want)) < bound) == holds
+
+
+BOUNDS = [  # old lengths, new tokens, prefix, heads, kv heads, head_dim; what of a head's row
+    ([390, 0, 127, 128], [1] * 4, None, 16, 4, 128, FEW),
+    ([100] * 40, [1] * 40, 250, 32, 8, 64, FEW),
+    ([7, 200, 380], [2, 2, 1], 0, 8, 2, 128, FEW),           # two tokens of four heads
+    ([380, 40, 3], [10, 0, 9], None, 4, 4, 64, FEW),
+    ([300, 0, 77], [200, 129, 11], None, 12, 4, 128, FULL),
+    ([10] * 12, [22, 9, 11, 4, 31, 8, 1, 1, 3, 5, 6, 7], 700, 16, 2, 64, FULL),
+    ([2000], [300], 500, 32, 8, 128, FULL),
+    ([17] * 40, [1] * 40, 4000, 6, 3, 64, FULL),             # the prefix on full row tiles, own rows on few
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("case", range(len(BOUNDS)))
+def test_a_head_row_within_its_bound(cuda, devbuf, case):
+    old, new, P, nh, nkv, hd, bound = BOUNDS[case]
+    starts = plan(cuda, old, new, P or 0, nh, nkv, F32, 148)[1]
+    assert (bound == FEW) == (not starts[0])                 # all of it on the kernel of few rows
+    s = Setup(cuda, old, [2 * n + 3 for n in new], P, nh, nkv, hd, F32, seed=170 + case)
+    for _ in range(2):
+        got, want, tol = attend(s, devbuf, new)
+        assert (np.abs(got - want) <= tol).all()
+        assert rel_head_err(got, want) < bound
     s.close()
