@@ -66,8 +66,6 @@ struct Pieces {
         at = tgkv_group_next_item(&s, at);
         set(s, most);
     }
-    // the last piece of the item in this CTA
-    __device__ bool last() const { return j1 == (tgkv_group_same_item(at, end) ? end.tile : nt); }
 
 private:
     __device__ void set(const TGKvGroupShape& s, uint32_t most) {
