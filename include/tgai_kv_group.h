@@ -71,8 +71,9 @@ int tg_kv_group_decode(TGKvGroup* g, const void* q, const void* k_new, const voi
  * ones: q and the weights enter as two bf16 terms (16 mantissa bits; within
  * 5e-5 of a head's output scale), or as three (24 bits) where no sequence has
  * more than 10 query rows per KV head (most decode steps' own rows).  Values of
- * K and V that are not finite reach the queries that see them and no others (with
- * fp32 activations an infinity of V as NaN where lo parts of weights meet it). */
+ * K and V that are not finite reach the queries that see them and no others (an
+ * infinity of V as NaN where a weight, or with fp32 activations a lo part of one,
+ * is 0). */
 int tg_kv_group_prompt(TGKvGroup* g, const uint32_t* n_new, const void* q, const void* k_new,
                        const void* v_new, void* out, void* stream);
 

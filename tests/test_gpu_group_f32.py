@@ -6,6 +6,22 @@ items whole in one CTA, by the plan for 148 SMs that a test without a device
 looks at; on the GPU every element is held against a plain 64-bit form within
 the roundings of group_model.py, and every head's row within the bound that
 tgai_kv_group.h states.
+
+group_model.py adds the roundings up as if all had one sign.  The bounds on a
+head's row (error over the row's largest value) let them average out, so that a
+lost term shows:
+  5e-5  full row tiles, q and weights as two bf16 terms.  A term is off by at most
+        half a step of 8 bits, so two by 2^-16, about 2^-19 on average (rms);
+        over the positions both roundings move an output by 1.4 * 2^-19 = 2.7e-6
+        of its rms, at worst of 10^5 outputs by 4.5 times that, and the truncated
+        fp32 sums (at most 128 steps of 16 positions, each for two terms, half a
+        step of 2^-23 of a sum that on average is half its end) by 7.7e-6.  One
+        term alone moves it by 2^-10.
+  2e-6  few rows, three terms (2^-24 at most), up to 400 positions: the scores'
+        sums and the exponential, 2^-21 of a weight, move an output by 4.8e-7 of
+        its rms, at worst by 4.5 times that, against a row maximum of at least
+        twice the rms; 16 steps of truncated sums by 6.4e-7: 1.8e-6 in all.  Two
+        terms alone move it by 2.7e-6 rms.
 """
 import numpy as np
 import pytest

@@ -21,13 +21,14 @@
 //                  shared memory bounds both), and here the other stream fills the
 //                  wait.
 // A tile with at most 64 rows is one half.
-// Bound, long prompts: a stream's chain scores - softmax - product, about 2150
-// cycles per 128 rows x 128 positions of 128 dims against 1024 of the tensor core
-// alone.  4 prompts of 2000 tokens behind 2048 (32/8 heads of 128): 490 us, 815
-// TFLOP/s with bf16 activations, 711 us with fp32 ones.  Measured slower in the
-// first case: both halves' scores at once (584 us), the streams' softmax in strict
-// turns (563 us), one thread watching both streams' barriers (728 us), sixteen
-// softmax warps, two threads a row (649 us).
+// Bound, long prompts: a stream's chain scores - softmax - product.  An SM takes
+// about 2400 cycles per 128 rows x 128 positions of 128 dims, the starts and ends of
+// items included; with two streams side by side that is about 4800 for a stream's
+// own, of which the tensor core has work for 1024.  4 prompts of 2000 tokens behind
+// 2048 (32/8 heads of 128): 488 us, 820 TFLOP/s with bf16 activations, 719 us with
+// fp32 ones.  Measured slower in the first case: both halves' scores at once (584
+// us), the streams' softmax in strict turns (563 us), one thread watching both
+// streams' barriers (728 us), sixteen softmax warps, two threads a row (649 us).
 // Warps (384 threads): 0-3 and 4-7 the streams' softmax, 8 TMA (K/V tiles in
 // 64-dim boxes, 128-byte swizzle, into two rings that run ahead over the whole
 // stretch; Q of bf16 calls), 9 and 10 the streams' MMAs (one lane each), 11 clears

@@ -9,8 +9,9 @@
 // streams take an item's alternate tiles, each with its own O^T, P^T and softmax
 // warps, and join at the item's end; K and V have three 32 KB stages each.
 // Decode without a prefix, 32/8 heads of 128, bf16 activations: 16 caches of
-// 30000-32000 positions 308 us (6.56 TB/s, the measured copy rate), 64 of
-// 1000-4000 110 us (5.7 TB/s).  Short items are bound by their start and end, so
+// 30000-32000 positions 292-308 us on different cards (6.6-6.9 TB/s, about the
+// measured copy rate), 64 of 1000-4000 107-110 us (5.7 TB/s); fp32 activations 307
+// and 113 us.  Short items are bound by their start and end, so
 // what runs once an item is kept small (unrolled code costs its fetch).
 // TERMS is 1 with bf16 activations; fp32 q and P enter as three bf16 terms (all 24
 // bits), stacked as columns: term t of row x is column t * ROWS + x.
